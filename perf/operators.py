@@ -187,7 +187,7 @@ def _run_own(state):
     small, lengths, sums, kept = kv8_evict(cache, state["lengths"], state["sums"], state["budget"], recent=state["recent"], sink=state["sink"],
                                            max_length=state["longest"])
     k, v = kv8_load(small, lengths, count=state["budget"])
-    return {"k": k, "v": v, "lengths": lengths, "sums": sums, "kept": kept}
+    return {"k": k, "v": v, "lengths": lengths, "sums": sums[..., : state["budget"]], "kept": kept}
 
 
 # ---- the plain forms -------------------------------------------------------------------------------------------------
