@@ -36,6 +36,7 @@ extern "C" {
                                 not ascending and disjoint, or marked columns without a vertical list; the affected
                                 row blocks are computed from the part of the plan read before the fault); bit 3: a
                                 range check of the debug build (-DMINF_BOUNDS) failed and the access was skipped */
+#define MINF_ERR_KV8_RANGE 16 /* MINF_ST_ERROR bit 4: a length or position outside its 8-bit cache (see minf_kv8_cache) */
 #define MINF_ST_NO_SLASH 1   /* number of row blocks whose slash list has no offset < end row */
 #define MINF_ST_AUX0 2        /* words 2-3, read as one uint64: 64x64 tile equivalents the attention kernel sent  */
 #define MINF_ST_AUX1 3        /* to the tensor pipe (its 128-row x 64/128-key steps), summed over launches         */
@@ -312,6 +313,85 @@ int minf_plan_count_tiles(const void* plan, int batch, int heads, int context_si
 /* The same for a plan built with minf_vs_build_plan_window. */
 int minf_plan_count_tiles_window(const void* plan, int batch, int heads, int q_pos0, int n_q,
                                  int cap_v, int cap_s, unsigned long long* tiles_out, void* stream);
+
+/*
+ * 8-bit key/value cache of one layer, for decoding after the sparse prefill (no counterpart in the reference, whose
+ * quantised cache is a 2-bit one of another package).
+ *   k, v              codes [batch, heads, capacity, 128], one byte each, contiguous, 16-byte aligned
+ *   k_scale, v_scale  fp32 [batch, heads, capacity / 64]: one scale for each block of 64 tokens of a head;
+ *                     value = code * scale
+ *   k_tail, v_tail    bf16 [batch, heads, 64, 128]: the tokens behind a sequence's last complete block, token t in
+ *                     row t % 64.  A block is quantised once, when its last token arrives.
+ *   status            int32 [MINF_STATUS_WORDS], zeroed by the caller once.  A length or position that does not fit
+ *                     sets MINF_ERR_KV8_RANGE in status[MINF_ST_ERROR]: lengths are clipped, and a sequence whose new
+ *                     tokens do not fit gets none of them.
+ * The scale of a block whose largest finite magnitude is m: the smallest power of two s with 448 s >= m (e4m3), or
+ * m / 127 rounded to fp32 (int8); at least 2^-100, and 1 for a block of zeros.  Codes are x / s rounded to nearest
+ * even; infinities become the largest code, NaN stays NaN in e4m3 and becomes 0 in int8.
+ * Where a call takes `lengths`, they are int32 [batch] on the device, or NULL when every sequence holds `length_all`
+ * tokens.  Calls on one cache must be ordered on one stream (or by events), as for any tensor.
+ */
+#define MINF_KV8_E4M3 0
+#define MINF_KV8_INT8 1
+typedef struct {
+    void* k;
+    void* v;
+    float* k_scale;
+    float* v_scale;
+    void* k_tail;
+    void* v_tail;
+    int32_t* status;
+    int32_t batch, heads, capacity, format;
+} minf_kv8_cache;
+
+/*
+ * Appends tokens: key / value bf16 [batch, heads, n_tokens, 128] (head_dim contiguous, 16-byte aligned, outer strides in
+ * multiples of 8 elements).  Sequence b holds start[b] (device; NULL: start_all) tokens before the call and gets the
+ * first counts[b] (device; NULL: n_tokens) of the new ones.
+ */
+int minf_kv8_store(
+    const minf_kv8_cache* cache, const void* key, const void* value, const int64_t k_strides[3], const int64_t v_strides[3],
+    int n_tokens, const int32_t* start, int start_all, const int32_t* counts, void* stream);
+
+/*
+ * Reads tokens first[b] (device; NULL: first_all) .. + count back: k_out / v_out bf16 [batch, heads, count, 128],
+ * contiguous, 16-byte aligned; zeros outside [0, length).
+ */
+int minf_kv8_load(
+    const minf_kv8_cache* cache, const int32_t* lengths, int length_all, const int32_t* first, int first_all, int count,
+    void* k_out, void* v_out, void* stream);
+
+/*
+ * Attention of the last n_q tokens of every sequence over the cache that holds them: query i of a sequence of n tokens
+ * sees the tokens before n - n_q + 1 + i.  q / o bf16 [batch, hq, n_q, 128] (head_dim contiguous); query head h reads
+ * cache head h / (hq / heads).  lse (optional, fp32 [batch, hq, n_q]) receives the base-2 log-sum-exp of the logits times
+ * sm_scale * log2(e).  A row that sees no token gives zeros and -inf.
+ * weights (optional, fp32 [batch, heads, >= max_length], tokens contiguous, strides in elements): the probabilities
+ * summed over the head's queries, plus add_to (NULL: zero; may be `weights` itself), for the tokens below the
+ * sequence's length; the others are not written.
+ * max_length bounds the lengths (capacity at most); longer ones are reported and clipped.
+ * scratch holds minf_kv8_attention_scratch_bytes() bytes, 16-byte aligned, whose content does not matter.
+ */
+size_t minf_kv8_attention_scratch_bytes(int batch, int hq, int heads, int n_q, int max_length, int with_weights);
+int minf_kv8_attention(
+    const minf_kv8_cache* cache, const void* q, const int64_t q_strides[3], void* o, const int64_t o_strides[3],
+    int hq, int n_q, const int32_t* lengths, int length_all, int max_length, float sm_scale, float* lse,
+    float* weights, const int64_t w_strides[2], const float* add_to, const int64_t add_strides[2],
+    void* scratch, void* stream);
+
+/*
+ * Eviction by accumulated attention weight: of a sequence of n > budget tokens every head keeps the first `sink`, the
+ * last `recent` and the budget - sink - recent others with the largest weights (of equal weights the earlier token; a
+ * NaN counts as the largest), in their order, and writes them into `dst` (another cache of the same format) as blocks
+ * quantised from their cached values.  A sequence of n <= budget tokens is copied.
+ * weights fp32 [batch, heads, >= max_length], tokens contiguous, strides in elements.  kept int32 [batch, heads, budget]:
+ * the tokens' old positions, ascending, -1 behind the last; weights_out fp32 [batch, heads, dst->capacity]: their
+ * weights, zeros behind the last; lengths_out int32 [batch].
+ */
+int minf_kv8_evict(
+    const minf_kv8_cache* src, const minf_kv8_cache* dst, const int32_t* lengths, int length_all, int max_length,
+    const float* weights, const int64_t w_strides[2], int budget, int recent, int sink,
+    int32_t* kept, float* weights_out, int32_t* lengths_out, void* stream);
 
 #ifdef __cplusplus
 }

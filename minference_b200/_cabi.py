@@ -20,11 +20,21 @@ LIB_PATH = os.environ.get("MINFER_B200_LIB") or os.path.join(_HERE, "libminfer_b
 
 STATUS_WORDS = 4
 ST_ERROR, ST_NO_SLASH = 0, 1
+ERR_KV8_RANGE = 16
 MODE_PLAN, MODE_ASHAPE = 0, 1
+KV8_E4M3, KV8_INT8 = 0, 1
 # (force_columns, force_diagonals, min_vertical, min_slash) of minf_vs_select
 SELECT_RULES = {"online": (30, 100, 30, 50), "static": (30, 30, 30, 50), "search": (30, 30, 0, 0)}
 
 _lib = None
+
+class Kv8Desc(ctypes.Structure):
+    """``minf_kv8_cache``: the pointers and sizes of one layer's 8-bit key/value cache."""
+    _fields_ = [(n, c_void_p) for n in ("k", "v", "k_scale", "v_scale", "k_tail", "v_tail", "status")] + \
+               [(n, c_int32) for n in ("batch", "heads", "capacity", "format")]
+
+
+_KV8 = POINTER(Kv8Desc)
 
 # name -> (restype, argtypes); must list every symbol of include/minfer_b200.h
 _I64x3 = POINTER(c_int64)
@@ -64,6 +74,12 @@ SIGNATURES = {
                                          [c_void_p] * 4 + [c_int, c_int] + [c_void_p, c_void_p]),
     "minf_plan_count_tiles": (c_int, [c_void_p] + [c_int] * 5 + [c_void_p, c_void_p]),
     "minf_plan_count_tiles_window": (c_int, [c_void_p] + [c_int] * 6 + [c_void_p, c_void_p]),
+    "minf_kv8_store": (c_int, [_KV8] + [c_void_p] * 2 + [_I64x3] * 2 + [c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "minf_kv8_load": (c_int, [_KV8, c_void_p, c_int, c_void_p, c_int, c_int] + [c_void_p] * 3),
+    "minf_kv8_attention_scratch_bytes": (c_size_t, [c_int] * 6),
+    "minf_kv8_attention": (c_int, [_KV8, c_void_p, _I64x3, c_void_p, _I64x3, c_int, c_int, c_void_p, c_int, c_int, c_float, c_void_p,
+                                   c_void_p, _I64x3, c_void_p, _I64x3, c_void_p, c_void_p]),
+    "minf_kv8_evict": (c_int, [_KV8, _KV8, c_void_p, c_int, c_int, c_void_p, _I64x3] + [c_int] * 3 + [c_void_p] * 4),
 }
 
 
@@ -141,7 +157,8 @@ def raise_on_status(status: torch.Tensor, what: str) -> None:
     if st[ST_ERROR]:
         raise MInferB200Error(f"{what}: device reported error bits {st[ST_ERROR]:#x} "
                               "(1 = abandoned wait, 2 = misaligned shared memory, 8 = a range check of the debug build failed, 4 = bad plan: a plan-mode head without a plan, "
-                              "a range count beyond the slot's capacity, unordered ranges, or columns without a vertical list)")
+                              "a range count beyond the slot's capacity, unordered ranges, or columns without a vertical list, "
+                              "16 = a length or position outside its 8-bit cache)")
     if st[ST_NO_SLASH]:
         raise MInferB200Error(f"{what}: {st[ST_NO_SLASH]} row blocks have no slash offset below their last row; "
                               "s_idx must contain an offset < 64")

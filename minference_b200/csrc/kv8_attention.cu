@@ -1,0 +1,638 @@
+// Attention over an 8-bit key/value cache (layout: kv8.cuh): decoding steps of one or a few tokens, and longer ones.
+//
+// For a row (query head, query token) with logits l_t = sm_scale log2(e) s_K,t (q . c_K,t) over the tokens it sees,
+//   out = sum_t 2^(l_t - lse) s_V,t c_V,t,    lse = log2 sum_t 2^l_t
+// in one pass over the cache.  The running maximum M is that of l_t + log2 s_V,t, so the numerators
+// P_t = 2^(l_t + log2 s_V,t - M) are at most 1 and multiply the codes as they are, whatever the scales; the
+// denominator is the sum over blocks of (sum P_t) / s_V.
+//
+// The products run on the tensor cores with the tokens as rows: S^T = K Q^T and O^T = V^T P^T, m16n8k16 in f16 with
+// fp32 accumulation.  Eight query rows (a group of query heads that share a cache head, times the new tokens) fill the
+// narrow side without padding to sixteen, and a code becomes an f16 value exactly.  Q is scaled by a power of two per
+// row so that its bf16 values are f16 values (what is lost lies 2^-24 below the row's largest).  P is rounded to f16:
+// half a step of 2^-11 relative, below the bf16 rounding of the output; sums and outputs are accumulated in fp32.
+// The tail (bf16) takes bf16 products, with P as a sum of two bf16 numbers.
+//
+// The tokens of a sequence are split over CTAs and, inside one, over warps by blocks of 64; the parts are joined by
+// their log-sum-exps in a second kernel.
+#include "kv8.cuh"
+
+#include <math_constants.h>
+
+#include <algorithm>
+
+#include "sm100_ptx.cuh"
+
+namespace minf {
+
+constexpr int kAttnWarps = 4;
+constexpr int kAttnThreads = kAttnWarps * 32;
+constexpr int kSMs = 148;
+
+struct Kv8AttnArgs {
+    minf_kv8_cache c;
+    const __nv_bfloat16* q;
+    long long qs[3];
+    __nv_bfloat16* o;
+    long long os[3];
+    int group, n_q, rows;           // rows = group * n_q per cache head; row r is query head r / n_q, token r % n_q
+    const int32_t* lengths;
+    int length_all, max_length;
+    float scale_log2;
+    int splits;
+    float* part_o;                  // [batch*heads*rows][splits][128], normalised
+    float* part_lse;                // [batch*heads*rows][splits]
+    float* lse;                     // caller's, [batch, hq, n_q], or NULL
+    float* row_lse;                 // [batch*heads*rows] (for the weights), or NULL
+    float* logits;                  // [batch*heads][tokens][pitch], or NULL
+    int pitch;
+    long long tokens;               // rows of `logits` per head
+    float* weights;
+    long long ws[2];
+    const float* add_to;
+    long long as[2];
+};
+
+__device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+        : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+        : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
+    uint32_t y;
+    asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+    return y;
+}
+__device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+// any half of the register infinite or NaN
+template <bool BF16>
+__device__ __forceinline__ bool not_finite(uint32_t x) {
+    constexpr uint32_t m = BF16 ? 0x7f80u : 0x7c00u;
+    return (x & m) == m || (x & (m << 16)) == (m << 16);
+}
+
+// What a warp carries along its tokens, for NT groups of eight rows: a lane holds columns 2c and 2c+1 of each group
+// (c = lane % 4), and of the outputs dims 16g .. 16g+15 (g = lane / 4): o[nt][i] = {(dim 2i, col 2c), (2i, 2c+1),
+// (2i+1, 2c), (2i+1, 2c+1)} of those.
+template <int NT>
+struct Rows {
+    float o[NT][8][4];
+    float m[NT][2];                 // running maximum of l + log2 s_V
+    float l[NT][2];                 // this lane's part of the denominator, relative to m
+    float mul[NT][2];               // logit of a unit of the accumulator, before the block's scale
+    int lim[NT][2];                 // tokens below this are seen
+};
+
+// Logits of 16 * SUB tokens -> P, with the running statistics moved on.  s[j][nt][e]: token t0 + 16 j + g (+ 8 for e = 2, 3),
+// column 2c (+ 1 for odd e).  On return s holds P.
+template <int NT, int SUB>
+__device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, float (&s)[SUB][NT][4], float k_scale, float v_scale,
+                                             int t0, bool masked, int end, size_t bh, int row0, int g, int c) {
+    const float lv = log2f(v_scale), inv_v = 1.f / v_scale;
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const float f0 = R.mul[nt][0] * k_scale, f1 = R.mul[nt][1] * k_scale;
+        float mx0 = -CUDART_INF_F, mx1 = -CUDART_INF_F;
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            float* x = s[j][nt];
+            x[0] *= f0;
+            x[1] *= f1;
+            x[2] *= f0;
+            x[3] *= f1;
+            if (masked) {
+                const int t = t0 + 16 * j + g;
+                if (t >= R.lim[nt][0]) x[0] = -CUDART_INF_F;
+                if (t >= R.lim[nt][1]) x[1] = -CUDART_INF_F;
+                if (t + 8 >= R.lim[nt][0]) x[2] = -CUDART_INF_F;
+                if (t + 8 >= R.lim[nt][1]) x[3] = -CUDART_INF_F;
+            }
+            if (a.logits) {
+                const int col = row0 + 8 * nt + 2 * c, t = t0 + 16 * j + g;
+                if (col < a.pitch) {
+                    float* p = a.logits + ((long long)bh * a.tokens + t) * a.pitch + col;
+                    if (t < end) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
+                    if (t + 8 < end) *reinterpret_cast<float2*>(p + 8ll * a.pitch) = make_float2(x[2], x[3]);
+                }
+            }
+            mx0 = fmaxf(mx0, fmaxf(x[0], x[2]));
+            mx1 = fmaxf(mx1, fmaxf(x[1], x[3]));
+        }
+#pragma unroll
+        for (int o = 4; o < 32; o <<= 1) {
+            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+        }
+        const float n0 = fmaxf(R.m[nt][0], mx0 + lv), n1 = fmaxf(R.m[nt][1], mx1 + lv);
+        const float r0 = n0 == -CUDART_INF_F ? 0.f : n0, r1 = n1 == -CUDART_INF_F ? 0.f : n1;   // nothing seen yet: keep -inf - 0
+        if (__any_sync(0xffffffffu, n0 != R.m[nt][0] || n1 != R.m[nt][1])) {
+            const float a0 = fast_exp2(R.m[nt][0] - r0), a1 = fast_exp2(R.m[nt][1] - r1);
+            R.l[nt][0] *= a0;
+            R.l[nt][1] *= a1;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                R.o[nt][i][0] *= a0;
+                R.o[nt][i][1] *= a1;
+                R.o[nt][i][2] *= a0;
+                R.o[nt][i][3] *= a1;
+            }
+            R.m[nt][0] = n0;
+            R.m[nt][1] = n1;
+        }
+        const float d0 = lv - r0, d1 = lv - r1;
+        float sum0 = 0.f, sum1 = 0.f;
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            float* x = s[j][nt];
+            x[0] = fast_exp2(x[0] + d0);
+            x[1] = fast_exp2(x[1] + d1);
+            x[2] = fast_exp2(x[2] + d0);
+            x[3] = fast_exp2(x[3] + d1);
+            sum0 += x[0] + x[2];
+            sum1 += x[1] + x[3];
+        }
+        R.l[nt][0] = fmaf(sum0, inv_v, R.l[nt][0]);
+        R.l[nt][1] = fmaf(sum1, inv_v, R.l[nt][1]);
+    }
+}
+
+// O^T += V^T P^T for 16 tokens of one column group.  v[i][0..3]: the A fragment of dims 16g+2i, 16g+2i+1 (rows g and
+// g + 8 of the product).  Where a value of a token that some column does not see may be infinite or NaN, the product
+// is taken column by column with the unseen tokens' values left out: zero times them would not be zero.
+template <bool BF16>
+__device__ __forceinline__ void pv_mma(float (&d)[4], const uint32_t (&v)[4], uint32_t b0, uint32_t b1) {
+    if constexpr (BF16) mma_bf16(d, v[0], v[1], v[2], v[3], b0, b1);
+    else mma_f16(d, v[0], v[1], v[2], v[3], b0, b1);
+}
+template <bool BF16, int NT>
+__device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], int nt, uint32_t b0, uint32_t b1, bool masked, int t0, int g, int c) {
+    if (masked) {
+        bool bad = false;
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) bad |= not_finite<BF16>(v[i][e]);
+        if (__any_sync(0xffffffffu, bad)) {
+            for (int col = 0; col < 8; ++col) {
+                const int l0 = __shfl_sync(0xffffffffu, R.lim[nt][0], col >> 1), l1 = __shfl_sync(0xffffffffu, R.lim[nt][1], col >> 1);
+                const int lim = (col & 1) ? l1 : l0;
+                const uint32_t k0 = (t0 + 2 * c < lim ? 0xffffu : 0u) | (t0 + 2 * c + 1 < lim ? 0xffff0000u : 0u);
+                const uint32_t k1 = (t0 + 2 * c + 8 < lim ? 0xffffu : 0u) | (t0 + 2 * c + 9 < lim ? 0xffff0000u : 0u);
+                const uint32_t c0 = g == col ? b0 : 0u, c1 = g == col ? b1 : 0u;
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    float d[4] = {0.f, 0.f, 0.f, 0.f};
+                    const uint32_t w[4] = {v[i][0] & k0, v[i][1] & k0, v[i][2] & k1, v[i][3] & k1};
+                    pv_mma<BF16>(d, w, c0, c1);
+                    if (2 * c == col) {             // the other columns' products are 0 times these values: left out
+                        R.o[nt][i][0] += d[0];
+                        R.o[nt][i][2] += d[2];
+                    }
+                    if (2 * c + 1 == col) {
+                        R.o[nt][i][1] += d[1];
+                        R.o[nt][i][3] += d[3];
+                    }
+                }
+            }
+            return;
+        }
+    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) pv_mma<BF16>(R.o[nt][i], v[i], b0, b1);
+}
+
+template <int FMT, int NT>
+__global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    constexpr int SUB = 4 / NT;                     // sub-tiles of 16 tokens per softmax step: 16 logits a lane for every NT
+    const int split = blockIdx.x, b = blockIdx.z;
+    const int tiles = (a.rows + 8 * NT - 1) / (8 * NT);
+    const int h = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * 8 * NT;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
+    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const int full = n / kKv8Block;                 // complete blocks
+    const int blk_lo = (int)((long long)full * split / a.splits), blk_hi = (int)((long long)full * (split + 1) / a.splits);
+    const int all_see = n - a.n_q + 1;              // tokens below this are seen by every row
+
+    // Q^T fragments: column g of group nt, dims of step s: 64 (s / 4) + 16 c + 4 (s % 4) + {0, 1 | 2, 3}
+    Rows<NT> R;
+    uint32_t qf[NT][8][2];
+    float q_unit[NT];                               // power of two the row was divided by
+    auto q_row = [&](int nt) {
+        const int r = row0 + 8 * nt + g;
+        return r < a.rows ? a.q + b * a.qs[0] + (long long)(h * a.group + r / a.n_q) * a.qs[1] + (long long)(r % a.n_q) * a.qs[2] : nullptr;
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const __nv_bfloat16* q = q_row(nt);
+        float top = 0.f;
+        float x[8][4];
+#pragma unroll
+        for (int s = 0; s < 8; ++s)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+                x[s][e] = q ? __bfloat162float(q[64 * (s >> 2) + 16 * c + 4 * (s & 3) + e]) : 0.f;
+                const float m = fabsf(x[s][e]);
+                if (m < CUDART_INF_F) top = fmaxf(top, m);
+            }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = 0;
+        if (top > 0.f) frexpf(top, &e);             // top < 2^e: scaled to below 2^8, so that the smallest products count too
+        e = max(min(e - 8, 100), -100);
+        const float inv = exp2f((float)-e);
+        q_unit[nt] = exp2f((float)e);
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            qf[nt][s][0] = pack_half2(x[s][0] * inv, x[s][1] * inv);
+            qf[nt][s][1] = pack_half2(x[s][2] * inv, x[s][3] * inv);
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+            const int r = row0 + 8 * nt + 2 * c + cc;
+            R.mul[nt][cc] = a.scale_log2 * __shfl_sync(0xffffffffu, q_unit[nt], 4 * (2 * c + cc));
+            R.lim[nt][cc] = r < a.rows ? all_see + r % a.n_q : 0x7fffffff;     // columns beyond the rows are dropped
+            R.m[nt][cc] = -CUDART_INF_F;
+            R.l[nt][cc] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) R.o[nt][i][k] = 0.f;
+    }
+
+    const uint8_t* kc = static_cast<const uint8_t*>(a.c.k) + bh * a.c.capacity * kKv8Dim;
+    const uint8_t* vc = static_cast<const uint8_t*>(a.c.v) + bh * a.c.capacity * kKv8Dim;
+    const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
+    const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
+
+    for (int blk = blk_lo + warp; blk < blk_hi; blk += kAttnWarps) {
+        const float k_scale = ks[blk], v_scale = vs[blk];
+        const bool masked = (blk + 1) * kKv8Block > all_see;
+#pragma unroll 1
+        for (int part = 0; part < NT; ++part) {
+            const int t0 = blk * kKv8Block + part * SUB * 16;
+            float s[SUB][NT][4];
+#pragma unroll
+            for (int j = 0; j < SUB; ++j) {
+                const uint8_t* p = kc + (size_t)(t0 + 16 * j + g) * kKv8Dim + 16 * c;
+                const uint4 k00 = *reinterpret_cast<const uint4*>(p), k01 = *reinterpret_cast<const uint4*>(p + 64);
+                const uint4 k10 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim), k11 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim + 64);
+                const uint32_t r0[8] = {k00.x, k00.y, k00.z, k00.w, k01.x, k01.y, k01.z, k01.w};
+                const uint32_t r1[8] = {k10.x, k10.y, k10.z, k10.w, k11.x, k11.y, k11.z, k11.w};
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) s[j][nt][e] = 0.f;
+#pragma unroll
+                for (int st = 0; st < 8; ++st) {
+                    uint32_t a0, a1, a2, a3;
+                    codes_to_half<FMT>(r0[st], a0, a2);
+                    codes_to_half<FMT>(r1[st], a1, a3);
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(s[j][nt], a0, a1, a2, a3, qf[nt][st][0], qf[nt][st][1]);
+                }
+            }
+            softmax_step<NT, SUB>(a, R, s, k_scale, v_scale, t0, masked, n, bh, row0, g, c);
+#pragma unroll
+            for (int j = 0; j < SUB; ++j) {
+                // A fragment of V^T: tokens 2c, 2c+1 (and + 8) in the halves of a register
+                uint32_t v[8][4];
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    const uint8_t* p = vc + (size_t)(t0 + 16 * j + 2 * c + 8 * hf) * kKv8Dim + 16 * g;
+                    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + kKv8Dim);
+                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                    for (int w = 0; w < 4; ++w) {
+                        codes_to_half<FMT>(__byte_perm(xs[w], ys[w], 0x5140), v[2 * w][2 * hf], v[2 * w][2 * hf + 1]);
+                        codes_to_half<FMT>(__byte_perm(xs[w], ys[w], 0x7362), v[2 * w + 1][2 * hf], v[2 * w + 1][2 * hf + 1]);
+                    }
+                }
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    const uint32_t b0 = transpose8x8(pack_half2(s[j][nt][0], s[j][nt][1])), b1 = transpose8x8(pack_half2(s[j][nt][2], s[j][nt][3]));
+                    pv_step<false, NT>(R, v, nt, b0, b1, masked, t0 + 16 * j, g, c);
+                }
+            }
+        }
+    }
+
+    // the tail: the last split's warps take 16 of its tokens each
+    const int t0 = full * kKv8Block + 16 * warp;
+    if (split == a.splits - 1 && t0 < n) {
+        const __nv_bfloat16* kt = static_cast<const __nv_bfloat16*>(a.c.k_tail) + (bh * kKv8Block + 16 * warp) * kKv8Dim;
+        const __nv_bfloat16* vt = static_cast<const __nv_bfloat16*>(a.c.v_tail) + (bh * kKv8Block + 16 * warp) * kKv8Dim;
+        float s[1][NT][4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[0][nt][e] = 0.f;
+            const __nv_bfloat16* q = q_row(nt);
+            const float inv = 1.f / q_unit[nt];
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                const int d = 64 * (st >> 2) + 16 * c + 4 * (st & 3);
+                uint32_t b0 = 0, b1 = 0;
+                if (q) {
+                    b0 = pack_bf16x2(__bfloat162float(q[d]) * inv, __bfloat162float(q[d + 1]) * inv);
+                    b1 = pack_bf16x2(__bfloat162float(q[d + 2]) * inv, __bfloat162float(q[d + 3]) * inv);
+                }
+                const uint2 x = *reinterpret_cast<const uint2*>(kt + g * kKv8Dim + d), y = *reinterpret_cast<const uint2*>(kt + (g + 8) * kKv8Dim + d);
+                mma_bf16(s[0][nt], x.x, y.x, x.y, y.y, b0, b1);
+            }
+        }
+        softmax_step<NT, 1>(a, R, s, 1.f, 1.f, t0, true, n, bh, row0, g, c);
+        uint32_t v[8][4];
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+            const int r = 2 * c + 8 * hf;
+            const __nv_bfloat16* p = vt + r * kKv8Dim + 16 * g;
+#pragma unroll
+            for (int w = 0; w < 2; ++w) {           // eight dims of the two tokens
+                uint4 x = *reinterpret_cast<const uint4*>(p + 8 * w), y = *reinterpret_cast<const uint4*>(p + kKv8Dim + 8 * w);
+                if (t0 + r >= n) x = make_uint4(0u, 0u, 0u, 0u);        // rows behind the last token hold anything
+                if (t0 + r + 1 >= n) y = make_uint4(0u, 0u, 0u, 0u);
+                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    v[4 * w + k][2 * hf] = __byte_perm(xs[k], ys[k], 0x5410);
+                    v[4 * w + k][2 * hf + 1] = __byte_perm(xs[k], ys[k], 0x7632);
+                }
+            }
+        }
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            float* x = s[0][nt];
+            const uint32_t h0 = pack_bf16x2(x[0], x[1]), h1 = pack_bf16x2(x[2], x[3]);
+            const uint32_t e0 = pack_bf16x2(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xffff0000u));
+            const uint32_t e1 = pack_bf16x2(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xffff0000u));
+            pv_step<true, NT>(R, v, nt, transpose8x8(h0), transpose8x8(h1), true, t0, g, c);
+            pv_step<true, NT>(R, v, nt, transpose8x8(e0), transpose8x8(e1), true, t0, g, c);
+        }
+    }
+
+    // join the warps, eight rows at a time
+    __shared__ __align__(16) float sm_o[kAttnWarps][8][kKv8Dim];
+    __shared__ float sm_lse[kAttnWarps][8];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+            float l = R.l[nt][cc];
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
+            const float inv = l == 0.f ? 0.f : 1.f / l;
+            if (g == 0) sm_lse[warp][2 * c + cc] = l == 0.f ? -CUDART_INF_F : (R.m[nt][cc] == -CUDART_INF_F ? l : R.m[nt][cc] + log2f(l));
+            float* dst = &sm_o[warp][2 * c + cc][16 * g];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(R.o[nt][2 * i][cc] * inv, R.o[nt][2 * i][2 + cc] * inv,
+                                                                      R.o[nt][2 * i + 1][cc] * inv, R.o[nt][2 * i + 1][2 + cc] * inv);
+        }
+        __syncthreads();
+        for (int i = threadIdx.x; i < 8 * 32; i += kAttnThreads) {
+            const int rr = i >> 5, d = (i & 31) * 4, r = row0 + 8 * nt + rr;
+            if (r >= a.rows) continue;
+            float top = sm_lse[0][rr];
+#pragma unroll
+            for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_lse[w][rr]);
+            float sum = 0.f;
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+            for (int w = 0; w < kAttnWarps; ++w) {
+                const float e = sm_lse[w][rr];
+                if (e == -CUDART_INF_F) continue;
+                const float f = exp2f(e - top);
+                const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][rr][d]);
+                sum += f;
+                acc.x = fmaf(f, x.x, acc.x);
+                acc.y = fmaf(f, x.y, acc.y);
+                acc.z = fmaf(f, x.z, acc.z);
+                acc.w = fmaf(f, x.w, acc.w);
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            acc.x *= inv;
+            acc.y *= inv;
+            acc.z *= inv;
+            acc.w *= inv;
+            const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+            const size_t row = bh * a.rows + r;
+            if (a.splits > 1) {
+                *reinterpret_cast<float4*>(a.part_o + (row * a.splits + split) * kKv8Dim + d) = acc;
+                if (d == 0) a.part_lse[row * a.splits + split] = lse;
+            } else {
+                const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
+                __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
+                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+                if (d == 0) {
+                    if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = lse;
+                    if (a.row_lse) a.row_lse[row] = lse;
+                }
+            }
+        }
+        __syncthreads();
+    }
+}
+
+// The splits of one row joined: four warps take every fourth split, a lane four dims.
+__global__ void __launch_bounds__(128) kv8_combine_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    __shared__ float4 sm[4][32];
+    __shared__ float sm_sum[4];
+    const size_t row = blockIdx.x;
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const float* lse = a.part_lse + row * a.splits;
+    float top = -CUDART_INF_F;
+    for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, lse[i]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int i = warp; i < a.splits; i += 4) {
+        const float e = lse[i];
+        if (e == -CUDART_INF_F) continue;
+        const float f = exp2f(e - top);
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * kKv8Dim + 4 * lane);
+        sum += f;
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+    }
+    sm[warp][lane] = acc;
+    if (lane == 0) sm_sum[warp] = sum;
+    __syncthreads();
+    if (warp) return;
+    sum = sm_sum[0] + sm_sum[1] + sm_sum[2] + sm_sum[3];
+    acc = sm[0][lane];
+#pragma unroll
+    for (int w = 1; w < 4; ++w) {
+        const float4 x = sm[w][lane];
+        acc.x += x.x;
+        acc.y += x.y;
+        acc.z += x.z;
+        acc.w += x.w;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const size_t bh = row / a.rows;
+    const int r = (int)(row % a.rows), b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+    const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
+    __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + 4 * lane;
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (lane == 0) {
+        const float e = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+        if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = e;
+        if (a.row_lse) a.row_lse[row] = e;
+    }
+}
+
+// Attention weight of every token of a head: the probabilities of the head's rows, summed in their order.
+__global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    const int b = blockIdx.z, h = blockIdx.y;
+    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
+    const int t = blockIdx.x * 256 + threadIdx.x;
+    if (t >= n) return;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const float* x = a.logits + ((long long)bh * a.tokens + t) * a.pitch;
+    const float* e = a.row_lse + bh * a.rows;
+    float sum = 0.f;
+    for (int r = 0; r < a.rows; r += 2) {
+        const float2 l = *reinterpret_cast<const float2*>(x + r);
+        const float e0 = e[r];
+        sum += l.x == -CUDART_INF_F ? 0.f : exp2f(l.x - e0);
+        if (r + 1 < a.rows) sum += l.y == -CUDART_INF_F ? 0.f : exp2f(l.y - e[r + 1]);
+    }
+    const float was = a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f;
+    a.weights[b * a.ws[0] + h * a.ws[1] + t] = was + sum;
+}
+
+// ---------------------------------------------------------------------------------------------------- host
+struct AttnShape {
+    int nt, tiles, splits, pitch;
+    long long tokens;
+    size_t part_o, part_lse, row_lse, logits, bytes;
+};
+
+static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
+    AttnShape s{};
+    const long long rows = (long long)(hq / heads) * n_q;
+    s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    s.tiles = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
+    const long long ctas = (long long)batch * heads * s.tiles;
+    const long long blocks = max_length / kKv8Block;
+    long long splits = (4 * kSMs + ctas - 1) / ctas;
+    splits = std::min(splits, (blocks + kAttnWarps - 1) / kAttnWarps);
+    s.splits = (int)std::max(splits, 1ll);
+    s.pitch = (int)((rows + 1) / 2 * 2);
+    s.tokens = max_length;
+    auto up = [](size_t x) { return (x + 255) / 256 * 256; };
+    const size_t all = (size_t)batch * heads * rows;
+    size_t at = 0;
+    s.part_o = at;
+    if (s.splits > 1) at = up(at + all * s.splits * kKv8Dim * sizeof(float));
+    s.part_lse = at;
+    if (s.splits > 1) at = up(at + all * s.splits * sizeof(float));
+    s.row_lse = at;
+    if (weights) at = up(at + all * sizeof(float));
+    s.logits = at;
+    if (weights) at = up(at + (size_t)batch * heads * s.tokens * s.pitch * sizeof(float));
+    s.bytes = at;
+    return s;
+}
+
+static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_length) {
+    return batch >= 1 && heads >= 1 && hq >= heads && hq % heads == 0 && n_q >= 1 && max_length >= 0 && (long long)hq * n_q <= (1 << 24);
+}
+
+template <int FMT>
+static void launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+    dim3 grid(s.splits, a.c.heads * s.tiles, a.c.batch);
+    if (s.nt == 1) kv8_attention_kernel<FMT, 1><<<grid, kAttnThreads, 0, stream>>>(a);
+    else if (s.nt == 2) kv8_attention_kernel<FMT, 2><<<grid, kAttnThreads, 0, stream>>>(a);
+    else kv8_attention_kernel<FMT, 4><<<grid, kAttnThreads, 0, stream>>>(a);
+}
+
+}  // namespace minf
+
+using namespace minf;
+
+extern "C" size_t minf_kv8_attention_scratch_bytes(int batch, int hq, int heads, int n_q, int max_length, int with_weights) {
+    if (!attention_sizes_ok(batch, hq, heads, n_q, max_length)) return 0;
+    return attention_shape(batch, hq, heads, n_q, max_length, with_weights != 0).bytes;
+}
+
+extern "C" int minf_kv8_attention(
+    const minf_kv8_cache* cache, const void* q, const int64_t q_strides[3], void* o, const int64_t o_strides[3],
+    int hq, int n_q, const int32_t* lengths, int length_all, int max_length, float sm_scale, float* lse,
+    float* weights, const int64_t w_strides[2], const float* add_to, const int64_t add_strides[2],
+    void* scratch, void* stream) {
+    if (int rc = kv8_check(cache)) return rc;
+    if (!q || !o || !q_strides || !o_strides || (weights && !w_strides) || (add_to && !add_strides)) return fail(MINF_E_ARG, "null pointer argument");
+    if (!attention_sizes_ok(cache->batch, hq, cache->heads, n_q, max_length))
+        return fail(MINF_E_ARG, "bad sizes (%d query heads over %d, %d queries, max_length %d)", hq, cache->heads, n_q, max_length);
+    if (max_length > cache->capacity) return fail(MINF_E_ARG, "max_length %d is outside the cache of %d tokens", max_length, cache->capacity);
+    if (!lengths && (length_all < 0 || length_all > max_length)) return fail(MINF_E_ARG, "length %d is outside [0, max_length %d]", length_all, max_length);
+    if (add_to && !weights) return fail(MINF_E_ARG, "add_to without weights");
+    const AttnShape s = attention_shape(cache->batch, hq, cache->heads, n_q, max_length, weights != nullptr);
+    if (s.bytes && !scratch) return fail(MINF_E_ARG, "scratch is needed (%zu bytes)", s.bytes);
+    if (reinterpret_cast<uintptr_t>(scratch) & 15) return fail(MINF_E_ARG, "scratch must be 16-byte aligned");
+    if ((long long)cache->heads * s.tiles > 65535) return fail(MINF_E_UNSUPPORTED, "too many query rows (%d heads of %d tiles)", cache->heads, s.tiles);
+    Kv8AttnArgs a{};
+    a.c = *cache;
+    a.q = static_cast<const __nv_bfloat16*>(q);
+    a.o = static_cast<__nv_bfloat16*>(o);
+    for (int i = 0; i < 3; ++i) {
+        a.qs[i] = q_strides[i];
+        a.os[i] = o_strides[i];
+        if (o_strides[i] % 4) return fail(MINF_E_ARG, "output strides must be multiples of 4 elements");
+    }
+    if (reinterpret_cast<uintptr_t>(o) & 7) return fail(MINF_E_ARG, "the output must be 8-byte aligned");
+    a.group = hq / cache->heads;
+    a.n_q = n_q;
+    a.rows = a.group * n_q;
+    a.lengths = lengths;
+    a.length_all = length_all;
+    a.max_length = max_length;
+    a.scale_log2 = sm_scale * 1.4426950408889634f;
+    a.splits = s.splits;
+    char* base = static_cast<char*>(scratch);
+    a.part_o = reinterpret_cast<float*>(base + s.part_o);
+    a.part_lse = reinterpret_cast<float*>(base + s.part_lse);
+    a.lse = lse;
+    a.pitch = s.pitch;
+    a.tokens = s.tokens;
+    if (weights) {
+        a.row_lse = reinterpret_cast<float*>(base + s.row_lse);
+        a.logits = reinterpret_cast<float*>(base + s.logits);
+        a.weights = weights;
+        a.ws[0] = w_strides[0];
+        a.ws[1] = w_strides[1];
+        a.add_to = add_to;
+        if (add_to) {
+            a.as[0] = add_strides[0];
+            a.as[1] = add_strides[1];
+        }
+    }
+    cudaStream_t st = static_cast<cudaStream_t>(stream);
+    if (cache->format == MINF_KV8_E4M3) launch_attention<MINF_KV8_E4M3>(a, s, st);
+    else launch_attention<MINF_KV8_INT8>(a, s, st);
+    MINF_LAUNCH_OK("kv8_attention_kernel");
+    if (s.splits > 1) {
+        kv8_combine_kernel<<<(unsigned)((size_t)cache->batch * cache->heads * a.rows), 128, 0, st>>>(a);
+        MINF_LAUNCH_OK("kv8_combine_kernel");
+    }
+    if (weights && max_length > 0) {
+        kv8_weights_kernel<<<dim3((max_length + 255) / 256, cache->heads, cache->batch), 256, 0, st>>>(a);
+        MINF_LAUNCH_OK("kv8_weights_kernel");
+    }
+    return MINF_OK;
+}

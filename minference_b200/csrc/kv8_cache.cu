@@ -1,0 +1,479 @@
+// Filling, reading back and shrinking an 8-bit key/value cache (layout: kv8.cuh).
+//
+// Quantisation of a block x (64 tokens x 128 of one head): with m the largest finite magnitude,
+//   e4m3: scale = 2^p, p the smallest with 448 * 2^p >= m -- dividing by a power of two is exact, so a code is the one
+//         rounding of x to e4m3's grid, and requantising values that came from codes loses nothing but what falls
+//         below the new grid's subnormals;
+//   int8: scale = m / 127 in fp32, code = round-half-even(x / scale) with an IEEE division.
+// Scales are at least 2^-100; an all-zero block has scale 1.  NaN stays NaN in e4m3 and becomes 0 in int8; infinities
+// become the largest code.
+#include "kv8.cuh"
+
+#include "sm100_ptx.cuh"
+
+namespace minf {
+
+int kv8_check(const minf_kv8_cache* c) {
+    if (!c) return fail(MINF_E_ARG, "null cache");
+    if (!c->k || !c->v || !c->k_scale || !c->v_scale || !c->k_tail || !c->v_tail || !c->status)
+        return fail(MINF_E_ARG, "null pointer in the cache");
+    if (c->batch < 1 || c->heads < 1 || c->batch > 65535 || c->heads > 32767)
+        return fail(MINF_E_ARG, "bad cache sizes (batch %d, heads %d)", c->batch, c->heads);
+    if (c->capacity < kKv8Block || c->capacity % kKv8Block || c->capacity > (1 << 30))
+        return fail(MINF_E_ARG, "the cache's capacity must be a positive multiple of %d tokens, 2^30 at most (got %d)", kKv8Block, c->capacity);
+    if (c->format != MINF_KV8_E4M3 && c->format != MINF_KV8_INT8) return fail(MINF_E_ARG, "unknown cache format %d", c->format);
+    const uintptr_t all = reinterpret_cast<uintptr_t>(c->k) | reinterpret_cast<uintptr_t>(c->v) |
+                          reinterpret_cast<uintptr_t>(c->k_tail) | reinterpret_cast<uintptr_t>(c->v_tail);
+    if (all & 15) return fail(MINF_E_ARG, "the cache's tensors must be 16-byte aligned");
+    return MINF_OK;
+}
+
+// Largest finite magnitude of the block from each thread's own, for all threads of the CTA.
+template <int THREADS>
+__device__ __forceinline__ float block_max(float m, float* red) {
+#pragma unroll
+    for (int o = 16; o; o >>= 1) m = fmaxf(m, __shfl_xor_sync(0xffffffffu, m, o));
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = m;
+    __syncthreads();
+    m = red[0];
+#pragma unroll
+    for (int i = 1; i < THREADS / 32; ++i) m = fmaxf(m, red[i]);
+    return m;
+}
+
+__device__ __forceinline__ float finite_magnitude(float x) {
+    const float a = fabsf(x);
+    return a < INFINITY ? a : 0.f;          // NaN compares false
+}
+
+template <int FMT>
+__device__ __forceinline__ float scale_of(float top) {
+    if (!(top > 0.f)) return 1.f;
+    if constexpr (FMT == MINF_KV8_E4M3) {
+        int e;
+        const float m = frexpf(top, &e);    // top = m * 2^e, 0.5 <= m < 1;  448 = 0.875 * 2^9
+        return exp2f((float)max(m <= 0.875f ? e - 9 : e - 8, -100));
+    } else {
+        return fmaxf(__fdiv_rn(top, 127.f), kKv8MinScale);
+    }
+}
+
+template <int FMT>
+__device__ __forceinline__ uint2 values_to_codes(const float (&x)[8], float scale) {
+    uint32_t c[2];
+    if constexpr (FMT == MINF_KV8_E4M3) {
+        const float inv = __fdiv_rn(1.f, scale);            // a power of two: exact
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint16_t lo, hi;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(lo) : "f"(x[4 * i + 1] * inv), "f"(x[4 * i] * inv));
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(x[4 * i + 3] * inv), "f"(x[4 * i + 2] * inv));
+            c[i] = (uint32_t)lo | ((uint32_t)hi << 16);
+        }
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            uint32_t w = 0;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float q = rintf(__fdiv_rn(x[4 * i + j], scale));
+                const int r = q != q ? 0 : (int)fminf(fmaxf(q, -127.f), 127.f);
+                w |= (uint32_t)(r & 0xff) << (8 * j);
+            }
+            c[i] = w;
+        }
+    }
+    return make_uint2(c[0], c[1]);
+}
+
+// ------------------------------------------------------------------------------------------------- store
+// One CTA per (block of 64 tokens that gets new ones, head, keys or values).  256 threads hold the block in
+// registers, eight values of four rows each: one read of the new tokens, one write of the codes.
+// Bound by HBM: 4 B read and 2 B written per (key, value) pair of elements.
+struct StoreArgs {
+    minf_kv8_cache c;
+    const __nv_bfloat16* src[2];
+    long long stride[2][3];
+    int n_tokens;
+    const int32_t* start;
+    int start_all;
+    const int32_t* counts;
+};
+
+constexpr int kStoreThreads = 256;
+
+template <int FMT>
+__global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(const __grid_constant__ StoreArgs a) {
+    __shared__ float red[kStoreThreads / 32];
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const int start = a.start ? a.start[b] : a.start_all;
+    const int count = a.counts ? a.counts[b] : a.n_tokens;
+    if (start < 0 || count < 0 || count > a.n_tokens || start > a.c.capacity - count) {
+        if (threadIdx.x == 0) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
+        return;                                             // nothing of this sequence is stored
+    }
+    if (count == 0) return;
+    const int end = start + count;
+    const int blk0 = start / kKv8Block, last = (end - 1) / kKv8Block;
+    const int blk = blk0 + blockIdx.x;
+    if (blk > last) return;
+    const bool complete = (blk + 1) * kKv8Block <= end;
+    if (!complete && blk != blk0) return;                   // the first block's CTA writes the tail once it has read it
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const __nv_bfloat16* src = a.src[which] + b * a.stride[which][0] + h * a.stride[which][1];
+    const long long row_stride = a.stride[which][2];
+    __nv_bfloat16* tail = static_cast<__nv_bfloat16*>(which ? a.c.v_tail : a.c.k_tail) + bh * (kKv8Block * kKv8Dim);
+    const int chunk = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+    auto new_row = [&](int t) { return *reinterpret_cast<const uint4*>(src + (t - start) * row_stride + chunk * 8); };
+    auto tail_row = [&](int r) { return reinterpret_cast<uint4*>(tail + r * kKv8Dim + chunk * 8); };
+
+    if (complete) {
+        float x[4][8];
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int r = row0 + 16 * i, t = blk * kKv8Block + r;
+            bf16x8_to_values(t < start ? *tail_row(r) : new_row(t), x[i]);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[i][j]));
+        }
+        top = block_max<kStoreThreads>(top, red);           // (its barrier also ends the reads of the tail)
+        const float scale = scale_of<FMT>(top);
+        uint8_t* codes = static_cast<uint8_t*>(which ? a.c.v : a.c.k) + (bh * a.c.capacity + (size_t)blk * kKv8Block) * kKv8Dim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint2*>(codes + (row0 + 16 * i) * kKv8Dim + chunk * 8) = values_to_codes<FMT>(x[i], scale);
+        if (threadIdx.x == 0) (which ? a.c.v_scale : a.c.k_scale)[bh * (a.c.capacity / kKv8Block) + blk] = scale;
+    }
+    if (blk == blk0 && end % kKv8Block) {                   // the tokens behind the last complete block
+        const int t0 = max(start, last * kKv8Block);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int t = last * kKv8Block + row0 + 16 * i;
+            if (t >= t0 && t < end) *tail_row(row0 + 16 * i) = new_row(t);
+        }
+    }
+}
+
+// -------------------------------------------------------------------------------------------------- load
+struct LoadArgs {
+    minf_kv8_cache c;
+    const int32_t* lengths;
+    int length_all;
+    const int32_t* first;
+    int first_all;
+    int count;
+    __nv_bfloat16* out[2];
+};
+
+// Eight values of token t (0 <= t < n) of one head.
+template <int FMT>
+__device__ __forceinline__ void token_values(const minf_kv8_cache& c, int which, size_t bh, int t, int n, int chunk, float (&v)[8]) {
+    if (t < n / kKv8Block * kKv8Block) {
+        const uint8_t* codes = static_cast<const uint8_t*>(which ? c.v : c.k) + (bh * c.capacity + t) * kKv8Dim + chunk * 8;
+        const float scale = (which ? c.v_scale : c.k_scale)[bh * (c.capacity / kKv8Block) + t / kKv8Block];
+        codes_to_values<FMT>(*reinterpret_cast<const uint2*>(codes), scale, v);
+    } else {
+        const __nv_bfloat16* tail = static_cast<const __nv_bfloat16*>(which ? c.v_tail : c.k_tail) + bh * (kKv8Block * kKv8Dim);
+        bf16x8_to_values(*reinterpret_cast<const uint4*>(tail + (t % kKv8Block) * kKv8Dim + chunk * 8), v);
+    }
+}
+
+__device__ __forceinline__ uint4 pack_bf16x8(const float (&v)[8]) {
+    return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
+}
+
+template <int FMT>
+__global__ void __launch_bounds__(kStoreThreads) kv8_load_kernel(const __grid_constant__ LoadArgs a) {
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1;
+    const int n = kv8_length(a.lengths, a.length_all, b, a.c.capacity, a.c.status);
+    const long long first = a.first ? a.first[b] : a.first_all;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const int chunk = threadIdx.x & 15;
+    __nv_bfloat16* out = a.out[which] + bh * a.count * kKv8Dim + chunk * 8;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int r = blockIdx.x * kKv8Block + (threadIdx.x >> 4) + 16 * i;
+        if (r >= a.count) break;
+        const long long t = first + r;
+        uint4 w = make_uint4(0u, 0u, 0u, 0u);
+        if (t >= 0 && t < n) {
+            float v[8];
+            token_values<FMT>(a.c, which, bh, (int)t, n, chunk, v);
+            w = pack_bf16x8(v);
+        }
+        *reinterpret_cast<uint4*>(out + (size_t)r * kKv8Dim) = w;
+    }
+}
+
+// ------------------------------------------------------------------------------------------------- evict
+struct SelectArgsKv8 {
+    minf_kv8_cache c;               // the source
+    const int32_t* lengths;
+    int length_all, max_length;
+    const float* weights;           // [batch, heads, >= max_length] with the strides below, tokens contiguous
+    long long w_stride[2];
+    int budget, recent, sink;
+    int32_t* kept;                  // [batch, heads, budget]
+};
+
+// Weights in the order of their keys: larger weight, larger key; -0 equals 0, a NaN is the largest.
+__device__ __forceinline__ uint32_t weight_key(float w) {
+    if (w != w) return 0xffffffffu;
+    const uint32_t u = __float_as_uint(w + 0.f);            // -0 + 0 = 0
+    return u & 0x80000000u ? ~u : u | 0x80000000u;
+}
+
+constexpr int kSelectThreads = 1024;
+
+// One CTA per (sequence, head): the key of the last token that is kept, by a radix select of four 8-bit digits, then
+// the kept tokens in ascending order.
+__global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
+    __shared__ uint32_t hist[256];
+    __shared__ uint32_t warp_count[2][32];
+    __shared__ uint32_t sh_prefix, sh_need;
+    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
+    const float* w = a.weights + b * a.w_stride[0] + h * a.w_stride[1];
+    int32_t* kept = a.kept + ((size_t)b * a.c.heads + h) * a.budget;
+    if (n <= a.budget) {                                    // everything stays
+        for (int i = tid; i < a.budget; i += kSelectThreads) kept[i] = i < n ? i : -1;
+        return;
+    }
+    const int lo = a.sink, hi = n - a.recent;
+    uint32_t need = a.budget - a.sink - a.recent;           // of hi - lo > need candidates
+    uint32_t prefix = 0;
+    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
+        if (tid < 256) hist[tid] = 0;
+        __syncthreads();
+        for (int t = lo + tid; t < hi; t += kSelectThreads) {
+            const uint32_t key = weight_key(w[t]);
+            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        }
+        __syncthreads();
+        if (tid == 0) {
+            uint32_t left = need;
+            int d = 255;
+            while (d > 0 && hist[d] < left) left -= hist[d--];
+            sh_need = left;
+            sh_prefix = (prefix << 8) | (uint32_t)d;
+        }
+        __syncthreads();
+        prefix = sh_prefix;
+        need = sh_need;
+        __syncthreads();
+    }
+    // keys above `prefix` are kept, and the first `need` that equal it
+    const bool any = a.budget > a.sink + a.recent;
+    uint32_t done = 0, ties_done = 0;
+    for (int t0 = 0; t0 < n; t0 += kSelectThreads) {
+        const int t = t0 + tid;
+        const bool forced = t < n && (t < lo || t >= hi);
+        const uint32_t key = t < n && !forced ? weight_key(w[t]) : 0u;
+        const bool cand = any && t < n && !forced;
+        const bool tie = cand && key == prefix;
+        const uint32_t tie_bits = __ballot_sync(0xffffffffu, tie);
+        if (lane == 0) warp_count[0][warp] = __popc(tie_bits);
+        __syncthreads();
+        uint32_t tie_rank = ties_done, ties_all = 0;
+        for (int i = 0; i < 32; ++i) {
+            if (i < warp) tie_rank += warp_count[0][i];
+            ties_all += warp_count[0][i];
+        }
+        tie_rank += __popc(tie_bits & ((1u << lane) - 1u));
+        const bool keep = forced || (cand && (key > prefix || (tie && tie_rank < need)));
+        const uint32_t keep_bits = __ballot_sync(0xffffffffu, keep);
+        if (lane == 0) warp_count[1][warp] = __popc(keep_bits);
+        __syncthreads();
+        uint32_t rank = done, all = 0;
+        for (int i = 0; i < 32; ++i) {
+            if (i < warp) rank += warp_count[1][i];
+            all += warp_count[1][i];
+        }
+        rank += __popc(keep_bits & ((1u << lane) - 1u));
+        if (keep && rank < (uint32_t)a.budget) kept[rank] = t;
+        done += all;
+        ties_done += ties_all;
+        __syncthreads();
+    }
+}
+
+struct GatherArgs {
+    minf_kv8_cache src, dst;
+    const int32_t* lengths;
+    int length_all, max_length;
+    const float* weights;
+    long long w_stride[2];
+    int budget;
+    const int32_t* kept;
+    float* weights_out;             // [batch, heads, dst.capacity]
+    int32_t* lengths_out;
+};
+
+// One CTA per (block of the new cache, head, keys or values): the kept tokens' values, quantised again as a block.
+template <int FMT>
+__global__ void __launch_bounds__(kStoreThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
+    __shared__ float red[kStoreThreads / 32];
+    const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, blk = blockIdx.x;
+    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.src.status);
+    const int m = min(n, a.budget);
+    const size_t bh = (size_t)b * a.src.heads + h;
+    const int32_t* kept = a.kept + bh * a.budget;
+    if (which == 0 && threadIdx.x < kKv8Block) {
+        const int slot = blk * kKv8Block + threadIdx.x;
+        float w = 0.f;
+        if (slot < m) {
+            const int t = kept[slot];
+            if (t >= 0 && t < n) w = a.weights[b * a.w_stride[0] + h * a.w_stride[1] + t];
+        }
+        a.weights_out[bh * a.dst.capacity + slot] = w;
+    }
+    if (blk == 0 && blockIdx.y == 0 && threadIdx.x == 0) a.lengths_out[b] = m;
+    if (blk * kKv8Block >= m) return;
+    const bool complete = (blk + 1) * kKv8Block <= m;
+    const int chunk = threadIdx.x & 15, row0 = threadIdx.x >> 4;
+    float x[4][8];
+    float top = 0.f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const int slot = blk * kKv8Block + row0 + 16 * i;
+        const int t = slot < m ? kept[slot] : -1;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
+        if (t >= 0 && t < n) token_values<FMT>(a.src, which, bh, t, n, chunk, x[i]);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[i][j]));
+    }
+    if (complete) {
+        top = block_max<kStoreThreads>(top, red);
+        const float scale = scale_of<FMT>(top);
+        uint8_t* codes = static_cast<uint8_t*>(which ? a.dst.v : a.dst.k) + (bh * a.dst.capacity + (size_t)blk * kKv8Block) * kKv8Dim;
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            *reinterpret_cast<uint2*>(codes + (row0 + 16 * i) * kKv8Dim + chunk * 8) = values_to_codes<FMT>(x[i], scale);
+        if (threadIdx.x == 0) (which ? a.dst.v_scale : a.dst.k_scale)[bh * (a.dst.capacity / kKv8Block) + blk] = scale;
+    } else {
+        __nv_bfloat16* tail = static_cast<__nv_bfloat16*>(which ? a.dst.v_tail : a.dst.k_tail) + bh * (kKv8Block * kKv8Dim);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (blk * kKv8Block + row0 + 16 * i < m)
+                *reinterpret_cast<uint4*>(tail + (row0 + 16 * i) * kKv8Dim + chunk * 8) = pack_bf16x8(x[i]);
+    }
+}
+
+}  // namespace minf
+
+using namespace minf;
+
+extern "C" int minf_kv8_store(
+    const minf_kv8_cache* cache, const void* key, const void* value, const int64_t k_strides[3], const int64_t v_strides[3],
+    int n_tokens, const int32_t* start, int start_all, const int32_t* counts, void* stream) {
+    if (int rc = kv8_check(cache)) return rc;
+    if (n_tokens && (!key || !value || !k_strides || !v_strides)) return fail(MINF_E_ARG, "null pointer argument");
+    if (n_tokens < 0) return fail(MINF_E_ARG, "n_tokens must not be negative (got %d)", n_tokens);
+    if (!start && (start_all < 0 || start_all > cache->capacity)) return fail(MINF_E_ARG, "start %d is outside the cache of %d tokens", start_all, cache->capacity);
+    if (!start && !counts && n_tokens > cache->capacity - start_all)
+        return fail(MINF_E_ARG, "%d tokens from position %d do not fit a cache of %d", n_tokens, start_all, cache->capacity);
+    if (n_tokens == 0) return MINF_OK;
+    StoreArgs a{};
+    a.c = *cache;
+    a.src[0] = static_cast<const __nv_bfloat16*>(key);
+    a.src[1] = static_cast<const __nv_bfloat16*>(value);
+    for (int i = 0; i < 3; ++i) {
+        a.stride[0][i] = k_strides[i];
+        a.stride[1][i] = v_strides[i];
+        if (k_strides[i] % 8 || v_strides[i] % 8) return fail(MINF_E_ARG, "strides must be multiples of 8 elements");
+    }
+    if ((reinterpret_cast<uintptr_t>(key) | reinterpret_cast<uintptr_t>(value)) & 15) return fail(MINF_E_ARG, "keys and values must be 16-byte aligned");
+    a.n_tokens = n_tokens;
+    a.start = start;
+    a.start_all = start_all;
+    a.counts = counts;
+    // the last position decides how many blocks can be touched: a start anywhere in its block, clipped by the capacity
+    const int blocks = (int)min((long long)cache->capacity / kKv8Block, ((long long)n_tokens + 2 * kKv8Block - 2) / kKv8Block);
+    dim3 grid(blocks, 2 * cache->heads, cache->batch);
+    if (cache->format == MINF_KV8_E4M3)
+        kv8_store_kernel<MINF_KV8_E4M3><<<grid, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    else
+        kv8_store_kernel<MINF_KV8_INT8><<<grid, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    MINF_LAUNCH_OK("kv8_store_kernel");
+    return MINF_OK;
+}
+
+extern "C" int minf_kv8_load(
+    const minf_kv8_cache* cache, const int32_t* lengths, int length_all, const int32_t* first, int first_all, int count,
+    void* k_out, void* v_out, void* stream) {
+    if (int rc = kv8_check(cache)) return rc;
+    if (count < 0 || count > (1 << 30)) return fail(MINF_E_ARG, "bad count %d", count);
+    if (!lengths && (length_all < 0 || length_all > cache->capacity)) return fail(MINF_E_ARG, "length %d is outside the cache of %d tokens", length_all, cache->capacity);
+    if (count == 0) return MINF_OK;
+    if (!k_out || !v_out) return fail(MINF_E_ARG, "null pointer argument");
+    if ((reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out)) & 15) return fail(MINF_E_ARG, "outputs must be 16-byte aligned");
+    LoadArgs a{};
+    a.c = *cache;
+    a.lengths = lengths;
+    a.length_all = length_all;
+    a.first = first;
+    a.first_all = first_all;
+    a.count = count;
+    a.out[0] = static_cast<__nv_bfloat16*>(k_out);
+    a.out[1] = static_cast<__nv_bfloat16*>(v_out);
+    dim3 grid((count + kKv8Block - 1) / kKv8Block, 2 * cache->heads, cache->batch);
+    if (cache->format == MINF_KV8_E4M3)
+        kv8_load_kernel<MINF_KV8_E4M3><<<grid, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    else
+        kv8_load_kernel<MINF_KV8_INT8><<<grid, kStoreThreads, 0, static_cast<cudaStream_t>(stream)>>>(a);
+    MINF_LAUNCH_OK("kv8_load_kernel");
+    return MINF_OK;
+}
+
+extern "C" int minf_kv8_evict(
+    const minf_kv8_cache* src, const minf_kv8_cache* dst, const int32_t* lengths, int length_all, int max_length,
+    const float* weights, const int64_t w_strides[2], int budget, int recent, int sink,
+    int32_t* kept, float* weights_out, int32_t* lengths_out, void* stream) {
+    if (int rc = kv8_check(src)) return rc;
+    if (int rc = kv8_check(dst)) return rc;
+    if (!weights || !w_strides || !kept || !weights_out || !lengths_out) return fail(MINF_E_ARG, "null pointer argument");
+    if (src->format != dst->format || src->batch != dst->batch || src->heads != dst->heads)
+        return fail(MINF_E_ARG, "the two caches must have one format, batch and head count");
+    if (src->k == dst->k || src->v == dst->v || src->k_tail == dst->k_tail || src->v_tail == dst->v_tail)
+        return fail(MINF_E_ARG, "eviction writes into another cache than it reads");
+    if (budget < 1 || recent < 0 || sink < 0 || (long long)recent + sink > budget)
+        return fail(MINF_E_ARG, "budget %d must hold the %d first and %d last tokens", budget, sink, recent);
+    if (budget > dst->capacity) return fail(MINF_E_ARG, "budget %d does not fit a cache of %d tokens", budget, dst->capacity);
+    if (!lengths && (length_all < 0 || length_all > max_length)) return fail(MINF_E_ARG, "length %d is outside [0, max_length %d]", length_all, max_length);
+    if (max_length < 0 || max_length > src->capacity) return fail(MINF_E_ARG, "max_length %d is outside the cache of %d tokens", max_length, src->capacity);
+    cudaStream_t s = static_cast<cudaStream_t>(stream);
+    SelectArgsKv8 a{};
+    a.c = *src;
+    a.lengths = lengths;
+    a.length_all = length_all;
+    a.max_length = max_length;
+    a.weights = weights;
+    a.w_stride[0] = w_strides[0];
+    a.w_stride[1] = w_strides[1];
+    a.budget = budget;
+    a.recent = recent;
+    a.sink = sink;
+    a.kept = kept;
+    kv8_select_kernel<<<dim3(src->heads, src->batch), kSelectThreads, 0, s>>>(a);
+    MINF_LAUNCH_OK("kv8_select_kernel");
+    GatherArgs g{};
+    g.src = *src;
+    g.dst = *dst;
+    g.lengths = lengths;
+    g.length_all = length_all;
+    g.max_length = max_length;
+    g.weights = weights;
+    g.w_stride[0] = w_strides[0];
+    g.w_stride[1] = w_strides[1];
+    g.budget = budget;
+    g.kept = kept;
+    g.weights_out = weights_out;
+    g.lengths_out = lengths_out;
+    dim3 grid(dst->capacity / kKv8Block, 2 * src->heads, src->batch);
+    if (src->format == MINF_KV8_E4M3) kv8_gather_kernel<MINF_KV8_E4M3><<<grid, kStoreThreads, 0, s>>>(g);
+    else kv8_gather_kernel<MINF_KV8_INT8><<<grid, kStoreThreads, 0, s>>>(g);
+    MINF_LAUNCH_OK("kv8_gather_kernel");
+    return MINF_OK;
+}

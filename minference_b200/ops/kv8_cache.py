@@ -1,0 +1,225 @@
+"""The 8-bit key/value cache of one layer and the operators over it: store, load, attention, eviction.
+
+What the sparse prefill leaves behind is the K and V of a long prompt, and every decoding step reads all of it.  Here
+it is held in 8 bits (e4m3 or int8) with one fp32 scale for each block of 64 tokens of a head; the tokens behind the
+last complete block stay in bf16 until their block fills.  The attention weights that decoding gives each token can be
+summed up on the way, and ``kv8_evict`` keeps the tokens that hold most of them.
+
+Sequences of a batch may hold different numbers of tokens.  Lengths and positions are Python integers (checked here)
+or int32 tensors ``[B]`` on the device, which keeps a decoding step free of synchronisation and fit for a CUDA graph; a
+value that does not fit is then reported in ``cache.status`` (``cache.check()`` raises for it) and clipped.
+The reference has no counterpart (its quantised cache is a 2-bit one of another package).
+"""
+from __future__ import annotations
+
+import ctypes
+
+import torch
+
+from .. import _cabi
+
+BLOCK = 64          # tokens that share a scale
+HEAD_DIM = 128
+_FORMATS = {torch.float8_e4m3fn: _cabi.KV8_E4M3, torch.int8: _cabi.KV8_INT8}
+
+
+def _fail(msg: str):
+    raise _cabi.MInferB200Error(msg)
+
+
+class KV8Cache:
+    """Tensors of one layer's cache: ``k, v [B, Hkv, capacity, 128]`` codes (``torch.float8_e4m3fn`` or ``torch.int8``),
+    ``k_scale, v_scale [B, Hkv, capacity / 64]`` fp32, ``k_tail, v_tail [B, Hkv, 64, 128]`` bf16 (token t of the last,
+    incomplete block in row ``t % 64``), all contiguous on one CUDA device.  The number of tokens held is the caller's
+    (it is an argument of every call), so one cache serves captured graphs whose lengths change between replays."""
+
+    def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
+        _cabi.require_cuda(k, v, k_scale, v_scale, k_tail, v_tail)
+        if k.dtype not in _FORMATS or v.dtype != k.dtype:
+            _fail(f"cache codes must both be float8_e4m3fn or int8 (got {k.dtype}, {v.dtype})")
+        if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] % BLOCK or k.shape[2] == 0:
+            _fail(f"cache codes must be [B, Hkv, capacity, {HEAD_DIM}] with a capacity that is a multiple of {BLOCK} (got {tuple(k.shape)})")
+        b, h, cap, d = k.shape
+        for t, shape, dtype in ((v, k.shape, k.dtype), (k_scale, (b, h, cap // BLOCK), torch.float32), (v_scale, (b, h, cap // BLOCK), torch.float32),
+                                (k_tail, (b, h, BLOCK, d), torch.bfloat16), (v_tail, (b, h, BLOCK, d), torch.bfloat16)):
+            if t.shape != torch.Size(shape) or t.dtype != dtype:
+                _fail(f"cache tensor {tuple(t.shape)} {t.dtype} where {tuple(shape)} {dtype} was expected")
+        for t in (k, v, k_scale, v_scale, k_tail, v_tail):
+            if not t.is_contiguous() or t.data_ptr() % 16:
+                _fail("cache tensors must be contiguous and 16-byte aligned")
+            if t.device != k.device:
+                _fail("cache tensors must be on one device")
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
+        self.batch, self.kv_heads, self.capacity, self.dtype, self.device = b, h, cap, k.dtype, k.device
+        self.status = _cabi.new_status(k.device)
+        p = [t.data_ptr() for t in (k, v, k_scale, v_scale, k_tail, v_tail, self.status)]
+        self._desc = _cabi.Kv8Desc(*p, b, h, cap, _FORMATS[k.dtype])
+        self._ref = ctypes.byref(self._desc)
+
+    @classmethod
+    def empty(cls, batch: int, kv_heads: int, capacity: int, dtype=torch.float8_e4m3fn, device="cuda"):
+        """A cache with room for ``capacity`` tokens (rounded up to whole blocks)."""
+        if batch < 1 or kv_heads < 1 or capacity < 1:
+            _fail(f"bad cache sizes: batch {batch}, kv_heads {kv_heads}, capacity {capacity}")
+        cap = (capacity + BLOCK - 1) // BLOCK * BLOCK
+        codes = lambda: torch.empty((batch, kv_heads, cap, HEAD_DIM), dtype=dtype, device=device)
+        scale = lambda: torch.empty((batch, kv_heads, cap // BLOCK), dtype=torch.float32, device=device)
+        tail = lambda: torch.empty((batch, kv_heads, BLOCK, HEAD_DIM), dtype=torch.bfloat16, device=device)
+        return cls(codes(), codes(), scale(), scale(), tail(), tail())
+
+    def check(self) -> None:
+        """Synchronising check that every length and position so far fitted; clears what it reports."""
+        bits = int(self.status[_cabi.ST_ERROR])
+        if bits:
+            self.status.zero_()
+            _fail(f"8-bit cache: device reported error bits {bits:#x} (16 = a length or position outside the cache of "
+                  f"{self.capacity} tokens, or outside max_length)")
+
+    def nbytes(self) -> int:
+        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
+
+
+def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
+    """(device pointer or None, host value, tensor to keep alive) of an int or an int32 tensor ``[B]``."""
+    if isinstance(x, torch.Tensor):
+        if x.dtype != torch.int32 or x.shape != (cache.batch,) or x.device != cache.device or not x.is_contiguous():
+            _fail(f"{what} must be an int or a contiguous int32 tensor [{cache.batch}] on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})")
+        return x.data_ptr(), 0
+    x = int(x)
+    if not low <= x <= high:
+        _fail(f"{what} {x} is outside [{low}, {high}]")
+    return None, x
+
+
+def _rows(t: torch.Tensor, what: str, cache: KV8Cache):
+    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or t.device != cache.device:
+        _fail(f"{what} must be bf16 [{cache.batch}, heads, tokens, {HEAD_DIM}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+    if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+        t = t.contiguous()
+    return t
+
+
+def _strides2(t: torch.Tensor):
+    return (ctypes.c_int64 * 3)(t.stride(0), t.stride(1), 0)
+
+
+def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
+    """Append tokens ``key, value [B, Hkv, n, 128]`` (bf16) behind the ``start`` tokens each sequence holds (an int or an
+    int32 tensor ``[B]``); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
+    same call.  A block that fills is quantised from its 64 tokens' bf16 values.  Only the touched blocks are written."""
+    key, value = _rows(key, "key", cache), _rows(value, "value", cache)
+    if key.shape[1] != cache.kv_heads or key.shape != value.shape:
+        _fail(f"key and value must be [{cache.batch}, {cache.kv_heads}, n, {HEAD_DIM}] both (got {tuple(key.shape)}, {tuple(value.shape)})")
+    n = key.shape[2]
+    dev_counts = None
+    if counts is not None:
+        if not isinstance(counts, torch.Tensor):
+            _fail("counts must be an int32 tensor")
+        dev_counts, _ = _per_sequence(cache, counts, "counts", 0, n)
+    dev_start, start = _per_sequence(cache, start, "start", 0, cache.capacity - (n if counts is None else 0))
+    with torch.cuda.device(cache.device):
+        _cabi.check(_cabi.lib().minf_kv8_store(cache._ref, key.data_ptr(), value.data_ptr(), _cabi.strides3(key), _cabi.strides3(value),
+                                               n, dev_start, start, dev_counts, _cabi.stream_ptr(cache.device)))
+
+
+def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
+    """Values of tokens ``first .. first + count`` (``count=None``: to the end of the capacity) as ``(k, v)``, bf16
+    ``[B, Hkv, count, 128]``; zeros outside ``[0, length)``.  ``lengths`` and ``first``: int or int32 tensor ``[B]``."""
+    dev_n, n = _per_sequence(cache, lengths, "lengths", 0, cache.capacity)
+    dev_first, first = _per_sequence(cache, first, "first", -(1 << 30), 1 << 30)
+    if count is None:
+        count = cache.capacity - first
+    if count < 0:
+        _fail(f"count {count} must not be negative")
+    shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    with torch.cuda.device(cache.device):
+        _cabi.check(_cabi.lib().minf_kv8_load(cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr(),
+                                              _cabi.stream_ptr(cache.device)))
+    return k, v
+
+
+def _weights_arg(t, what: str, cache: KV8Cache, max_length: int):
+    if t.dtype != torch.float32 or t.dim() != 3 or t.shape[:2] != (cache.batch, cache.kv_heads) or t.shape[2] < max_length or t.device != cache.device:
+        _fail(f"{what} must be fp32 [{cache.batch}, {cache.kv_heads}, >= {max_length}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
+    if t.stride(2) != 1 and t.shape[2] > 1:
+        _fail(f"{what} must be contiguous along its tokens")
+
+
+def _max_length(cache: KV8Cache, lengths, max_length):
+    if max_length is None:
+        return cache.capacity if isinstance(lengths, torch.Tensor) else int(lengths)
+    if not 0 <= max_length <= cache.capacity:
+        _fail(f"max_length {max_length} is outside [0, {cache.capacity}]")
+    return int(max_length)
+
+
+def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int | None = None, sm_scale: float | None = None,
+                  weights: torch.Tensor | None = None, add_to: torch.Tensor | None = None, return_lse: bool = False):
+    """Attention of the last S tokens of every sequence, ``query [B, H, S, 128]`` (bf16, H a multiple of the cache's
+    heads), over the cache that already holds them: query i of a sequence of n tokens sees its first ``n - S + 1 + i``.
+    Returns ``[B, H, S, 128]`` bf16 and, with ``return_lse``, the base-2 log-sum-exp of the scaled logits, fp32
+    ``[B, H, S]``.  A row that sees nothing gives zeros and -inf.
+
+    ``lengths``: int or int32 tensor ``[B]``, the new tokens included; ``max_length``: an upper bound of them known on the
+    host (the capacity if not given), by which the work is split and scratch memory sized.
+    ``weights [B, Hkv, >= max_length]`` fp32 receives the attention weight of each token -- the probabilities summed over
+    the head's queries -- plus ``add_to`` (``add_to=weights`` sums up in place); entries behind a sequence's length are
+    left as they were.
+    """
+    query = _rows(query, "query", cache)
+    b, hq, s, d = query.shape
+    if s < 1 or hq % cache.kv_heads:
+        _fail(f"query must be [B, H, S >= 1, {HEAD_DIM}] with H a multiple of {cache.kv_heads} (got {tuple(query.shape)})")
+    longest = _max_length(cache, lengths, max_length)
+    dev_n, n = _per_sequence(cache, lengths, "lengths", 0, longest)
+    if weights is not None:
+        _weights_arg(weights, "weights", cache, longest)
+    if add_to is not None:
+        if weights is None:
+            _fail("add_to without weights")
+        _weights_arg(add_to, "add_to", cache, longest)
+    L = _cabi.lib()
+    out = torch.empty((b, hq, s, d), dtype=query.dtype, device=cache.device)
+    lse = torch.empty((b, hq, s), dtype=torch.float32, device=cache.device) if return_lse else None
+    nbytes = L.minf_kv8_attention_scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
+    scratch = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
+    with torch.cuda.device(cache.device):
+        _cabi.check(L.minf_kv8_attention(
+            cache._ref, query.data_ptr(), _cabi.strides3(query), out.data_ptr(), _cabi.strides3(out), hq, s, dev_n, n, longest,
+            float(d ** -0.5 if sm_scale is None else sm_scale), _cabi.ptr(lse),
+            _cabi.ptr(weights), None if weights is None else _strides2(weights),
+            _cabi.ptr(add_to), None if add_to is None else _strides2(add_to), _cabi.ptr(scratch), _cabi.stream_ptr(cache.device)))
+    return (out, lse) if return_lse else out
+
+
+def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, recent: int, sink: int = 0,
+              max_length: int | None = None, out: KV8Cache | None = None):
+    """Keep ``budget`` tokens of every head: the first ``sink``, the last ``recent`` and those with the largest ``weights
+    [B, Hkv, >= max_length]`` (fp32, as ``kv8_attention`` sums them up) of the others; equal weights: the earlier token.
+    Sequences of ``budget`` tokens or fewer are copied.
+
+    Writes into ``out`` (another cache of the same type, batch and heads; a new one with room for ``budget`` tokens if not
+    given) and returns ``(out, lengths int32 [B], weights fp32 [B, Hkv, out.capacity] -- zeros behind the last --, kept int32
+    [B, Hkv, budget] -- old positions, ascending, -1 behind the last)``.  Keys keep the rotary phase they were stored
+    with: the caller goes on counting positions from the full sequence."""
+    budget, recent, sink = int(budget), int(recent), int(sink)
+    if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget:
+        _fail(f"budget {budget} must hold the {sink} first and {recent} last tokens")
+    longest = _max_length(cache, lengths, max_length)
+    dev_n, n = _per_sequence(cache, lengths, "lengths", 0, longest)
+    _weights_arg(weights, "weights", cache, longest)
+    if out is None:
+        out = KV8Cache.empty(cache.batch, cache.kv_heads, budget, cache.dtype, cache.device)
+    elif out is cache or (out.batch, out.kv_heads, out.dtype, out.device) != (cache.batch, cache.kv_heads, cache.dtype, cache.device) or out.capacity < budget:
+        _fail("out must be another cache of the same batch, heads, type and device with room for the budget")
+    dev = cache.device
+    kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=dev)
+    weights_out = torch.empty((cache.batch, cache.kv_heads, out.capacity), dtype=torch.float32, device=dev)
+    lengths_out = torch.empty((cache.batch,), dtype=torch.int32, device=dev)
+    with torch.cuda.device(dev):
+        _cabi.check(_cabi.lib().minf_kv8_evict(
+            cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides2(weights), budget, recent, sink,
+            kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr(), _cabi.stream_ptr(dev)))
+    return out, lengths_out, weights_out, kept

@@ -1,0 +1,90 @@
+"""Host-side checks of the 8-bit cache operators: what is refused before anything reaches the device (no GPU needed)."""
+import ctypes
+
+import pytest
+import torch
+
+
+def _desc(cabi, **kw):
+    d = dict(k=256, v=512, k_scale=1024, v_scale=2048, k_tail=4096, v_tail=8192, status=64, batch=1, heads=2, capacity=128, format=0)
+    d.update(kw)
+    return cabi.Kv8Desc(*[d[n] for n, _ in cabi.Kv8Desc._fields_])
+
+
+@pytest.fixture()
+def cabi(built_lib):
+    from minference_b200 import _cabi
+
+    return _cabi
+
+
+@pytest.mark.parametrize("change, word", [
+    ({"k": 0}, b"null"), ({"status": 0}, b"null"), ({"batch": 0}, b"sizes"), ({"heads": 0}, b"sizes"), ({"capacity": 0}, b"capacity"),
+    ({"capacity": 100}, b"capacity"), ({"format": 7}, b"format"), ({"v": 520}, b"aligned"), ({"k_tail": 4104}, b"aligned")])
+def test_descriptor_checks(cabi, change, word):
+    lib = cabi.lib()
+    d = ctypes.byref(_desc(cabi, **change))
+    st = (ctypes.c_int64 * 3)(256, 128, 128)
+    assert lib.minf_kv8_store(d, 256, 256, st, st, 1, None, 0, None, None) == -1 and word in lib.minf_last_error()
+    assert lib.minf_kv8_load(d, None, 0, None, 0, 1, 256, 256, None) == -1 and word in lib.minf_last_error()
+    assert lib.minf_kv8_attention(d, 256, st, 256, st, 2, 1, None, 0, 0, 1.0, None, None, None, None, None, 256, None) == -1
+    assert word in lib.minf_last_error()
+
+
+def test_store_checks(cabi):
+    lib, d = cabi.lib(), ctypes.byref(_desc(cabi))
+    ok = (ctypes.c_int64 * 3)(256, 128, 128)
+    odd = (ctypes.c_int64 * 3)(256, 129, 128)
+    for args, word in [((0, 256, ok, ok, 1, None, 0, None), b"null"), ((256, 264, ok, ok, 1, None, 0, None), b"aligned"),
+                       ((256, 256, ok, odd, 1, None, 0, None), b"strides"), ((256, 256, ok, ok, -1, None, 0, None), b"n_tokens"),
+                       ((256, 256, ok, ok, 1, None, 128, None), b"fit"), ((256, 256, ok, ok, 1, None, -1, None), b"outside"),
+                       ((256, 256, ok, ok, 129, None, 0, None), b"fit")]:
+        assert lib.minf_kv8_store(d, *args, None) == -1 and word in lib.minf_last_error(), args
+    assert lib.minf_kv8_store(d, 256, 256, ok, ok, 0, None, 128, None, None) == 0        # nothing to store: no launch
+
+
+def test_load_checks(cabi):
+    lib, d = cabi.lib(), ctypes.byref(_desc(cabi))
+    for args, word in [((None, 129, None, 0, 1, 256, 256), b"outside"), ((None, 1, None, 0, -1, 256, 256), b"count"),
+                       ((None, 1, None, 0, 1, 0, 256), b"null"), ((None, 1, None, 0, 1, 256, 264), b"aligned")]:
+        assert lib.minf_kv8_load(d, *args, None) == -1 and word in lib.minf_last_error(), args
+    assert lib.minf_kv8_load(d, None, 1, None, 0, 0, None, None, None) == 0
+
+
+def test_attention_checks(cabi):
+    lib, d = cabi.lib(), ctypes.byref(_desc(cabi))
+    st = (ctypes.c_int64 * 3)(512, 128, 128)
+    bad = (ctypes.c_int64 * 3)(512, 130, 128)
+    w = (ctypes.c_int64 * 3)(128, 128, 0)
+    base = dict(q=256, qs=st, o=256, os=st, hq=4, n_q=1, lengths=None, n=100, longest=128, scale=1.0, lse=None, weights=None, ws=None,
+                add=None, adds=None, scratch=256)
+    for change, word in [({"q": 0}, b"null"), ({"o": 0}, b"null"), ({"hq": 3}, b"sizes"), ({"hq": 0}, b"sizes"), ({"n_q": 0}, b"sizes"),
+                         ({"longest": 129}, b"max_length"), ({"longest": -1}, b"sizes"), ({"n": 129}, b"outside"), ({"n": -1}, b"outside"),
+                         ({"scratch": 0}, b"scratch"), ({"scratch": 264}, b"aligned"), ({"os": bad}, b"strides"), ({"o": 260}, b"aligned"),
+                         ({"weights": 256}, b"null"), ({"add": 256}, b"null"), ({"add": 256, "adds": w}, b"add_to")]:
+        a = {**base, **change}
+        if "scratch" in change and not change["scratch"]:
+            a.update(weights=256, ws=w)              # weights always need scratch
+        assert lib.minf_kv8_attention(d, *a.values(), None) == -1 and word in lib.minf_last_error(), (change, lib.minf_last_error())
+    assert lib.minf_kv8_attention_scratch_bytes(1, 3, 2, 1, 128, 0) == 0
+    assert lib.minf_kv8_attention_scratch_bytes(1, 4, 2, 1, 128, 1) >= 2 * 128 * 2 * 4
+
+
+def test_evict_checks(cabi):
+    lib = cabi.lib()
+    src, dst = _desc(cabi), _desc(cabi, k=1 << 20, v=2 << 20, k_tail=3 << 20, v_tail=4 << 20, capacity=64)
+    w = (ctypes.c_int64 * 3)(128, 128, 0)
+    def call(s=src, d=dst, n=128, longest=128, weights=256, budget=32, recent=8, sink=4, kept=256):
+        return lib.minf_kv8_evict(ctypes.byref(s), ctypes.byref(d), None, n, longest, weights, w, budget, recent, sink, kept, 256, 256, None)
+    for kw, word in [(dict(d=src), b"another"), (dict(d=_desc(cabi, k=1 << 20, v=2 << 20, k_tail=3 << 20, v_tail=4 << 20, format=1)), b"format"),
+                     (dict(budget=0), b"budget"), (dict(recent=30), b"budget"), (dict(sink=-1), b"budget"), (dict(recent=-1), b"budget"),
+                     (dict(budget=65), b"fit"), (dict(n=129), b"outside"), (dict(longest=129), b"max_length"), (dict(weights=0), b"null"),
+                     (dict(kept=0), b"null")]:
+        assert call(**kw) == -1 and word in lib.minf_last_error(), (kw, lib.minf_last_error())
+
+
+def test_no_cpu_path(cabi):
+    from minference_b200 import KV8Cache
+
+    with pytest.raises(cabi.MInferB200Error):
+        KV8Cache.empty(1, 1, 64, device="cpu")
