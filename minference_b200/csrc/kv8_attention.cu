@@ -28,6 +28,9 @@ namespace minf {
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kSMs = 148;
+constexpr int kSlotBytes = kKv8Block * kKv8Dim;     // keys or values of a block
+constexpr int kRingSlots = 3;
+constexpr int kRingBytes = kAttnWarps * kRingSlots * kSlotBytes;
 
 struct Kv8AttnArgs {
     minf_kv8_cache c;
@@ -92,11 +95,11 @@ struct Rows {
     int lim[NT][2];                 // tokens below this are seen
 };
 
-// Logits of 16 * SUB tokens -> P, with the running statistics moved on.  s[j][nt][e]: token t0 + 16 j + g (+ 8 for e = 2, 3),
+// Logits of 16 * SUB tokens -> P, with the running statistics moved on.  s[j][nt][e]: token t0 + 16 j + tg (+ 8 for e = 2, 3),
 // column 2c (+ 1 for odd e).  On return s holds P.
 template <int NT, int SUB>
 __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, float (&s)[SUB][NT][4], float k_scale, float v_scale,
-                                             int t0, bool masked, int end, size_t bh, int row0, int g, int c) {
+                                             int t0, bool masked, int end, size_t bh, int row0, int tg, int c) {
     const float lv = log2f(v_scale), inv_v = 1.f / v_scale;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -110,14 +113,14 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             x[2] *= f0;
             x[3] *= f1;
             if (masked) {
-                const int t = t0 + 16 * j + g;
+                const int t = t0 + 16 * j + tg;
                 if (t >= R.lim[nt][0]) x[0] = -CUDART_INF_F;
                 if (t >= R.lim[nt][1]) x[1] = -CUDART_INF_F;
                 if (t + 8 >= R.lim[nt][0]) x[2] = -CUDART_INF_F;
                 if (t + 8 >= R.lim[nt][1]) x[3] = -CUDART_INF_F;
             }
             if (a.logits) {
-                const int col = row0 + 8 * nt + 2 * c, t = t0 + 16 * j + g;
+                const int col = row0 + 8 * nt + 2 * c, t = t0 + 16 * j + tg;
                 if (col < a.pitch) {
                     float* p = a.logits + ((long long)bh * a.tokens + t) * a.pitch + col;
                     if (t < end) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
@@ -166,7 +169,7 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
 }
 
 // O^T += V^T P^T for 16 tokens of one column group.  v[i][0..3]: the A fragment of dims 16g+2i, 16g+2i+1 (rows g and
-// g + 8 of the product).  Where a value of a token that some column does not see may be infinite or NaN, the product
+// g + 8 of the product), for tokens ta, tb in the halves of a register and ta + 8, tb + 8.  Where a value of a token that some column does not see may be infinite or NaN, the product
 // is taken column by column with the unseen tokens' values left out: zero times them would not be zero.
 template <bool BF16>
 __device__ __forceinline__ void pv_mma(float (&d)[4], const uint32_t (&v)[4], uint32_t b0, uint32_t b1) {
@@ -174,7 +177,7 @@ __device__ __forceinline__ void pv_mma(float (&d)[4], const uint32_t (&v)[4], ui
     else mma_f16(d, v[0], v[1], v[2], v[3], b0, b1);
 }
 template <bool BF16, int NT>
-__device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], int nt, uint32_t b0, uint32_t b1, bool masked, int t0, int g, int c) {
+__device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], int nt, uint32_t b0, uint32_t b1, bool masked, int ta, int tb, int g, int c) {
     if (masked) {
         bool bad = false;
 #pragma unroll
@@ -185,8 +188,8 @@ __device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], 
             for (int col = 0; col < 8; ++col) {
                 const int l0 = __shfl_sync(0xffffffffu, R.lim[nt][0], col >> 1), l1 = __shfl_sync(0xffffffffu, R.lim[nt][1], col >> 1);
                 const int lim = (col & 1) ? l1 : l0;
-                const uint32_t k0 = (t0 + 2 * c < lim ? 0xffffu : 0u) | (t0 + 2 * c + 1 < lim ? 0xffff0000u : 0u);
-                const uint32_t k1 = (t0 + 2 * c + 8 < lim ? 0xffffu : 0u) | (t0 + 2 * c + 9 < lim ? 0xffff0000u : 0u);
+                const uint32_t k0 = (ta < lim ? 0xffffu : 0u) | (tb < lim ? 0xffff0000u : 0u);
+                const uint32_t k1 = (ta + 8 < lim ? 0xffffu : 0u) | (tb + 8 < lim ? 0xffff0000u : 0u);
                 const uint32_t c0 = g == col ? b0 : 0u, c1 = g == col ? b1 : 0u;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
@@ -212,7 +215,8 @@ __device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], 
 
 template <int FMT, int NT>
 __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    constexpr int SUB = 4 / NT;                     // sub-tiles of 16 tokens per softmax step: 16 logits a lane for every NT
+    constexpr int SUB = 4 / NT;                     // sub-tiles of 16 tokens per softmax step: up to 16 logits a lane
+    constexpr int PARTS = 4 / SUB;                  // softmax steps of a block
     const int split = blockIdx.x, b = blockIdx.z;
     const int tiles = (a.rows + 8 * NT - 1) / (8 * NT);
     const int h = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * 8 * NT;
@@ -275,18 +279,67 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
     const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
     const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
 
+    // The warp's own ring of three slots of 8 KB: keys of a block, values of it, keys of its next block, ...; two
+    // copies are in flight while the third is used.  16-byte chunk ch of row r lies at ch ^ (r & 7).
+    extern __shared__ __align__(128) unsigned char ring_all[];
+    unsigned char* const ring = ring_all + warp * (kRingSlots * kSlotBytes);
+    const uint32_t ring_u = smem_u32(ring);
+    const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4)) << 4);
+    auto fetch = [&](int slot, const uint8_t* src) {
+        src += lane * 16;
+        const uint32_t dst = ring_u + slot * kSlotBytes;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) cp_async_16(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i);
+    };
+    // Row i of the eight of a fragment is token perm(i): with it, and the chunks' places above, the eight lanes of a
+    // quarter of a shared-memory access touch all 32 banks, for the keys' rows and for the values' alike.
+    const int pg = (g & 1) ? (g - 1) ^ 5 : g;       // perm(g)
+    const int pa = 2 * c, pb = (2 * c) ^ 5;         // perm(2c), perm(2c + 1)
+
+    const uint8_t* next_k = kc + (size_t)(blk_lo + warp) * kSlotBytes;
+    const uint8_t* next_v = vc + (size_t)(blk_lo + warp) * kSlotBytes;
+    constexpr size_t kHop = (size_t)kAttnWarps * kSlotBytes;
+    int slot = 0;
+    float k_scale = 1.f, v_scale = 1.f;
+    if (blk_lo + warp < blk_hi) {
+        fetch(0, next_k);
+        cp_async_commit();
+        fetch(1, next_v);
+        k_scale = ks[blk_lo + warp];
+        v_scale = vs[blk_lo + warp];
+    } else {
+        cp_async_commit();
+    }
+    cp_async_commit();
     for (int blk = blk_lo + warp; blk < blk_hi; blk += kAttnWarps) {
-        const float k_scale = ks[blk], v_scale = vs[blk];
+        const bool more = blk + kAttnWarps < blk_hi;
         const bool masked = (blk + 1) * kKv8Block > all_see;
+        const float ksc = k_scale, vsc = v_scale;
+        next_k += kHop;
+        next_v += kHop;
+        const int slot_v = slot == 2 ? 0 : slot + 1, slot_n = slot_v == 2 ? 0 : slot_v + 1;
+        if (more) {
+            fetch(slot_n, next_k);
+            k_scale = ks[blk + kAttnWarps];
+            v_scale = vs[blk + kAttnWarps];
+        }
+        cp_async_commit();
+        cp_async_wait<2>();
+        __syncwarp();
+        const unsigned char* kb = ring + slot * kSlotBytes;
+        const unsigned char* vb = ring + slot_v * kSlotBytes;
+        bool v_here = false;
 #pragma unroll 1
-        for (int part = 0; part < NT; ++part) {
+        for (int part = 0; part < PARTS; ++part) {
             const int t0 = blk * kKv8Block + part * SUB * 16;
             float s[SUB][NT][4];
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
-                const uint8_t* p = kc + (size_t)(t0 + 16 * j + g) * kKv8Dim + 16 * c;
-                const uint4 k00 = *reinterpret_cast<const uint4*>(p), k01 = *reinterpret_cast<const uint4*>(p + 64);
-                const uint4 k10 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim), k11 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim + 64);
+                const unsigned char* p = kb + (part * SUB * 16 + 16 * j + pg) * kKv8Dim;       // rows pg and pg + 8: the same r & 7
+                const uint4 k00 = *reinterpret_cast<const uint4*>(p + ((c ^ pg) << 4));
+                const uint4 k01 = *reinterpret_cast<const uint4*>(p + (((c + 4) ^ pg) << 4));
+                const uint4 k10 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim + ((c ^ pg) << 4));
+                const uint4 k11 = *reinterpret_cast<const uint4*>(p + 8 * kKv8Dim + (((c + 4) ^ pg) << 4));
                 const uint32_t r0[8] = {k00.x, k00.y, k00.z, k00.w, k01.x, k01.y, k01.z, k01.w};
                 const uint32_t r1[8] = {k10.x, k10.y, k10.z, k10.w, k11.x, k11.y, k11.z, k11.w};
 #pragma unroll
@@ -302,15 +355,21 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
                     for (int nt = 0; nt < NT; ++nt) mma_f16(s[j][nt], a0, a1, a2, a3, qf[nt][st][0], qf[nt][st][1]);
                 }
             }
-            softmax_step<NT, SUB>(a, R, s, k_scale, v_scale, t0, masked, n, bh, row0, g, c);
+            softmax_step<NT, SUB>(a, R, s, ksc, vsc, t0, masked, n, bh, row0, pg, c);
+            if (!v_here) {
+                cp_async_wait<1>();
+                __syncwarp();
+                v_here = true;
+            }
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
-                // A fragment of V^T: tokens 2c, 2c+1 (and + 8) in the halves of a register
+                // A fragment of V^T: two tokens in the halves of a register
                 uint32_t v[8][4];
 #pragma unroll
                 for (int hf = 0; hf < 2; ++hf) {
-                    const uint8_t* p = vc + (size_t)(t0 + 16 * j + 2 * c + 8 * hf) * kKv8Dim + 16 * g;
-                    const uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + kKv8Dim);
+                    const unsigned char* p = vb + (part * SUB * 16 + 16 * j + 8 * hf) * kKv8Dim;
+                    const uint4 x = *reinterpret_cast<const uint4*>(p + pa * kKv8Dim + ((g ^ pa) << 4));
+                    const uint4 y = *reinterpret_cast<const uint4*>(p + pb * kKv8Dim + ((g ^ pb) << 4));
                     const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
 #pragma unroll
                     for (int w = 0; w < 4; ++w) {
@@ -321,10 +380,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
                     const uint32_t b0 = transpose8x8(pack_half2(s[j][nt][0], s[j][nt][1])), b1 = transpose8x8(pack_half2(s[j][nt][2], s[j][nt][3]));
-                    pv_step<false, NT>(R, v, nt, b0, b1, masked, t0 + 16 * j, g, c);
+                    pv_step<false, NT>(R, v, nt, b0, b1, masked, t0 + 16 * j + pa, t0 + 16 * j + pb, g, c);
                 }
             }
         }
+        __syncwarp();
+        // both slots are free: the values of the next block take the one the keys were in
+        if (more) fetch(slot, next_v);
+        cp_async_commit();
+        slot = slot_n;
     }
 
     // the tail: the last split's warps take 16 of its tokens each
@@ -376,14 +440,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
             const uint32_t h0 = pack_bf16x2(x[0], x[1]), h1 = pack_bf16x2(x[2], x[3]);
             const uint32_t e0 = pack_bf16x2(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xffff0000u));
             const uint32_t e1 = pack_bf16x2(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xffff0000u));
-            pv_step<true, NT>(R, v, nt, transpose8x8(h0), transpose8x8(h1), true, t0, g, c);
-            pv_step<true, NT>(R, v, nt, transpose8x8(e0), transpose8x8(e1), true, t0, g, c);
+            pv_step<true, NT>(R, v, nt, transpose8x8(h0), transpose8x8(h1), true, t0 + 2 * c, t0 + 2 * c + 1, g, c);
+            pv_step<true, NT>(R, v, nt, transpose8x8(e0), transpose8x8(e1), true, t0 + 2 * c, t0 + 2 * c + 1, g, c);
         }
     }
 
     // join the warps, eight rows at a time
-    __shared__ __align__(16) float sm_o[kAttnWarps][8][kKv8Dim];
-    __shared__ float sm_lse[kAttnWarps][8];
+    __syncthreads();                                // the rings are read out
+    float (*sm_o)[8][kKv8Dim] = reinterpret_cast<float (*)[8][kKv8Dim]>(ring_all);
+    float (*sm_lse)[8] = reinterpret_cast<float (*)[8]>(ring_all + kAttnWarps * 8 * kKv8Dim * sizeof(float));
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
 #pragma unroll
@@ -525,11 +590,11 @@ struct AttnShape {
 static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
     AttnShape s{};
     const long long rows = (long long)(hq / heads) * n_q;
-    s.nt = rows <= 8 ? 1 : rows <= 16 ? 2 : 4;
+    s.nt = (int)std::min<long long>(4, (rows + 7) / 8);
     s.tiles = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
     const long long ctas = (long long)batch * heads * s.tiles;
     const long long blocks = max_length / kKv8Block;
-    long long splits = (4 * kSMs + ctas - 1) / ctas;
+    long long splits = (2 * kSMs + ctas - 1) / ctas;
     splits = std::min(splits, (blocks + kAttnWarps - 1) / kAttnWarps);
     s.splits = (int)std::max(splits, 1ll);
     s.pitch = (int)((rows + 1) / 2 * 2);
@@ -553,12 +618,23 @@ static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_le
     return batch >= 1 && heads >= 1 && hq >= heads && hq % heads == 0 && n_q >= 1 && max_length >= 0 && (long long)hq * n_q <= (1 << 24);
 }
 
+template <int FMT, int NT>
+static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+    // per device, and cheap: every call sets it
+    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<FMT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    if (e != cudaSuccess) return e;
+    kv8_attention_kernel<FMT, NT><<<dim3(s.splits, a.c.heads * s.tiles, a.c.batch), kAttnThreads, kRingBytes, stream>>>(a);
+    return cudaGetLastError();
+}
+
 template <int FMT>
-static void launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-    dim3 grid(s.splits, a.c.heads * s.tiles, a.c.batch);
-    if (s.nt == 1) kv8_attention_kernel<FMT, 1><<<grid, kAttnThreads, 0, stream>>>(a);
-    else if (s.nt == 2) kv8_attention_kernel<FMT, 2><<<grid, kAttnThreads, 0, stream>>>(a);
-    else kv8_attention_kernel<FMT, 4><<<grid, kAttnThreads, 0, stream>>>(a);
+static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+    switch (s.nt) {
+        case 1: return launch_attention<FMT, 1>(a, s, stream);
+        case 2: return launch_attention<FMT, 2>(a, s, stream);
+        case 3: return launch_attention<FMT, 3>(a, s, stream);
+        default: return launch_attention<FMT, 4>(a, s, stream);
+    }
 }
 
 }  // namespace minf
@@ -623,9 +699,8 @@ extern "C" int minf_kv8_attention(
         }
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (cache->format == MINF_KV8_E4M3) launch_attention<MINF_KV8_E4M3>(a, s, st);
-    else launch_attention<MINF_KV8_INT8>(a, s, st);
-    MINF_LAUNCH_OK("kv8_attention_kernel");
+    const cudaError_t e = cache->format == MINF_KV8_E4M3 ? launch_attention<MINF_KV8_E4M3>(a, s, st) : launch_attention<MINF_KV8_INT8>(a, s, st);
+    if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_attention_kernel failed: %s", cudaGetErrorString(e));
     if (s.splits > 1) {
         kv8_combine_kernel<<<(unsigned)((size_t)cache->batch * cache->heads * a.rows), 128, 0, st>>>(a);
         MINF_LAUNCH_OK("kv8_combine_kernel");
