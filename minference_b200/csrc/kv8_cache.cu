@@ -9,6 +9,8 @@
 // become the largest code.
 #include "kv8.cuh"
 
+#include <cooperative_groups.h>
+
 #include "sm100_ptx.cuh"
 
 namespace minf {
@@ -225,77 +227,153 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 }
 
 constexpr int kSelectThreads = 1024;
+constexpr int kSelectWarps = kSelectThreads / 32;
+constexpr int kSelectCluster = 8;                           // CTAs that share a head's tokens
+constexpr int kSelectBins = 2048;
+constexpr int kSelectCached = 40960;                        // keys a CTA keeps in shared memory
+constexpr int kSelectSmem = (kSelectBins + kSelectCached) * 4;
 
-// One CTA per (sequence, head): the key of the last token that is kept, by a radix select of four 8-bit digits, then
-// the kept tokens in ascending order.
-__global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
-    __shared__ uint32_t hist[256];
-    __shared__ uint32_t warp_count[2][32];
-    __shared__ uint32_t sh_prefix, sh_need;
-    const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+// A cluster per (sequence, head), each CTA a contiguous part of the candidates, whose keys it reads once and keeps in
+// shared memory (beyond 8 x 40960 candidates it reads them again from L2 in each pass).  Three passes of 11, 11 and 10
+// bits find the key of the last token that is kept; the histograms are summed over the cluster through distributed
+// shared memory and every CTA takes the same digit.  Then the warps, each with a contiguous stretch, count what they
+// keep and write it at the offset of everything before them: ascending order without a sort, equal keys by position.
+// What bounds it: the barriers of the three passes (two across the cluster each), not the 4 B a token it reads.
+__global__ void __cluster_dims__(kSelectCluster, 1, 1) __launch_bounds__(kSelectThreads)
+kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
+    extern __shared__ uint32_t dyn[];
+    uint32_t* hist = dyn;
+    uint32_t* cached = dyn + kSelectBins;
+    __shared__ uint32_t warp_sum[kSelectWarps];
+    __shared__ uint32_t sh_digit, sh_need;
+    __shared__ uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
+    __shared__ uint32_t cta_above, cta_equal;
+    namespace cg = cooperative_groups;
+    cg::cluster_group cluster = cg::this_cluster();
+    const int part = blockIdx.x % kSelectCluster, h = blockIdx.x / kSelectCluster, b = blockIdx.y;
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
     const float* w = a.weights + b * a.w_stride[0] + h * a.w_stride[1];
     int32_t* kept = a.kept + ((size_t)b * a.c.heads + h) * a.budget;
-    if (n <= a.budget) {                                    // everything stays
-        for (int i = tid; i < a.budget; i += kSelectThreads) kept[i] = i < n ? i : -1;
+    if (n <= a.budget) {                                    // everything stays (the whole cluster leaves here)
+        for (int i = part * kSelectThreads + tid; i < a.budget; i += kSelectCluster * kSelectThreads) kept[i] = i < n ? i : -1;
         return;
     }
     const int lo = a.sink, hi = n - a.recent;
+    for (int i = part * kSelectThreads + tid; i < a.sink + a.recent; i += kSelectCluster * kSelectThreads)
+        kept[i < a.sink ? i : a.budget - a.recent + (i - a.sink)] = i < a.sink ? i : hi + (i - a.sink);
     uint32_t need = a.budget - a.sink - a.recent;           // of hi - lo > need candidates
+    if (need == 0) return;
+    const int chunk = ((hi - lo + kSelectCluster - 1) / kSelectCluster + 31) / 32 * 32;
+    const int c0 = min(hi, lo + part * chunk), c1 = min(hi, c0 + chunk), count = c1 - c0;
+    const bool in_smem = count <= kSelectCached;
+    auto key_at = [&](int i) { return in_smem ? cached[i] : weight_key(w[c0 + i]); };
+
     uint32_t prefix = 0;
-    for (int shift = 24; shift >= 0 && need > 0; shift -= 8) {
-        if (tid < 256) hist[tid] = 0;
+#pragma unroll 1
+    for (int pass = 0; pass < 3; ++pass) {
+        const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
+        const uint32_t mask = (1u << bits) - 1u;
+        hist[tid] = 0;
+        hist[tid + kSelectThreads] = 0;
         __syncthreads();
-        for (int t = lo + tid; t < hi; t += kSelectThreads) {
-            const uint32_t key = weight_key(w[t]);
-            if (shift == 24 || (key >> (shift + 8)) == prefix) atomicAdd(&hist[(key >> shift) & 255], 1u);
+        for (int i0 = 0; i0 < count; i0 += 8 * kSelectThreads) {
+            uint32_t key[8];
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * kSelectThreads + tid;
+                if (i < count) key[u] = pass == 0 ? weight_key(w[c0 + i]) : key_at(i);
+            }
+#pragma unroll
+            for (int u = 0; u < 8; ++u) {
+                const int i = i0 + u * kSelectThreads + tid;
+                const bool live = i < count && (pass == 0 || (key[u] >> (shift + bits)) == prefix);
+                if (pass == 0 && in_smem && i < count) cached[i] = key[u];
+                const uint32_t bin = live ? (key[u] >> shift) & mask : 0xffffffffu;
+                // weights share their exponents: one addition for all lanes of a warp that hit the same bin
+                const uint32_t same = __match_any_sync(0xffffffffu, bin);
+                if (live && (__ffs(same) - 1) == lane) atomicAdd(&hist[bin], __popc(same));
+            }
         }
-        __syncthreads();
-        if (tid == 0) {
-            uint32_t left = need;
-            int d = 255;
-            while (d > 0 && hist[d] < left) left -= hist[d--];
-            sh_need = left;
-            sh_prefix = (prefix << 8) | (uint32_t)d;
+        cluster.sync();
+        // thread t sums bins 2046 - 2t and 2047 - 2t over the cluster: a scan over the threads runs from the largest key down
+        const int bin = kSelectBins - 2 - 2 * tid;
+        uint32_t x1 = 0, x0 = 0;
+#pragma unroll
+        for (int r = 0; r < kSelectCluster; ++r) {
+            const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
+            x0 += v.x;
+            x1 += v.y;
         }
+        uint32_t scan = x0 + x1;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
+            if (lane >= o) scan += y;
+        }
+        if (lane == 31) warp_sum[warp] = scan;
         __syncthreads();
-        prefix = sh_prefix;
+        uint32_t before = scan - x0 - x1;
+        for (int i = 0; i < warp; ++i) before += warp_sum[i];
+        if (before < need && need <= before + x1) {
+            sh_digit = bin + 1;
+            sh_need = need - before;
+        } else if (before + x1 < need && need <= before + x1 + x0) {
+            sh_digit = bin;
+            sh_need = need - before - x1;
+        }
+        cluster.sync();                                     // digit and histograms: read by all before the next pass clears them
+        prefix = (prefix << bits) | sh_digit;
         need = sh_need;
-        __syncthreads();
     }
     // keys above `prefix` are kept, and the first `need` that equal it
-    const bool any = a.budget > a.sink + a.recent;
-    uint32_t done = 0, ties_done = 0;
-    for (int t0 = 0; t0 < n; t0 += kSelectThreads) {
-        const int t = t0 + tid;
-        const bool forced = t < n && (t < lo || t >= hi);
-        const uint32_t key = t < n && !forced ? weight_key(w[t]) : 0u;
-        const bool cand = any && t < n && !forced;
-        const bool tie = cand && key == prefix;
-        const uint32_t tie_bits = __ballot_sync(0xffffffffu, tie);
-        if (lane == 0) warp_count[0][warp] = __popc(tie_bits);
-        __syncthreads();
-        uint32_t tie_rank = ties_done, ties_all = 0;
-        for (int i = 0; i < 32; ++i) {
-            if (i < warp) tie_rank += warp_count[0][i];
-            ties_all += warp_count[0][i];
-        }
-        tie_rank += __popc(tie_bits & ((1u << lane) - 1u));
-        const bool keep = forced || (cand && (key > prefix || (tie && tie_rank < need)));
-        const uint32_t keep_bits = __ballot_sync(0xffffffffu, keep);
-        if (lane == 0) warp_count[1][warp] = __popc(keep_bits);
-        __syncthreads();
-        uint32_t rank = done, all = 0;
-        for (int i = 0; i < 32; ++i) {
-            if (i < warp) rank += warp_count[1][i];
-            all += warp_count[1][i];
-        }
-        rank += __popc(keep_bits & ((1u << lane) - 1u));
-        if (keep && rank < (uint32_t)a.budget) kept[rank] = t;
-        done += all;
-        ties_done += ties_all;
-        __syncthreads();
+    const int seg = ((count + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
+    const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
+    uint32_t above = 0, equal = 0;
+    for (int i = s0 + lane; i < s1; i += 32) {
+        const uint32_t k = key_at(i);
+        above += k > prefix;
+        equal += k == prefix;
     }
+    above = __reduce_add_sync(0xffffffffu, above);
+    equal = __reduce_add_sync(0xffffffffu, equal);
+    if (lane == 0) {
+        warp_above[warp] = above;
+        warp_equal[warp] = equal;
+    }
+    __syncthreads();
+    if (warp == 0) {
+        const uint32_t ca = __reduce_add_sync(0xffffffffu, warp_above[lane]), ce = __reduce_add_sync(0xffffffffu, warp_equal[lane]);
+        if (lane == 0) {
+            cta_above = ca;
+            cta_equal = ce;
+        }
+    }
+    cluster.sync();
+    uint32_t gt = 0, eq = 0;                                // before this warp's stretch
+    for (int r = 0; r < part; ++r) {
+        gt += *cluster.map_shared_rank(&cta_above, r);
+        eq += *cluster.map_shared_rank(&cta_equal, r);
+    }
+    for (int i = 0; i < warp; ++i) {
+        gt += warp_above[i];
+        eq += warp_equal[i];
+    }
+    const uint32_t below_lane = (1u << lane) - 1u;
+    for (int i0 = s0; i0 < s1; i0 += 32) {
+        const int i = i0 + lane;
+        const uint32_t k = i < s1 ? key_at(i) : 0u;
+        const bool is_gt = i < s1 && k > prefix, is_eq = i < s1 && k == prefix;
+        const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
+        const uint32_t my_eq = eq + __popc(be & below_lane);
+        if (is_gt || (is_eq && my_eq < need)) {
+            const uint32_t at = a.sink + gt + __popc(bg & below_lane) + min(my_eq, need);
+            if (at < (uint32_t)a.budget) kept[at] = c0 + i;
+        }
+        gt += __popc(bg);
+        eq += __popc(be);
+    }
+    cluster.sync();                                         // the counts are read by the others
 }
 
 struct GatherArgs {
@@ -456,7 +534,8 @@ extern "C" int minf_kv8_evict(
     a.recent = recent;
     a.sink = sink;
     a.kept = kept;
-    kv8_select_kernel<<<dim3(src->heads, src->batch), kSelectThreads, 0, s>>>(a);
+    MINF_CUDA_OK(cudaFuncSetAttribute(kv8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSmem));
+    kv8_select_kernel<<<dim3(src->heads * kSelectCluster, src->batch), kSelectThreads, kSelectSmem, s>>>(a);
     MINF_LAUNCH_OK("kv8_select_kernel");
     GatherArgs g{};
     g.src = *src;

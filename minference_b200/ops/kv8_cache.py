@@ -12,7 +12,9 @@ The reference has no counterpart (its quantised cache is a 2-bit one of another 
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
+import functools
 
 import torch
 
@@ -21,6 +23,20 @@ from .. import _cabi
 BLOCK = 64          # tokens that share a scale
 HEAD_DIM = 128
 _FORMATS = {torch.float8_e4m3fn: _cabi.KV8_E4M3, torch.int8: _cabi.KV8_INT8}
+
+
+_I64x3 = ctypes.c_int64 * 3
+
+
+@functools.lru_cache(maxsize=1024)
+def _scratch_bytes(batch: int, hq: int, heads: int, n_q: int, max_length: int, with_weights: bool) -> int:
+    return _cabi.lib().minf_kv8_attention_scratch_bytes(batch, hq, heads, n_q, max_length, with_weights)
+
+
+def _on_device(cache):
+    """Context in which a launch goes to the cache's device: nothing to switch in the usual case (a decoding step is a few
+    microseconds of work, and the context manager costs one of them)."""
+    return contextlib.nullcontext() if torch.cuda.current_device() == cache.device.index else torch.cuda.device(cache.device)
 
 
 def _fail(msg: str):
@@ -35,6 +51,7 @@ class KV8Cache:
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
         _cabi.require_cuda(k, v, k_scale, v_scale, k_tail, v_tail)
+        _cabi.lib()
         if k.dtype not in _FORMATS or v.dtype != k.dtype:
             _fail(f"cache codes must both be float8_e4m3fn or int8 (got {k.dtype}, {v.dtype})")
         if k.dim() != 4 or k.shape[3] != HEAD_DIM or k.shape[2] % BLOCK or k.shape[2] == 0:
@@ -82,7 +99,7 @@ class KV8Cache:
 def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
     """(device pointer or None, host value, tensor to keep alive) of an int or an int32 tensor ``[B]``."""
     if isinstance(x, torch.Tensor):
-        if x.dtype != torch.int32 or x.shape != (cache.batch,) or x.device != cache.device or not x.is_contiguous():
+        if x.dtype != torch.int32 or x.dim() != 1 or x.numel() != cache.batch or x.device != cache.device or not x.is_contiguous():
             _fail(f"{what} must be an int or a contiguous int32 tensor [{cache.batch}] on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})")
         return x.data_ptr(), 0
     x = int(x)
@@ -94,13 +111,18 @@ def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
 def _rows(t: torch.Tensor, what: str, cache: KV8Cache):
     if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or t.device != cache.device:
         _fail(f"{what} must be bf16 [{cache.batch}, heads, tokens, {HEAD_DIM}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
-    if t.stride(3) != 1 or any(s % 8 for s in t.stride()[:3]) or t.data_ptr() % 16:
+    s0, s1, s2, s3 = t.stride()
+    if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15:
         t = t.contiguous()
     return t
 
 
-def _strides2(t: torch.Tensor):
-    return (ctypes.c_int64 * 3)(t.stride(0), t.stride(1), 0)
+def _strides(t: torch.Tensor):
+    return _I64x3(*t.stride()[:3])
+
+
+def _stream(cache: KV8Cache) -> int:
+    return torch.cuda.current_stream(cache.device).cuda_stream
 
 
 def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
@@ -117,9 +139,9 @@ def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, co
             _fail("counts must be an int32 tensor")
         dev_counts, _ = _per_sequence(cache, counts, "counts", 0, n)
     dev_start, start = _per_sequence(cache, start, "start", 0, cache.capacity - (n if counts is None else 0))
-    with torch.cuda.device(cache.device):
-        _cabi.check(_cabi.lib().minf_kv8_store(cache._ref, key.data_ptr(), value.data_ptr(), _cabi.strides3(key), _cabi.strides3(value),
-                                               n, dev_start, start, dev_counts, _cabi.stream_ptr(cache.device)))
+    with _on_device(cache):
+        _cabi.check(_cabi.lib().minf_kv8_store(cache._ref, key.data_ptr(), value.data_ptr(), _strides(key), _strides(value),
+                                               n, dev_start, start, dev_counts, _stream(cache)))
 
 
 def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
@@ -134,9 +156,9 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
     k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
     v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    with torch.cuda.device(cache.device):
+    with _on_device(cache):
         _cabi.check(_cabi.lib().minf_kv8_load(cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr(),
-                                              _cabi.stream_ptr(cache.device)))
+                                              _stream(cache)))
     return k, v
 
 
@@ -180,17 +202,17 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
         if weights is None:
             _fail("add_to without weights")
         _weights_arg(add_to, "add_to", cache, longest)
-    L = _cabi.lib()
     out = torch.empty((b, hq, s, d), dtype=query.dtype, device=cache.device)
     lse = torch.empty((b, hq, s), dtype=torch.float32, device=cache.device) if return_lse else None
-    nbytes = L.minf_kv8_attention_scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
+    nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
     scratch = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-    with torch.cuda.device(cache.device):
-        _cabi.check(L.minf_kv8_attention(
-            cache._ref, query.data_ptr(), _cabi.strides3(query), out.data_ptr(), _cabi.strides3(out), hq, s, dev_n, n, longest,
-            float(d ** -0.5 if sm_scale is None else sm_scale), _cabi.ptr(lse),
-            _cabi.ptr(weights), None if weights is None else _strides2(weights),
-            _cabi.ptr(add_to), None if add_to is None else _strides2(add_to), _cabi.ptr(scratch), _cabi.stream_ptr(cache.device)))
+    with _on_device(cache):
+        _cabi.check(_cabi.lib().minf_kv8_attention(
+            cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _strides(out), hq, s, dev_n, n, longest,
+            d ** -0.5 if sm_scale is None else float(sm_scale), lse.data_ptr() if return_lse else None,
+            weights.data_ptr() if weights is not None else None, _strides(weights) if weights is not None else None,
+            add_to.data_ptr() if add_to is not None else None, _strides(add_to) if add_to is not None else None,
+            scratch.data_ptr() if nbytes else None, _stream(cache)))
     return (out, lse) if return_lse else out
 
 
@@ -218,8 +240,8 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=dev)
     weights_out = torch.empty((cache.batch, cache.kv_heads, out.capacity), dtype=torch.float32, device=dev)
     lengths_out = torch.empty((cache.batch,), dtype=torch.int32, device=dev)
-    with torch.cuda.device(dev):
+    with _on_device(cache):
         _cabi.check(_cabi.lib().minf_kv8_evict(
-            cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides2(weights), budget, recent, sink,
-            kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr(), _cabi.stream_ptr(dev)))
+            cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides(weights), budget, recent, sink,
+            kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr(), _stream(cache)))
     return out, lengths_out, weights_out, kept
