@@ -13,7 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
 LIB = os.path.join(HERE, "libminfer_b200.so")
 SOURCES = ["cabi.cu", "vs_index.cu", "sparse_attn_fwd.cu", "vs_estimate.cu", "block_sparse_index.cu", "block_mask_plan.cu",
-           "kv8_cache.cu", "kv8_attention.cu"]
+           "kv8_cache.cu", "kv8_attention.cu", "kv8_attention_wide.cu"]
 NVCC_FLAGS = [
     "-gencode", "arch=compute_100a,code=sm_100a", "-lineinfo", "-O3", "-std=c++17",
     "--expt-relaxed-constexpr", "-Xcompiler", "-fPIC", "-Xptxas", "-v",

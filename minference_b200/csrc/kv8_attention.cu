@@ -15,7 +15,7 @@
 //
 // The tokens of a sequence are split over CTAs and, inside one, over warps by blocks of 64; the parts are joined by
 // their log-sum-exps in a second kernel.
-#include "kv8.cuh"
+#include "kv8_attention.cuh"
 
 #include <math_constants.h>
 
@@ -27,34 +27,9 @@ namespace minf {
 
 constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kSMs = 148;
 constexpr int kSlotBytes = kKv8Block * kKv8Dim;     // keys or values of a block
 constexpr int kRingSlots = 3;
 constexpr int kRingBytes = kAttnWarps * kRingSlots * kSlotBytes;
-
-struct Kv8AttnArgs {
-    minf_kv8_cache c;
-    const __nv_bfloat16* q;
-    long long qs[3];
-    __nv_bfloat16* o;
-    long long os[3];
-    int group, n_q, rows;           // rows = group * n_q per cache head; row r is query head r / n_q, token r % n_q
-    const int32_t* lengths;
-    int length_all, max_length;
-    float scale_log2;
-    int splits;
-    float* part_o;                  // [batch*heads*rows][splits][128], normalised
-    float* part_lse;                // [batch*heads*rows][splits]
-    float* lse;                     // caller's, [batch, hq, n_q], or NULL
-    float* row_lse;                 // [batch*heads*rows] (for the weights), or NULL
-    float* logits;                  // [batch*heads][tokens][pitch], or NULL
-    int pitch;
-    long long tokens;               // rows of `logits` per head
-    float* weights;
-    long long ws[2];
-    const float* add_to;
-    long long as[2];
-};
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -590,13 +565,27 @@ struct AttnShape {
 static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
     AttnShape s{};
     const long long rows = (long long)(hq / heads) * n_q;
-    s.nt = (int)std::min<long long>(4, (rows + 7) / 8);
-    s.tiles = (int)((rows + 8 * s.nt - 1) / (8 * s.nt));
+    s.nt = rows <= 8 ? 1 : 0;
+    s.tiles = s.nt ? 1 : (int)((rows + kWideRows - 1) / kWideRows);
     const long long ctas = (long long)batch * heads * s.tiles;
     const long long blocks = max_length / kKv8Block;
-    long long splits = (2 * kSMs + ctas - 1) / ctas;
-    splits = std::min(splits, (blocks + kAttnWarps - 1) / kAttnWarps);
-    s.splits = (int)std::max(splits, 1ll);
+    if (s.nt) {
+        long long splits = (2 * kSMs + ctas - 1) / ctas;
+        splits = std::min(splits, (blocks + kAttnWarps - 1) / kAttnWarps);
+        s.splits = (int)std::max(splits, 1ll);
+    } else {
+        // one CTA an SM: the number of splits (of two tiles of tokens at least) that wastes least of its last wave; each
+        // costs about as much again as two tiles (its start, its end and the joining)
+        const long long tiles = (max_length + 127) / 128;
+        double best = 1e30;
+        for (long long k = 1; k <= std::max(1ll, tiles / 2) && k <= kSMs; ++k) {
+            const double cost = (double)((ctas * k + kSMs - 1) / kSMs) * ((double)((tiles + k - 1) / k) + 2.0);
+            if (cost < best - 1e-9) {
+                best = cost;
+                s.splits = (int)k;
+            }
+        }
+    }
     s.pitch = (int)((rows + 1) / 2 * 2);
     s.tokens = max_length;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
@@ -627,14 +616,9 @@ static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cu
     return cudaGetLastError();
 }
 
-template <int FMT>
 static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
-    switch (s.nt) {
-        case 1: return launch_attention<FMT, 1>(a, s, stream);
-        case 2: return launch_attention<FMT, 2>(a, s, stream);
-        case 3: return launch_attention<FMT, 3>(a, s, stream);
-        default: return launch_attention<FMT, 4>(a, s, stream);
-    }
+    if (!s.nt) return launch_attention_wide(a, s.tiles, stream);
+    return a.c.format == MINF_KV8_E4M3 ? launch_attention<MINF_KV8_E4M3, 1>(a, s, stream) : launch_attention<MINF_KV8_INT8, 1>(a, s, stream);
 }
 
 }  // namespace minf
@@ -699,7 +683,7 @@ extern "C" int minf_kv8_attention(
         }
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = cache->format == MINF_KV8_E4M3 ? launch_attention<MINF_KV8_E4M3>(a, s, st) : launch_attention<MINF_KV8_INT8>(a, s, st);
+    const cudaError_t e = launch_attention(a, s, st);
     if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_attention_kernel failed: %s", cudaGetErrorString(e));
     if (s.splits > 1) {
         kv8_combine_kernel<<<(unsigned)((size_t)cache->batch * cache->heads * a.rows), 128, 0, st>>>(a);
