@@ -29,6 +29,7 @@ constexpr int kAttnWarps = 4;
 constexpr int kAttnThreads = kAttnWarps * 32;
 constexpr int kSlotBytes = kKv8Block * kKv8Dim;     // keys or values of a block
 constexpr int kRingSlots = 3;
+constexpr int kNarrowRows = 32;                     // rows per cache head this kernel takes
 constexpr int kRingBytes = kAttnWarps * kRingSlots * kSlotBytes;
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
@@ -51,11 +52,14 @@ __device__ __forceinline__ uint32_t pack_half2(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// any half of the register infinite or NaN
+// Halves (f16, or bf16) that are infinite or NaN become zero; true if there were any.
 template <bool BF16>
-__device__ __forceinline__ bool not_finite(uint32_t x) {
+__device__ __forceinline__ bool drop_not_finite(uint32_t& x) {
     constexpr uint32_t m = BF16 ? 0x7f80u : 0x7c00u;
-    return (x & m) == m || (x & (m << 16)) == (m << 16);
+    const bool lo = (x & m) == m, hi = (x & (m << 16)) == (m << 16);
+    if (lo) x &= 0xffff0000u;
+    if (hi) x &= 0x0000ffffu;
+    return lo || hi;
 }
 
 // What a warp carries along its tokens, for NT groups of eight rows: a lane holds columns 2c and 2c+1 of each group
@@ -67,14 +71,14 @@ struct Rows {
     float m[NT][2];                 // running maximum of l + log2 s_V
     float l[NT][2];                 // this lane's part of the denominator, relative to m
     float mul[NT][2];               // logit of a unit of the accumulator, before the block's scale
-    int lim[NT][2];                 // tokens below this are seen
 };
 
 // Logits of 16 * SUB tokens -> P, with the running statistics moved on.  s[j][nt][e]: token t0 + 16 j + tg (+ 8 for e = 2, 3),
-// column 2c (+ 1 for odd e).  On return s holds P.
-template <int NT, int SUB>
+// column 2c (+ 1 for odd e).  On return s holds P.  Where `masked`, a row sees the tokens below all_see + its own token's
+// number only (columns behind the last row: anything, they are dropped).
+template <int NT, int SUB, bool LOGITS>
 __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, float (&s)[SUB][NT][4], float k_scale, float v_scale,
-                                             int t0, bool masked, int end, size_t bh, int row0, int tg, int c) {
+                                             int t0, bool masked, int all_see, int end, size_t bh, int tg, int c) {
     const float lv = log2f(v_scale), inv_v = 1.f / v_scale;
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
@@ -87,21 +91,36 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             x[1] *= f1;
             x[2] *= f0;
             x[3] *= f1;
-            if (masked) {
+        }
+        if (masked) {
+            const int r = 8 * nt + 2 * c;
+            const int lim0 = all_see + r % a.n_q, lim1 = all_see + (r + 1) % a.n_q;
+#pragma unroll
+            for (int j = 0; j < SUB; ++j) {
+                float* x = s[j][nt];
                 const int t = t0 + 16 * j + tg;
-                if (t >= R.lim[nt][0]) x[0] = -CUDART_INF_F;
-                if (t >= R.lim[nt][1]) x[1] = -CUDART_INF_F;
-                if (t + 8 >= R.lim[nt][0]) x[2] = -CUDART_INF_F;
-                if (t + 8 >= R.lim[nt][1]) x[3] = -CUDART_INF_F;
+                if (t >= lim0) x[0] = -CUDART_INF_F;
+                if (t >= lim1) x[1] = -CUDART_INF_F;
+                if (t + 8 >= lim0) x[2] = -CUDART_INF_F;
+                if (t + 8 >= lim1) x[3] = -CUDART_INF_F;
             }
-            if (a.logits) {
-                const int col = row0 + 8 * nt + 2 * c, t = t0 + 16 * j + tg;
-                if (col < a.pitch) {
-                    float* p = a.logits + ((long long)bh * a.tokens + t) * a.pitch + col;
-                    if (t < end) *reinterpret_cast<float2*>(p) = make_float2(x[0], x[1]);
-                    if (t + 8 < end) *reinterpret_cast<float2*>(p + 8ll * a.pitch) = make_float2(x[2], x[3]);
+        }
+        if (LOGITS) {
+            const int col = 8 * nt + 2 * c;
+            if (col < a.pitch) {
+                float* p = a.logits + ((long long)bh * a.tokens + t0 + tg) * a.pitch + col;
+#pragma unroll
+                for (int j = 0; j < SUB; ++j) {
+                    const float* x = s[j][nt];
+                    const int t = t0 + 16 * j + tg;
+                    if (t < end) *reinterpret_cast<float2*>(p + 16 * j * a.pitch) = make_float2(x[0], x[1]);
+                    if (t + 8 < end) *reinterpret_cast<float2*>(p + (16 * j + 8) * a.pitch) = make_float2(x[2], x[3]);
                 }
             }
+        }
+#pragma unroll
+        for (int j = 0; j < SUB; ++j) {
+            const float* x = s[j][nt];
             mx0 = fmaxf(mx0, fmaxf(x[0], x[2]));
             mx1 = fmaxf(mx1, fmaxf(x[1], x[3]));
         }
@@ -110,10 +129,14 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
             mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
         }
-        const float n0 = fmaxf(R.m[nt][0], mx0 + lv), n1 = fmaxf(R.m[nt][1], mx1 + lv);
-        const float r0 = n0 == -CUDART_INF_F ? 0.f : n0, r1 = n1 == -CUDART_INF_F ? 0.f : n1;   // nothing seen yet: keep -inf - 0
-        if (__any_sync(0xffffffffu, n0 != R.m[nt][0] || n1 != R.m[nt][1])) {
-            const float a0 = fast_exp2(R.m[nt][0] - r0), a1 = fast_exp2(R.m[nt][1] - r1);
+        // the reference is raised on a jump of more than 2^8: P stays far below f16's largest, and outputs are rarely rescaled
+        mx0 += lv;
+        mx1 += lv;
+        const bool up0 = mx0 > R.m[nt][0] + 8.f, up1 = mx1 > R.m[nt][1] + 8.f;
+        if (__any_sync(0xffffffffu, up0 || up1)) {
+            const float a0 = up0 ? fast_exp2(R.m[nt][0] - mx0) : 1.f, a1 = up1 ? fast_exp2(R.m[nt][1] - mx1) : 1.f;
+            if (up0) R.m[nt][0] = mx0;
+            if (up1) R.m[nt][1] = mx1;
             R.l[nt][0] *= a0;
             R.l[nt][1] *= a1;
 #pragma unroll
@@ -123,10 +146,9 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
                 R.o[nt][i][2] *= a0;
                 R.o[nt][i][3] *= a1;
             }
-            R.m[nt][0] = n0;
-            R.m[nt][1] = n1;
         }
-        const float d0 = lv - r0, d1 = lv - r1;
+        // nothing seen yet: -inf - 0
+        const float d0 = lv - (R.m[nt][0] == -CUDART_INF_F ? 0.f : R.m[nt][0]), d1 = lv - (R.m[nt][1] == -CUDART_INF_F ? 0.f : R.m[nt][1]);
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {
@@ -143,120 +165,24 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
     }
 }
 
-// O^T += V^T P^T for 16 tokens of one column group.  v[i][0..3]: the A fragment of dims 16g+2i, 16g+2i+1 (rows g and
-// g + 8 of the product), for tokens ta, tb in the halves of a register and ta + 8, tb + 8.  Where a value of a token that some column does not see may be infinite or NaN, the product
-// is taken column by column with the unseen tokens' values left out: zero times them would not be zero.
-template <bool BF16>
-__device__ __forceinline__ void pv_mma(float (&d)[4], const uint32_t (&v)[4], uint32_t b0, uint32_t b1) {
-    if constexpr (BF16) mma_bf16(d, v[0], v[1], v[2], v[3], b0, b1);
-    else mma_f16(d, v[0], v[1], v[2], v[3], b0, b1);
-}
-template <bool BF16, int NT>
-__device__ __forceinline__ void pv_step(Rows<NT>& R, const uint32_t (&v)[8][4], int nt, uint32_t b0, uint32_t b1, bool masked, int ta, int tb, int g, int c) {
-    if (masked) {
-        bool bad = false;
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) bad |= not_finite<BF16>(v[i][e]);
-        if (__any_sync(0xffffffffu, bad)) {
-            for (int col = 0; col < 8; ++col) {
-                const int l0 = __shfl_sync(0xffffffffu, R.lim[nt][0], col >> 1), l1 = __shfl_sync(0xffffffffu, R.lim[nt][1], col >> 1);
-                const int lim = (col & 1) ? l1 : l0;
-                const uint32_t k0 = (ta < lim ? 0xffffu : 0u) | (tb < lim ? 0xffff0000u : 0u);
-                const uint32_t k1 = (ta + 8 < lim ? 0xffffu : 0u) | (tb + 8 < lim ? 0xffff0000u : 0u);
-                const uint32_t c0 = g == col ? b0 : 0u, c1 = g == col ? b1 : 0u;
-#pragma unroll
-                for (int i = 0; i < 8; ++i) {
-                    float d[4] = {0.f, 0.f, 0.f, 0.f};
-                    const uint32_t w[4] = {v[i][0] & k0, v[i][1] & k0, v[i][2] & k1, v[i][3] & k1};
-                    pv_mma<BF16>(d, w, c0, c1);
-                    if (2 * c == col) {             // the other columns' products are 0 times these values: left out
-                        R.o[nt][i][0] += d[0];
-                        R.o[nt][i][2] += d[2];
-                    }
-                    if (2 * c + 1 == col) {
-                        R.o[nt][i][1] += d[1];
-                        R.o[nt][i][3] += d[3];
-                    }
-                }
-            }
-            return;
-        }
-    }
-#pragma unroll
-    for (int i = 0; i < 8; ++i) pv_mma<BF16>(R.o[nt][i], v[i], b0, b1);
-}
-
-template <int FMT, int NT>
+template <int FMT, int NT, bool LOGITS>
 __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __grid_constant__ Kv8AttnArgs a) {
     constexpr int SUB = 4 / NT;                     // sub-tiles of 16 tokens per softmax step: up to 16 logits a lane
     constexpr int PARTS = 4 / SUB;                  // softmax steps of a block
-    const int split = blockIdx.x, b = blockIdx.z;
-    const int tiles = (a.rows + 8 * NT - 1) / (8 * NT);
-    const int h = blockIdx.y / tiles, row0 = (blockIdx.y % tiles) * 8 * NT;
+    constexpr bool kQShared = NT > 2;               // Q's fragments in shared memory (from there each is read once per sub-tile)
+    extern __shared__ __align__(128) unsigned char ring_all[];
+    const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
     const size_t bh = (size_t)b * a.c.heads + h;
     const int full = n / kKv8Block;                 // complete blocks
-    const int blk_lo = (int)((long long)full * split / a.splits), blk_hi = (int)((long long)full * (split + 1) / a.splits);
+    // the last split takes the tail too, which keeps all four warps busy: it counts as four blocks
+    const int units = full + (n % kKv8Block ? kAttnWarps : 0);
+    const int blk_lo = min(full, (int)((long long)units * split / a.splits)), blk_hi = min(full, (int)((long long)units * (split + 1) / a.splits));
     const int all_see = n - a.n_q + 1;              // tokens below this are seen by every row
-
-    // Q^T fragments: column g of group nt, dims of step s: 64 (s / 4) + 16 c + 4 (s % 4) + {0, 1 | 2, 3}
-    Rows<NT> R;
-    uint32_t qf[NT][8][2];
-    float q_unit[NT];                               // power of two the row was divided by
-    auto q_row = [&](int nt) {
-        const int r = row0 + 8 * nt + g;
-        return r < a.rows ? a.q + b * a.qs[0] + (long long)(h * a.group + r / a.n_q) * a.qs[1] + (long long)(r % a.n_q) * a.qs[2] : nullptr;
-    };
-#pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
-        const __nv_bfloat16* q = q_row(nt);
-        float top = 0.f;
-        float x[8][4];
-#pragma unroll
-        for (int s = 0; s < 8; ++s)
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                x[s][e] = q ? __bfloat162float(q[64 * (s >> 2) + 16 * c + 4 * (s & 3) + e]) : 0.f;
-                const float m = fabsf(x[s][e]);
-                if (m < CUDART_INF_F) top = fmaxf(top, m);
-            }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = 0;
-        if (top > 0.f) frexpf(top, &e);             // top < 2^e: scaled to below 2^8, so that the smallest products count too
-        e = max(min(e - 8, 100), -100);
-        const float inv = exp2f((float)-e);
-        q_unit[nt] = exp2f((float)e);
-#pragma unroll
-        for (int s = 0; s < 8; ++s) {
-            qf[nt][s][0] = pack_half2(x[s][0] * inv, x[s][1] * inv);
-            qf[nt][s][1] = pack_half2(x[s][2] * inv, x[s][3] * inv);
-        }
-#pragma unroll
-        for (int cc = 0; cc < 2; ++cc) {
-            const int r = row0 + 8 * nt + 2 * c + cc;
-            R.mul[nt][cc] = a.scale_log2 * __shfl_sync(0xffffffffu, q_unit[nt], 4 * (2 * c + cc));
-            R.lim[nt][cc] = r < a.rows ? all_see + r % a.n_q : 0x7fffffff;     // columns beyond the rows are dropped
-            R.m[nt][cc] = -CUDART_INF_F;
-            R.l[nt][cc] = 0.f;
-        }
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-            for (int k = 0; k < 4; ++k) R.o[nt][i][k] = 0.f;
-    }
-
-    const uint8_t* kc = static_cast<const uint8_t*>(a.c.k) + bh * a.c.capacity * kKv8Dim;
-    const uint8_t* vc = static_cast<const uint8_t*>(a.c.v) + bh * a.c.capacity * kKv8Dim;
-    const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
-    const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
 
     // The warp's own ring of three slots of 8 KB: keys of a block, values of it, keys of its next block, ...; two
     // copies are in flight while the third is used.  16-byte chunk ch of row r lies at ch ^ (r & 7).
-    extern __shared__ __align__(128) unsigned char ring_all[];
     unsigned char* const ring = ring_all + warp * (kRingSlots * kSlotBytes);
     const uint32_t ring_u = smem_u32(ring);
     const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4)) << 4);
@@ -266,15 +192,11 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
 #pragma unroll
         for (int i = 0; i < 16; ++i) cp_async_16(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i);
     };
-    // Row i of the eight of a fragment is token perm(i): with it, and the chunks' places above, the eight lanes of a
-    // quarter of a shared-memory access touch all 32 banks, for the keys' rows and for the values' alike.
-    const int pg = (g & 1) ? (g - 1) ^ 5 : g;       // perm(g)
-    const int pa = 2 * c, pb = (2 * c) ^ 5;         // perm(2c), perm(2c + 1)
-
-    const uint8_t* next_k = kc + (size_t)(blk_lo + warp) * kSlotBytes;
-    const uint8_t* next_v = vc + (size_t)(blk_lo + warp) * kSlotBytes;
-    constexpr size_t kHop = (size_t)kAttnWarps * kSlotBytes;
-    int slot = 0;
+    const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
+    const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
+    const size_t first = (bh * (a.c.capacity / kKv8Block) + blk_lo + warp) * kSlotBytes;
+    const uint8_t* next_k = static_cast<const uint8_t*>(a.c.k) + first;
+    const uint8_t* next_v = static_cast<const uint8_t*>(a.c.v) + first;
     float k_scale = 1.f, v_scale = 1.f;
     if (blk_lo + warp < blk_hi) {
         fetch(0, next_k);
@@ -286,6 +208,75 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
         cp_async_commit();
     }
     cp_async_commit();
+
+    // Q^T fragments: column g of group nt, dims of step s: 64 (s / 4) + 16 c + 4 (s % 4) + {0, 1 | 2, 3}
+    Rows<NT> R;
+    uint32_t qf[kQShared ? 1 : NT][8][2];
+    uint2* const q_sm = reinterpret_cast<uint2*>(ring_all + kRingBytes);        // [nt][step][lane]
+    float q_unit[NT];                               // power of two the row was divided by
+    // eight dims of row 8 nt + g from dim d on (zeros behind the last row)
+    auto q_load = [&](int nt, int d, float (&v)[8]) {
+        const int r = 8 * nt + g;
+        uint4 x = make_uint4(0u, 0u, 0u, 0u);
+        if (r < a.rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.qs[0] + (long long)(h * a.group + r / a.n_q) * a.qs[1] + (long long)(r % a.n_q) * a.qs[2] + d);
+        bf16x8_to_values(x, v);
+    };
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        float top = 0.f;
+        float x[4][8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            q_load(nt, 64 * (i >> 1) + 16 * c + 8 * (i & 1), x[i]);
+#pragma unroll
+            for (int e = 0; e < 8; ++e) {
+                const float m = fabsf(x[i][e]);
+                if (m < CUDART_INF_F) top = fmaxf(top, m);
+            }
+        }
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+        int e = 0;
+        if (top > 0.f) frexpf(top, &e);             // top < 2^e: scaled to below 2^8, so that the smallest products count too
+        e = max(min(e - 8, 100), -100);
+        const float inv = exp2f((float)-e);
+        q_unit[nt] = exp2f((float)e);
+#pragma unroll
+        for (int st = 0; st < 8; ++st) {
+            const float* v = &x[st >> 1][4 * (st & 1)];
+            const uint32_t b0 = pack_half2(v[0] * inv, v[1] * inv), b1 = pack_half2(v[2] * inv, v[3] * inv);
+            if constexpr (kQShared) {
+                if (warp == 0) q_sm[(nt * 8 + st) * 32 + lane] = make_uint2(b0, b1);
+            } else {
+                qf[nt][st][0] = b0;
+                qf[nt][st][1] = b1;
+            }
+        }
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+            R.mul[nt][cc] = a.scale_log2 * __shfl_sync(0xffffffffu, q_unit[nt], 4 * (2 * c + cc));
+            R.m[nt][cc] = -CUDART_INF_F;
+            R.l[nt][cc] = 0.f;
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) R.o[nt][i][k] = 0.f;
+    }
+    if (kQShared) __syncthreads();
+    auto q_frag = [&](int nt, int st) {
+        if constexpr (kQShared) return q_sm[(nt * 8 + st) * 32 + lane];
+        else return make_uint2(qf[nt][st][0], qf[nt][st][1]);
+    };
+
+    // Row i of the eight of a fragment is token perm(i): with it, and the chunks' places in the ring, the eight lanes of a
+    // quarter of a shared-memory access touch all 32 banks, for the keys' rows and for the values' alike.
+    const int pg = (g & 1) ? (g - 1) ^ 5 : g;       // perm(g)
+    const int pa = 2 * c, pb = (2 * c) ^ 5;         // perm(2c), perm(2c + 1)
+    bool bad = false;                               // values left out of the products, see below
+
+    constexpr size_t kHop = (size_t)kAttnWarps * kSlotBytes;
+    int slot = 0;
     for (int blk = blk_lo + warp; blk < blk_hi; blk += kAttnWarps) {
         const bool more = blk + kAttnWarps < blk_hi;
         const bool masked = (blk + 1) * kKv8Block > all_see;
@@ -327,10 +318,13 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
                     codes_to_half<FMT>(r0[st], a0, a2);
                     codes_to_half<FMT>(r1[st], a1, a3);
 #pragma unroll
-                    for (int nt = 0; nt < NT; ++nt) mma_f16(s[j][nt], a0, a1, a2, a3, qf[nt][st][0], qf[nt][st][1]);
+                    for (int nt = 0; nt < NT; ++nt) {
+                        const uint2 q = q_frag(nt, st);
+                        mma_f16(s[j][nt], a0, a1, a2, a3, q.x, q.y);
+                    }
                 }
             }
-            softmax_step<NT, SUB>(a, R, s, ksc, vsc, t0, masked, n, bh, row0, pg, c);
+            softmax_step<NT, SUB, LOGITS>(a, R, s, ksc, vsc, t0, masked, all_see, n, bh, pg, c);
             if (!v_here) {
                 cp_async_wait<1>();
                 __syncwarp();
@@ -338,24 +332,34 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
             }
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
-                // A fragment of V^T: two tokens in the halves of a register
-                uint32_t v[8][4];
-#pragma unroll
-                for (int hf = 0; hf < 2; ++hf) {
-                    const unsigned char* p = vb + (part * SUB * 16 + 16 * j + 8 * hf) * kKv8Dim;
-                    const uint4 x = *reinterpret_cast<const uint4*>(p + pa * kKv8Dim + ((g ^ pa) << 4));
-                    const uint4 y = *reinterpret_cast<const uint4*>(p + pb * kKv8Dim + ((g ^ pb) << 4));
-                    const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                    for (int w = 0; w < 4; ++w) {
-                        codes_to_half<FMT>(__byte_perm(xs[w], ys[w], 0x5140), v[2 * w][2 * hf], v[2 * w][2 * hf + 1]);
-                        codes_to_half<FMT>(__byte_perm(xs[w], ys[w], 0x7362), v[2 * w + 1][2 * hf], v[2 * w + 1][2 * hf + 1]);
-                    }
-                }
+                uint32_t b0[NT], b1[NT];
 #pragma unroll
                 for (int nt = 0; nt < NT; ++nt) {
-                    const uint32_t b0 = transpose8x8(pack_half2(s[j][nt][0], s[j][nt][1])), b1 = transpose8x8(pack_half2(s[j][nt][2], s[j][nt][3]));
-                    pv_step<false, NT>(R, v, nt, b0, b1, masked, t0 + 16 * j + pa, t0 + 16 * j + pb, g, c);
+                    b0[nt] = transpose8x8(pack_half2(s[j][nt][0], s[j][nt][1]));
+                    b1[nt] = transpose8x8(pack_half2(s[j][nt][2], s[j][nt][3]));
+                }
+                // A fragments of V^T: two tokens in the halves of a register, rows g and g + 8 are dims 16g+2i, 16g+2i+1
+                const unsigned char* p = vb + (part * SUB * 16 + 16 * j) * kKv8Dim;
+                const uint4 x0 = *reinterpret_cast<const uint4*>(p + pa * kKv8Dim + ((g ^ pa) << 4));
+                const uint4 y0 = *reinterpret_cast<const uint4*>(p + pb * kKv8Dim + ((g ^ pb) << 4));
+                const uint4 x1 = *reinterpret_cast<const uint4*>(p + (pa + 8) * kKv8Dim + ((g ^ pa) << 4));
+                const uint4 y1 = *reinterpret_cast<const uint4*>(p + (pb + 8) * kKv8Dim + ((g ^ pb) << 4));
+                const uint32_t xs0[4] = {x0.x, x0.y, x0.z, x0.w}, ys0[4] = {y0.x, y0.y, y0.z, y0.w};
+                const uint32_t xs1[4] = {x1.x, x1.y, x1.z, x1.w}, ys1[4] = {y1.x, y1.y, y1.z, y1.w};
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const uint32_t sel = (i & 1) ? 0x7362 : 0x5140;
+                    uint32_t v0, v1, v2, v3;
+                    codes_to_half<FMT>(__byte_perm(xs0[i >> 1], ys0[i >> 1], sel), v0, v1);
+                    codes_to_half<FMT>(__byte_perm(xs1[i >> 1], ys1[i >> 1], sel), v2, v3);
+                    if (FMT == MINF_KV8_E4M3 && masked) {
+                        bad |= drop_not_finite<false>(v0);
+                        bad |= drop_not_finite<false>(v1);
+                        bad |= drop_not_finite<false>(v2);
+                        bad |= drop_not_finite<false>(v3);
+                    }
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt) mma_f16(R.o[nt][i], v0, v1, v2, v3, b0[nt], b1[nt]);
                 }
             }
         }
@@ -373,55 +377,68 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
         const __nv_bfloat16* vt = static_cast<const __nv_bfloat16*>(a.c.v_tail) + (bh * kKv8Block + 16 * warp) * kKv8Dim;
         float s[1][NT][4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
+        for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[0][nt][e] = 0.f;
-            const __nv_bfloat16* q = q_row(nt);
-            const float inv = 1.f / q_unit[nt];
 #pragma unroll
-            for (int st = 0; st < 8; ++st) {
-                const int d = 64 * (st >> 2) + 16 * c + 4 * (st & 3);
-                uint32_t b0 = 0, b1 = 0;
-                if (q) {
-                    b0 = pack_bf16x2(__bfloat162float(q[d]) * inv, __bfloat162float(q[d + 1]) * inv);
-                    b1 = pack_bf16x2(__bfloat162float(q[d + 2]) * inv, __bfloat162float(q[d + 3]) * inv);
-                }
-                const uint2 x = *reinterpret_cast<const uint2*>(kt + g * kKv8Dim + d), y = *reinterpret_cast<const uint2*>(kt + (g + 8) * kKv8Dim + d);
-                mma_bf16(s[0][nt], x.x, y.x, x.y, y.y, b0, b1);
+        for (int i = 0; i < 4; ++i) {               // 16 dims of a lane quad: two steps
+            const int d = 64 * (i >> 1) + 16 * c + 8 * (i & 1);
+            const uint4 x = *reinterpret_cast<const uint4*>(kt + g * kKv8Dim + d), y = *reinterpret_cast<const uint4*>(kt + (g + 8) * kKv8Dim + d);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                float v[8];
+                q_load(nt, d, v);
+                const float inv = 1.f / q_unit[nt];
+                mma_bf16(s[0][nt], x.x, y.x, x.y, y.y, pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
+                mma_bf16(s[0][nt], x.z, y.z, x.w, y.w, pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
             }
         }
-        softmax_step<NT, 1>(a, R, s, 1.f, 1.f, t0, true, n, bh, row0, g, c);
-        uint32_t v[8][4];
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-            const int r = 2 * c + 8 * hf;
-            const __nv_bfloat16* p = vt + r * kKv8Dim + 16 * g;
-#pragma unroll
-            for (int w = 0; w < 2; ++w) {           // eight dims of the two tokens
-                uint4 x = *reinterpret_cast<const uint4*>(p + 8 * w), y = *reinterpret_cast<const uint4*>(p + kKv8Dim + 8 * w);
-                if (t0 + r >= n) x = make_uint4(0u, 0u, 0u, 0u);        // rows behind the last token hold anything
-                if (t0 + r + 1 >= n) y = make_uint4(0u, 0u, 0u, 0u);
-                const uint32_t xs[4] = {x.x, x.y, x.z, x.w}, ys[4] = {y.x, y.y, y.z, y.w};
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    v[4 * w + k][2 * hf] = __byte_perm(xs[k], ys[k], 0x5410);
-                    v[4 * w + k][2 * hf + 1] = __byte_perm(xs[k], ys[k], 0x7632);
-                }
-            }
-        }
+        // tokens behind the last one must not count: no row sees them (all_see + n_q - 1 = n)
+        softmax_step<NT, 1, LOGITS>(a, R, s, 1.f, 1.f, t0, true, all_see, n, bh, g, c);
+        uint32_t h0[NT], h1[NT], e0[NT], e1[NT];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt) {
-            float* x = s[0][nt];
-            const uint32_t h0 = pack_bf16x2(x[0], x[1]), h1 = pack_bf16x2(x[2], x[3]);
-            const uint32_t e0 = pack_bf16x2(x[0] - __uint_as_float(h0 << 16), x[1] - __uint_as_float(h0 & 0xffff0000u));
-            const uint32_t e1 = pack_bf16x2(x[2] - __uint_as_float(h1 << 16), x[3] - __uint_as_float(h1 & 0xffff0000u));
-            pv_step<true, NT>(R, v, nt, transpose8x8(h0), transpose8x8(h1), true, t0 + 2 * c, t0 + 2 * c + 1, g, c);
-            pv_step<true, NT>(R, v, nt, transpose8x8(e0), transpose8x8(e1), true, t0 + 2 * c, t0 + 2 * c + 1, g, c);
+            const float* x = s[0][nt];
+            h0[nt] = pack_bf16x2(x[0], x[1]);
+            h1[nt] = pack_bf16x2(x[2], x[3]);
+            e0[nt] = transpose8x8(pack_bf16x2(x[0] - __uint_as_float(h0[nt] << 16), x[1] - __uint_as_float(h0[nt] & 0xffff0000u)));
+            e1[nt] = transpose8x8(pack_bf16x2(x[2] - __uint_as_float(h1[nt] << 16), x[3] - __uint_as_float(h1[nt] & 0xffff0000u)));
+            h0[nt] = transpose8x8(h0[nt]);
+            h1[nt] = transpose8x8(h1[nt]);
+        }
+#pragma unroll
+        for (int w = 0; w < 2; ++w) {               // eight dims of four tokens
+            uint32_t xs[2][4], ys[2][4];
+#pragma unroll
+            for (int hf = 0; hf < 2; ++hf) {
+                const int r = 2 * c + 8 * hf;
+                const __nv_bfloat16* p = vt + r * kKv8Dim + 16 * g + 8 * w;
+                uint4 x = *reinterpret_cast<const uint4*>(p), y = *reinterpret_cast<const uint4*>(p + kKv8Dim);
+                if (t0 + r >= n) x = make_uint4(0u, 0u, 0u, 0u);        // rows behind the last token hold anything
+                if (t0 + r + 1 >= n) y = make_uint4(0u, 0u, 0u, 0u);
+                xs[hf][0] = x.x; xs[hf][1] = x.y; xs[hf][2] = x.z; xs[hf][3] = x.w;
+                ys[hf][0] = y.x; ys[hf][1] = y.y; ys[hf][2] = y.z; ys[hf][3] = y.w;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                uint32_t v0 = __byte_perm(xs[0][k], ys[0][k], 0x5410), v1 = __byte_perm(xs[0][k], ys[0][k], 0x7632);
+                uint32_t v2 = __byte_perm(xs[1][k], ys[1][k], 0x5410), v3 = __byte_perm(xs[1][k], ys[1][k], 0x7632);
+                bad |= drop_not_finite<true>(v0);
+                bad |= drop_not_finite<true>(v1);
+                bad |= drop_not_finite<true>(v2);
+                bad |= drop_not_finite<true>(v3);
+#pragma unroll
+                for (int nt = 0; nt < NT; ++nt) {
+                    mma_bf16(R.o[nt][4 * w + k], v0, v1, v2, v3, h0[nt], h1[nt]);
+                    mma_bf16(R.o[nt][4 * w + k], v0, v1, v2, v3, e0[nt], e1[nt]);
+                }
+            }
         }
     }
 
-    // join the warps, eight rows at a time
-    __syncthreads();                                // the rings are read out
+    // Join the warps, eight rows at a time.  Where a row did not see all of a block's tokens, values that are infinite or
+    // NaN were left out of the products (zero times them would not be zero) and are added here to the rows that see them.
+    const bool any_bad = __syncthreads_or(bad);     // (and the rings are read out)
     float (*sm_o)[8][kKv8Dim] = reinterpret_cast<float (*)[8][kKv8Dim]>(ring_all);
     float (*sm_lse)[8] = reinterpret_cast<float (*)[8]>(ring_all + kAttnWarps * 8 * kKv8Dim * sizeof(float));
 #pragma unroll
@@ -440,14 +457,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
                                                                       R.o[nt][2 * i + 1][cc] * inv, R.o[nt][2 * i + 1][2 + cc] * inv);
         }
         __syncthreads();
+#pragma unroll 1
         for (int i = threadIdx.x; i < 8 * 32; i += kAttnThreads) {
-            const int rr = i >> 5, d = (i & 31) * 4, r = row0 + 8 * nt + rr;
+            const int rr = i >> 5, d = (i & 31) * 4, r = 8 * nt + rr;
             if (r >= a.rows) continue;
             float top = sm_lse[0][rr];
 #pragma unroll
             for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_lse[w][rr]);
             float sum = 0.f;
-            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            float acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
             for (int w = 0; w < kAttnWarps; ++w) {
                 const float e = sm_lse[w][rr];
@@ -455,25 +473,36 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
                 const float f = exp2f(e - top);
                 const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][rr][d]);
                 sum += f;
-                acc.x = fmaf(f, x.x, acc.x);
-                acc.y = fmaf(f, x.y, acc.y);
-                acc.z = fmaf(f, x.z, acc.z);
-                acc.w = fmaf(f, x.w, acc.w);
+                acc[0] = fmaf(f, x.x, acc[0]);
+                acc[1] = fmaf(f, x.y, acc[1]);
+                acc[2] = fmaf(f, x.z, acc[2]);
+                acc[3] = fmaf(f, x.w, acc[3]);
             }
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            acc.x *= inv;
-            acc.y *= inv;
-            acc.z *= inv;
-            acc.w *= inv;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) acc[k] *= inv;
+            if (any_bad) {
+                const int lo = max(blk_lo, max(all_see, 0) / kKv8Block) * kKv8Block, lim = all_see + r % a.n_q;
+                const int hi = min(split == a.splits - 1 ? n : blk_hi * kKv8Block, lim);
+                for (int t = lo; t < hi; ++t)
+                    for (int k = 0; k < 4; ++k) {
+                        float v = 0.f;
+                        if (t >= full * kKv8Block)
+                            v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.c.v_tail)[(bh * kKv8Block + t % kKv8Block) * kKv8Dim + d + k]);
+                        else if (FMT == MINF_KV8_E4M3 && (static_cast<const uint8_t*>(a.c.v)[(bh * a.c.capacity + t) * kKv8Dim + d + k] & 0x7f) == 0x7f)
+                            v = CUDART_NAN_F;
+                        if (!(fabsf(v) < CUDART_INF_F)) acc[k] += v;
+                    }
+            }
             const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
             const size_t row = bh * a.rows + r;
             if (a.splits > 1) {
-                *reinterpret_cast<float4*>(a.part_o + (row * a.splits + split) * kKv8Dim + d) = acc;
+                *reinterpret_cast<float4*>(a.part_o + (row * a.splits + split) * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
                 if (d == 0) a.part_lse[row * a.splits + split] = lse;
             } else {
                 const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
                 __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
-                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x, acc.y), pack_bf16x2(acc.z, acc.w));
+                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
                 if (d == 0) {
                     if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = lse;
                     if (a.row_lse) a.row_lse[row] = lse;
@@ -565,7 +594,7 @@ struct AttnShape {
 static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
     AttnShape s{};
     const long long rows = (long long)(hq / heads) * n_q;
-    s.nt = rows <= 8 ? 1 : 0;
+    s.nt = rows <= kNarrowRows ? (int)((rows + 7) / 8) : 0;
     s.tiles = s.nt ? 1 : (int)((rows + kWideRows - 1) / kWideRows);
     const long long ctas = (long long)batch * heads * s.tiles;
     const long long blocks = max_length / kKv8Block;
@@ -607,18 +636,30 @@ static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_le
     return batch >= 1 && heads >= 1 && hq >= heads && hq % heads == 0 && n_q >= 1 && max_length >= 0 && (long long)hq * n_q <= (1 << 24);
 }
 
-template <int FMT, int NT>
-static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
+template <int FMT, int NT, bool LOGITS>
+static cudaError_t launch_narrow(const Kv8AttnArgs& a, cudaStream_t stream) {
+    constexpr int bytes = kRingBytes + (NT > 2 ? NT * 2048 : 0);
     // per device, and cheap: every call sets it
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<FMT, NT>, cudaFuncAttributeMaxDynamicSharedMemorySize, kRingBytes);
+    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<FMT, NT, LOGITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    kv8_attention_kernel<FMT, NT><<<dim3(s.splits, a.c.heads * s.tiles, a.c.batch), kAttnThreads, kRingBytes, stream>>>(a);
+    kv8_attention_kernel<FMT, NT, LOGITS><<<dim3(a.splits, a.c.heads, a.c.batch), kAttnThreads, bytes, stream>>>(a);
     return cudaGetLastError();
+}
+
+template <int FMT, bool LOGITS>
+static cudaError_t launch_narrow(const Kv8AttnArgs& a, int nt, cudaStream_t stream) {
+    switch (nt) {
+        case 1: return launch_narrow<FMT, 1, LOGITS>(a, stream);
+        case 2: return launch_narrow<FMT, 2, LOGITS>(a, stream);
+        case 3: return launch_narrow<FMT, 3, LOGITS>(a, stream);
+        default: return launch_narrow<FMT, 4, LOGITS>(a, stream);
+    }
 }
 
 static cudaError_t launch_attention(const Kv8AttnArgs& a, const AttnShape& s, cudaStream_t stream) {
     if (!s.nt) return launch_attention_wide(a, s.tiles, stream);
-    return a.c.format == MINF_KV8_E4M3 ? launch_attention<MINF_KV8_E4M3, 1>(a, s, stream) : launch_attention<MINF_KV8_INT8, 1>(a, s, stream);
+    if (a.c.format == MINF_KV8_E4M3) return a.logits ? launch_narrow<MINF_KV8_E4M3, true>(a, s.nt, stream) : launch_narrow<MINF_KV8_E4M3, false>(a, s.nt, stream);
+    return a.logits ? launch_narrow<MINF_KV8_INT8, true>(a, s.nt, stream) : launch_narrow<MINF_KV8_INT8, false>(a, s.nt, stream);
 }
 
 }  // namespace minf
