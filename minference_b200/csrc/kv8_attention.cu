@@ -13,8 +13,8 @@
 // half a step of 2^-11 relative, below the bf16 rounding of the output; sums and outputs are accumulated in fp32.
 // The tail (bf16) takes bf16 products, with P as a sum of two bf16 numbers.
 //
-// The tokens of a sequence are split over CTAs and, inside one, over warps by blocks of 64; the parts are joined by
-// their log-sum-exps in a second kernel.
+// The tokens are split over CTAs and, inside one, over warps by units of 32; the parts are joined by their log-sum-exps in a
+// second kernel, launched behind the first one's end.
 #include "kv8_attention.cuh"
 
 #include <math_constants.h>
@@ -25,12 +25,12 @@
 
 namespace minf {
 
-constexpr int kAttnWarps = 4;
-constexpr int kAttnThreads = kAttnWarps * 32;
-constexpr int kSlotBytes = kKv8Block * kKv8Dim;     // keys or values of a block
+constexpr int kUnit = 32;                           // tokens a warp takes at a time: half a block
+constexpr int kSlotBytes = kUnit * kKv8Dim;         // their keys or values
 constexpr int kRingSlots = 3;
 constexpr int kNarrowRows = 32;                     // rows per cache head this kernel takes
-constexpr int kRingBytes = kAttnWarps * kRingSlots * kSlotBytes;
+// warps of a CTA: two CTAs fit an SM with 128 registers a thread for one group of rows, twice that for more
+__host__ __device__ constexpr int narrow_warps(int nt) { return nt == 1 ? 8 : 4; }
 
 __device__ __forceinline__ void mma_f16(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -124,16 +124,17 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             mx0 = fmaxf(mx0, fmaxf(x[0], x[2]));
             mx1 = fmaxf(mx1, fmaxf(x[1], x[3]));
         }
-#pragma unroll
-        for (int o = 4; o < 32; o <<= 1) {
-            mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
-            mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
-        }
-        // the reference is raised on a jump of more than 2^8: P stays far below f16's largest, and outputs are rarely rescaled
+        // the reference is raised on a jump of more than 2^8: P stays far below f16's largest, outputs are rarely rescaled,
+        // and the lanes compare their maxima only then
         mx0 += lv;
         mx1 += lv;
-        const bool up0 = mx0 > R.m[nt][0] + 8.f, up1 = mx1 > R.m[nt][1] + 8.f;
-        if (__any_sync(0xffffffffu, up0 || up1)) {
+        if (__any_sync(0xffffffffu, mx0 > R.m[nt][0] + 8.f || mx1 > R.m[nt][1] + 8.f)) {
+#pragma unroll
+            for (int o = 4; o < 32; o <<= 1) {
+                mx0 = fmaxf(mx0, __shfl_xor_sync(0xffffffffu, mx0, o));
+                mx1 = fmaxf(mx1, __shfl_xor_sync(0xffffffffu, mx1, o));
+            }
+            const bool up0 = mx0 > R.m[nt][0] + 8.f, up1 = mx1 > R.m[nt][1] + 8.f;
             const float a0 = up0 ? fast_exp2(R.m[nt][0] - mx0) : 1.f, a1 = up1 ? fast_exp2(R.m[nt][1] - mx1) : 1.f;
             if (up0) R.m[nt][0] = mx0;
             if (up1) R.m[nt][1] = mx1;
@@ -165,24 +166,123 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
     }
 }
 
+// How the narrow kernel's CTAs share the work: the tokens of all sequences and heads are one row of units, (sequence, head,
+// unit) in that order, and CTA i of N takes the units [U i / N, U (i + 1) / N).  Sequences of any lengths keep every CTA
+// equally busy; where a CTA's share crosses into another head or sequence, it works on pieces one after the other.  The
+// tail counts as a unit for each of the W warps.  Every CTA finds its place from the lengths by itself (a warp scans 32
+// sequences at a time), so lengths may live on the device.
+struct Place {
+    int b, h, u, n;
+};
+template <int W>
+__host__ __device__ constexpr int units_of(int n) {
+    return n / kKv8Block * (kKv8Block / kUnit) + (n % kKv8Block ? W : 0);
+}
+__device__ __forceinline__ int clipped_length(const Kv8AttnArgs& a, int b) {
+    const int n = a.lengths ? a.lengths[b] : a.length_all;
+    return max(0, min(n, a.max_length));
+}
+template <int W>
+__device__ __forceinline__ long long total_units(const Kv8AttnArgs& a, bool report) {
+    if (!a.lengths) return (long long)a.c.batch * a.c.heads * units_of<W>(a.length_all);
+    const int lane = threadIdx.x & 31;
+    long long sum = 0;
+    for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
+        int x = 0;
+        if (b0 + lane < a.c.batch) {
+            const int n = clipped_length(a, b0 + lane);
+            if (report && threadIdx.x < 32 && n != a.lengths[b0 + lane]) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
+            x = units_of<W>(n);
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        sum += x;
+    }
+    return sum * a.c.heads;
+}
+// CTAs that get work: every warp of one a unit, as far as there are
+template <int W>
+__device__ __forceinline__ int pieces_ctas(long long units, int ctas) {
+    return (int)min((long long)ctas, (units + W - 1) / W);
+}
+// the CTA that has a unit
+__device__ __forceinline__ long long owner_of(long long unit, long long units, int ctas) { return ((unit + 1) * ctas - 1) / units; }
+
+template <int W>
+__device__ __forceinline__ Place locate(const Kv8AttnArgs& a, long long at) {
+    const int lane = threadIdx.x & 31;
+    if (!a.lengths) {
+        const int per = units_of<W>(a.length_all);
+        const int bh = (int)(at / per);
+        return {bh / a.c.heads, bh % a.c.heads, (int)(at % per), a.length_all};
+    }
+    for (int b0 = 0;; b0 += 32) {
+        const int n = b0 + lane < a.c.batch ? clipped_length(a, b0 + lane) : 0;
+        const long long mine = (long long)units_of<W>(n) * a.c.heads;
+        long long upto = mine;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
+            if (lane >= o) upto += y;
+        }
+        const unsigned here = __ballot_sync(0xffffffffu, at < upto);
+        if (here) {
+            const int src = __ffs(here) - 1;
+            const int nb = __shfl_sync(0xffffffffu, n, src);
+            const long long rest = at - __shfl_sync(0xffffffffu, upto - mine, src);        // within the sequence's heads
+            const int per = units_of<W>(nb);
+            return {b0 + src, (int)(rest / per), (int)(rest % per), nb};
+        }
+        if (b0 + 32 >= a.c.batch) return {0, 0, 0, 0};          // (not reached: `at` is below the total)
+        at -= __shfl_sync(0xffffffffu, upto, 31);
+    }
+}
+// units before sequence b
+template <int W>
+__device__ __forceinline__ long long units_before(const Kv8AttnArgs& a, int b) {
+    if (!a.lengths) return (long long)b * a.c.heads * units_of<W>(a.length_all);
+    const int lane = threadIdx.x & 31;
+    long long sum = 0;
+    for (int b0 = 0; b0 < b; b0 += 32) {
+        int x = b0 + lane < b ? units_of<W>(clipped_length(a, b0 + lane)) : 0;
+#pragma unroll
+        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+        sum += x;
+    }
+    return sum * a.c.heads;
+}
+
 template <int FMT, int NT, bool LOGITS>
-__global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    constexpr int SUB = 4 / NT;                     // sub-tiles of 16 tokens per softmax step: up to 16 logits a lane
-    constexpr int PARTS = 4 / SUB;                  // softmax steps of a block
+__global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    constexpr int kAttnWarps = narrow_warps(NT), kAttnThreads = kAttnWarps * 32, kRingBytes = kAttnWarps * kRingSlots * kSlotBytes;
+    constexpr int SUB = NT == 2 ? 2 : 1;            // sub-tiles of 16 tokens per softmax step: two hide latencies where registers allow
+    constexpr int PARTS = kUnit / 16 / SUB;         // softmax steps of a unit
     constexpr bool kQShared = NT > 2;               // Q's fragments in shared memory (from there each is read once per sub-tile)
     extern __shared__ __align__(128) unsigned char ring_all[];
-    const int split = blockIdx.x, h = blockIdx.y, b = blockIdx.z;
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
-    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
+    dependents_launch();
+    const long long all_units = total_units<kAttnWarps>(a, blockIdx.x == 0);
+    const int ctas = pieces_ctas<kAttnWarps>(all_units, a.splits);
+    if ((int)blockIdx.x >= ctas) return;
+    long long at = all_units * blockIdx.x / ctas;
+    const long long stop = all_units * (blockIdx.x + 1) / ctas;
+#pragma unroll 1
+    while (at < stop) {                             // a piece: units of one sequence and head
+    const Place place = locate<kAttnWarps>(a, at);
+    const int h = place.h, b = place.b, n = place.n;
     const size_t bh = (size_t)b * a.c.heads + h;
     const int full = n / kKv8Block;                 // complete blocks
-    // the last split takes the tail too, which keeps all four warps busy: it counts as four blocks
-    const int units = full + (n % kKv8Block ? kAttnWarps : 0);
-    const int blk_lo = min(full, (int)((long long)units * split / a.splits)), blk_hi = min(full, (int)((long long)units * (split + 1) / a.splits));
+    const int full_u = full * (kKv8Block / kUnit), units = units_of<kAttnWarps>(n);
+    const int x_lo = place.u, x_hi = (int)min((long long)units, x_lo + (stop - at));
+    const int u_lo = min(full_u, x_lo), u_hi = min(full_u, x_hi);
+    const bool takes_tail = x_hi == units;          // the tail's units: its last one's piece takes all of it
+    const bool whole = x_lo == 0 && x_hi == units;  // nothing to join: the output is written here
+    const size_t piece = blockIdx.x + bh;           // pieces are numbered so: both grow along the units, one of them at each new piece
+    at += x_hi - x_lo;
     const int all_see = n - a.n_q + 1;              // tokens below this are seen by every row
 
-    // The warp's own ring of three slots of 8 KB: keys of a block, values of it, keys of its next block, ...; two
-    // copies are in flight while the third is used.  16-byte chunk ch of row r lies at ch ^ (r & 7).
+    // The warp's own ring of three slots of 4 KB: keys of a unit, values of it, keys of its next unit, ...; two copies
+    // are in flight while the third is used.  16-byte chunk ch of row r lies at ch ^ (r & 7).
     unsigned char* const ring = ring_all + warp * (kRingSlots * kSlotBytes);
     const uint32_t ring_u = smem_u32(ring);
     const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4)) << 4);
@@ -190,20 +290,21 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
         src += lane * 16;
         const uint32_t dst = ring_u + slot * kSlotBytes;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) cp_async_16(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i);
+        for (int i = 0; i < kSlotBytes / 512; ++i) cp_async_16(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i);
     };
     const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
     const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
-    const size_t first = (bh * (a.c.capacity / kKv8Block) + blk_lo + warp) * kSlotBytes;
+    const size_t first = (bh * (a.c.capacity / kUnit) + u_lo + warp) * kSlotBytes;
     const uint8_t* next_k = static_cast<const uint8_t*>(a.c.k) + first;
     const uint8_t* next_v = static_cast<const uint8_t*>(a.c.v) + first;
     float k_scale = 1.f, v_scale = 1.f;
-    if (blk_lo + warp < blk_hi) {
+    auto scale_at = [](int u) { return u / (kKv8Block / kUnit); };
+    if (u_lo + warp < u_hi) {
         fetch(0, next_k);
         cp_async_commit();
         fetch(1, next_v);
-        k_scale = ks[blk_lo + warp];
-        v_scale = vs[blk_lo + warp];
+        k_scale = ks[scale_at(u_lo + warp)];
+        v_scale = vs[scale_at(u_lo + warp)];
     } else {
         cp_async_commit();
     }
@@ -277,17 +378,17 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
 
     constexpr size_t kHop = (size_t)kAttnWarps * kSlotBytes;
     int slot = 0;
-    for (int blk = blk_lo + warp; blk < blk_hi; blk += kAttnWarps) {
-        const bool more = blk + kAttnWarps < blk_hi;
-        const bool masked = (blk + 1) * kKv8Block > all_see;
+    for (int u = u_lo + warp; u < u_hi; u += kAttnWarps) {
+        const bool more = u + kAttnWarps < u_hi;
+        const bool masked = (u + 1) * kUnit > all_see;
         const float ksc = k_scale, vsc = v_scale;
         next_k += kHop;
         next_v += kHop;
         const int slot_v = slot == 2 ? 0 : slot + 1, slot_n = slot_v == 2 ? 0 : slot_v + 1;
         if (more) {
             fetch(slot_n, next_k);
-            k_scale = ks[blk + kAttnWarps];
-            v_scale = vs[blk + kAttnWarps];
+            k_scale = ks[scale_at(u + kAttnWarps)];
+            v_scale = vs[scale_at(u + kAttnWarps)];
         }
         cp_async_commit();
         cp_async_wait<2>();
@@ -297,7 +398,7 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
         bool v_here = false;
 #pragma unroll 1
         for (int part = 0; part < PARTS; ++part) {
-            const int t0 = blk * kKv8Block + part * SUB * 16;
+            const int t0 = u * kUnit + part * SUB * 16;
             float s[SUB][NT][4];
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
@@ -364,15 +465,15 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
             }
         }
         __syncwarp();
-        // both slots are free: the values of the next block take the one the keys were in
+        // both slots are free: the values of the next unit take the one the keys were in
         if (more) fetch(slot, next_v);
         cp_async_commit();
         slot = slot_n;
     }
 
-    // the tail: the last split's warps take 16 of its tokens each
+    // the tail: four warps take 16 of its tokens each
     const int t0 = full * kKv8Block + 16 * warp;
-    if (split == a.splits - 1 && t0 < n) {
+    if (takes_tail && warp < 4 && t0 < n) {
         const __nv_bfloat16* kt = static_cast<const __nv_bfloat16*>(a.c.k_tail) + (bh * kKv8Block + 16 * warp) * kKv8Dim;
         const __nv_bfloat16* vt = static_cast<const __nv_bfloat16*>(a.c.v_tail) + (bh * kKv8Block + 16 * warp) * kKv8Dim;
         float s[1][NT][4];
@@ -436,8 +537,8 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
         }
     }
 
-    // Join the warps, eight rows at a time.  Where a row did not see all of a block's tokens, values that are infinite or
-    // NaN were left out of the products (zero times them would not be zero) and are added here to the rows that see them.
+    // Join the warps, eight rows at a time.  In units that some row does not see to their end and in the tail, values that
+    // are infinite or NaN were left out of the products (zero times them would not be zero) and are added here to the rows that see them.
     const bool any_bad = __syncthreads_or(bad);     // (and the rings are read out)
     float (*sm_o)[8][kKv8Dim] = reinterpret_cast<float (*)[8][kKv8Dim]>(ring_all);
     float (*sm_lse)[8] = reinterpret_cast<float (*)[8]>(ring_all + kAttnWarps * 8 * kKv8Dim * sizeof(float));
@@ -482,8 +583,8 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
 #pragma unroll
             for (int k = 0; k < 4; ++k) acc[k] *= inv;
             if (any_bad) {
-                const int lo = max(blk_lo, max(all_see, 0) / kKv8Block) * kKv8Block, lim = all_see + r % a.n_q;
-                const int hi = min(split == a.splits - 1 ? n : blk_hi * kKv8Block, lim);
+                const int lo = max(u_lo * kUnit, min(max(all_see, 0) / kUnit * kUnit, full * kKv8Block)), lim = all_see + r % a.n_q;
+                const int hi = min(takes_tail ? n : u_hi * kUnit, lim);
                 for (int t = lo; t < hi; ++t)
                     for (int k = 0; k < 4; ++k) {
                         float v = 0.f;
@@ -495,42 +596,117 @@ __global__ void __launch_bounds__(kAttnThreads) kv8_attention_kernel(const __gri
                     }
             }
             const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
-            const size_t row = bh * a.rows + r;
-            if (a.splits > 1) {
-                *reinterpret_cast<float4*>(a.part_o + (row * a.splits + split) * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-                if (d == 0) a.part_lse[row * a.splits + split] = lse;
+            const size_t row = piece * a.rows + r;
+            if (d == 0) a.part_lse[row] = lse;
+            if (!whole) {
+                *reinterpret_cast<float4*>(a.part_o + row * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
             } else {
                 const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
                 __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
                 *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
-                if (d == 0) {
-                    if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = lse;
-                    if (a.row_lse) a.row_lse[row] = lse;
-                }
+                if (d == 0 && a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = lse;
             }
         }
         __syncthreads();
     }
+    }
 }
 
-// The splits of one row joined: four warps take every fourth split, a lane four dims.
-__global__ void __launch_bounds__(128) kv8_combine_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    __shared__ float4 sm[4][32];
-    __shared__ float sm_sum[4];
-    const size_t row = blockIdx.x;
+// Parts of a row: `count` of them, the first at row `base` of part_o / part_lse, `step` rows apart.
+struct Parts {
+    size_t base, step;
+    int count;
+};
+template <int W>
+__device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r) {
+    if constexpr (W == 0) {                         // wide kernel: a fixed number of splits
+        return {(bh * a.rows + r) * a.splits, 1, a.splits};
+    } else {
+        const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+        const long long all = total_units<W>(a, false);
+        const int ctas = pieces_ctas<W>(all, a.splits);
+        const int per = units_of<W>(a.lengths ? clipped_length(a, b) : a.length_all);
+        if (per == 0) return {0, 0, 0};
+        const long long start = units_before<W>(a, b) + (long long)h * per;
+        const long long lo = owner_of(start, all, ctas), hi = owner_of(start + per - 1, all, ctas);
+        return {((size_t)lo + bh) * a.rows + r, (size_t)a.rows, (int)(hi - lo + 1)};
+    }
+}
+
+constexpr int kFinishThreads = 256;
+constexpr int kFinishTokens = 1024;                 // tokens of a CTA that sums weights
+
+// weights of tokens [t0, t0 + kFinishTokens) of a head: the probabilities of its rows, summed in their order
+__device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, int n, int t0, const float* row_lse) {
+    const size_t bh = (size_t)b * a.c.heads + h;
+    for (int t = t0 + threadIdx.x; t < min(n, t0 + kFinishTokens); t += kFinishThreads) {
+        const float* x = a.logits + ((long long)bh * a.tokens + t) * a.pitch;
+        const float was = a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f;
+        float sum = 0.f;
+#pragma unroll 4
+        for (int r = 0; r < a.rows; r += 2) {
+            const float2 l = *reinterpret_cast<const float2*>(x + r);
+            sum += l.x == -CUDART_INF_F ? 0.f : exp2f(l.x - row_lse[r]);
+            if (r + 1 < a.rows) sum += l.y == -CUDART_INF_F ? 0.f : exp2f(l.y - row_lse[r + 1]);
+        }
+        a.weights[b * a.ws[0] + h * a.ws[1] + t] = was + sum;
+    }
+}
+
+// The first CTAs join the parts of one row each: eight warps take every eighth part, a lane four dims.  The others (narrow
+// kernel) sum the weights, for which they join the log-sum-exps of their head's rows themselves: no second wait.
+template <int W>
+__global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    __shared__ float4 sm[8][32];
+    __shared__ float sm_sum[8];
+    __shared__ float sm_lse[kNarrowRows];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const float* lse = a.part_lse + row * a.splits;
+    const size_t rows = (size_t)a.c.batch * a.c.heads * a.rows;
+    dependents_launch();
+    if (blockIdx.x >= rows) {
+        if constexpr (W > 0) {
+            const int chunks = (int)((a.tokens + kFinishTokens - 1) / kFinishTokens);
+            const int i = (int)(blockIdx.x - rows), chunk = i % chunks;
+            const size_t bh = i / chunks;
+            const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+            const int n = clipped_length(a, b);
+            const Parts p = parts_of<W>(a, bh, 0);
+            dependents_wait();
+            if (chunk * kFinishTokens >= n) return;
+            for (int r = warp; r < a.rows; r += 8) {
+                float top = -CUDART_INF_F, sum = 0.f;
+                for (int k = lane; k < p.count; k += 32) top = fmaxf(top, a.part_lse[p.base + r + k * p.step]);
+#pragma unroll
+                for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+                for (int k = lane; k < p.count; k += 32) {
+                    const float e = a.part_lse[p.base + r + k * p.step];
+                    sum += e == -CUDART_INF_F ? 0.f : exp2f(e - top);
+                }
+#pragma unroll
+                for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
+                if (lane == 0) sm_lse[r] = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+            }
+            __syncthreads();
+            sum_weights(a, b, h, n, chunk * kFinishTokens, sm_lse);
+        }
+        return;
+    }
+    const size_t bh = blockIdx.x / a.rows;
+    const int r = (int)(blockIdx.x % a.rows), b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+    const Parts p = parts_of<W>(a, bh, r);
+    dependents_wait();
+    if (W > 0 && p.count == 1) return;              // the attention kernel wrote this row itself
     float top = -CUDART_INF_F;
-    for (int i = lane; i < a.splits; i += 32) top = fmaxf(top, lse[i]);
+    for (int k = lane; k < p.count; k += 32) top = fmaxf(top, a.part_lse[p.base + k * p.step]);
 #pragma unroll
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int i = warp; i < a.splits; i += 4) {
-        const float e = lse[i];
-        if (e == -CUDART_INF_F) continue;
-        const float f = exp2f(e - top);
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (row * a.splits + i) * kKv8Dim + 4 * lane);
+#pragma unroll 4
+    for (int k = warp; k < p.count; k += 8) {
+        const float e = a.part_lse[p.base + k * p.step];
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p.base + k * p.step) * kKv8Dim + 4 * lane);
+        const float f = e == -CUDART_INF_F ? 0.f : exp2f(e - top);     // (a part that saw nothing holds zeros)
         sum += f;
         acc.x = fmaf(f, x.x, acc.x);
         acc.y = fmaf(f, x.y, acc.y);
@@ -541,71 +717,59 @@ __global__ void __launch_bounds__(128) kv8_combine_kernel(const __grid_constant_
     if (lane == 0) sm_sum[warp] = sum;
     __syncthreads();
     if (warp) return;
-    sum = sm_sum[0] + sm_sum[1] + sm_sum[2] + sm_sum[3];
-    acc = sm[0][lane];
+    sum = 0.f;
+    acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-    for (int w = 1; w < 4; ++w) {
+    for (int w = 0; w < 8; ++w) {
         const float4 x = sm[w][lane];
+        sum += sm_sum[w];
         acc.x += x.x;
         acc.y += x.y;
         acc.z += x.z;
         acc.w += x.w;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const size_t bh = row / a.rows;
-    const int r = (int)(row % a.rows), b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
     const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
     __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + 4 * lane;
     *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
     if (lane == 0) {
         const float e = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
         if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = e;
-        if (a.row_lse) a.row_lse[row] = e;
+        if (W == 0 && a.row_lse) a.row_lse[bh * a.rows + r] = e;
     }
 }
 
-// Attention weight of every token of a head: the probabilities of the head's rows, summed in their order.
-__global__ void __launch_bounds__(256) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    const int b = blockIdx.z, h = blockIdx.y;
-    const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
-    const int t = blockIdx.x * 256 + threadIdx.x;
-    if (t >= n) return;
-    const size_t bh = (size_t)b * a.c.heads + h;
-    const float* x = a.logits + ((long long)bh * a.tokens + t) * a.pitch;
-    const float* e = a.row_lse + bh * a.rows;
-    float sum = 0.f;
-    for (int r = 0; r < a.rows; r += 2) {
-        const float2 l = *reinterpret_cast<const float2*>(x + r);
-        const float e0 = e[r];
-        sum += l.x == -CUDART_INF_F ? 0.f : exp2f(l.x - e0);
-        if (r + 1 < a.rows) sum += l.y == -CUDART_INF_F ? 0.f : exp2f(l.y - e[r + 1]);
-    }
-    const float was = a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f;
-    a.weights[b * a.ws[0] + h * a.ws[1] + t] = was + sum;
+// Weights after the wide kernel: its rows' log-sum-exps are joined by then.
+__global__ void __launch_bounds__(kFinishThreads) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    const int b = blockIdx.z, h = blockIdx.y, n = clipped_length(a, b);
+    dependents_wait();
+    if ((int)blockIdx.x * kFinishTokens >= n) return;
+    sum_weights(a, b, h, n, blockIdx.x * kFinishTokens, a.row_lse + ((size_t)b * a.c.heads + h) * a.rows);
 }
 
 // ---------------------------------------------------------------------------------------------------- host
 struct AttnShape {
-    int nt, tiles, splits, pitch;
+    int nt;                         // column groups of the narrow kernel, 0: the wide kernel
+    int tiles, splits, pitch;
     long long tokens;
     size_t part_o, part_lse, row_lse, logits, bytes;
 };
 
 static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
     AttnShape s{};
-    const long long rows = (long long)(hq / heads) * n_q;
+    const long long rows = (long long)(hq / heads) * n_q, pairs = (long long)batch * heads;
     s.nt = rows <= kNarrowRows ? (int)((rows + 7) / 8) : 0;
     s.tiles = s.nt ? 1 : (int)((rows + kWideRows - 1) / kWideRows);
-    const long long ctas = (long long)batch * heads * s.tiles;
-    const long long blocks = max_length / kKv8Block;
+    long long parts;                // rows of partial results
     if (s.nt) {
-        long long splits = (2 * kSMs + ctas - 1) / ctas;
-        splits = std::min(splits, (blocks + kAttnWarps - 1) / kAttnWarps);
-        s.splits = (int)std::max(splits, 1ll);
+        const int warps = narrow_warps(s.nt);
+        const long long units = (long long)(max_length / kKv8Block) * (kKv8Block / kUnit) + warps;
+        s.splits = (int)std::min<long long>(2 * kSMs, (pairs * units + warps - 1) / warps);
+        parts = (s.splits + pairs) * rows;
     } else {
         // one CTA an SM: the number of splits (of two tiles of tokens at least) that wastes least of its last wave; each
         // costs about as much again as two tiles (its start, its end and the joining)
-        const long long tiles = (max_length + 127) / 128;
+        const long long ctas = pairs * s.tiles, tiles = (max_length + 127) / 128;
         double best = 1e30;
         for (long long k = 1; k <= std::max(1ll, tiles / 2) && k <= kSMs; ++k) {
             const double cost = (double)((ctas * k + kSMs - 1) / kSMs) * ((double)((tiles + k - 1) / k) + 2.0);
@@ -614,20 +778,20 @@ static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_
                 s.splits = (int)k;
             }
         }
+        parts = s.splits > 1 ? pairs * rows * s.splits : 0;
     }
     s.pitch = (int)((rows + 1) / 2 * 2);
     s.tokens = max_length;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
-    const size_t all = (size_t)batch * heads * rows;
     size_t at = 0;
     s.part_o = at;
-    if (s.splits > 1) at = up(at + all * s.splits * kKv8Dim * sizeof(float));
+    at = up(at + (size_t)parts * kKv8Dim * sizeof(float));
     s.part_lse = at;
-    if (s.splits > 1) at = up(at + all * s.splits * sizeof(float));
+    at = up(at + (size_t)parts * sizeof(float));
     s.row_lse = at;
-    if (weights) at = up(at + all * sizeof(float));
+    if (weights && !s.nt) at = up(at + (size_t)pairs * rows * sizeof(float));
     s.logits = at;
-    if (weights) at = up(at + (size_t)batch * heads * s.tokens * s.pitch * sizeof(float));
+    if (weights) at = up(at + (size_t)pairs * s.tokens * s.pitch * sizeof(float));
     s.bytes = at;
     return s;
 }
@@ -638,11 +802,11 @@ static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_le
 
 template <int FMT, int NT, bool LOGITS>
 static cudaError_t launch_narrow(const Kv8AttnArgs& a, cudaStream_t stream) {
-    constexpr int bytes = kRingBytes + (NT > 2 ? NT * 2048 : 0);
+    constexpr int bytes = narrow_warps(NT) * kRingSlots * kSlotBytes + (NT > 2 ? NT * 2048 : 0);
     // per device, and cheap: every call sets it
     const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<FMT, NT, LOGITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
     if (e != cudaSuccess) return e;
-    kv8_attention_kernel<FMT, NT, LOGITS><<<dim3(a.splits, a.c.heads, a.c.batch), kAttnThreads, bytes, stream>>>(a);
+    kv8_attention_kernel<FMT, NT, LOGITS><<<a.splits, narrow_warps(NT) * 32, bytes, stream>>>(a);
     return cudaGetLastError();
 }
 
@@ -684,8 +848,11 @@ extern "C" int minf_kv8_attention(
     if (!lengths && (length_all < 0 || length_all > max_length)) return fail(MINF_E_ARG, "length %d is outside [0, max_length %d]", length_all, max_length);
     if (add_to && !weights) return fail(MINF_E_ARG, "add_to without weights");
     const AttnShape s = attention_shape(cache->batch, hq, cache->heads, n_q, max_length, weights != nullptr);
+    const long long a_rows = (long long)(hq / cache->heads) * n_q;
     if (s.bytes && !scratch) return fail(MINF_E_ARG, "scratch is needed (%zu bytes)", s.bytes);
     if (reinterpret_cast<uintptr_t>(scratch) & 15) return fail(MINF_E_ARG, "scratch must be 16-byte aligned");
+    if (s.bytes > (size_t)1 << 46 || ((long long)max_length / kFinishTokens + 1 + a_rows) * cache->heads * cache->batch > 0x7fffffffll)
+        return fail(MINF_E_UNSUPPORTED, "too large a call (%d sequences, %d heads, %lld rows)", cache->batch, cache->heads, a_rows);
     if ((long long)cache->heads * s.tiles > 65535) return fail(MINF_E_UNSUPPORTED, "too many query rows (%d heads of %d tiles)", cache->heads, s.tiles);
     Kv8AttnArgs a{};
     a.c = *cache;
@@ -712,7 +879,7 @@ extern "C" int minf_kv8_attention(
     a.pitch = s.pitch;
     a.tokens = s.tokens;
     if (weights) {
-        a.row_lse = reinterpret_cast<float*>(base + s.row_lse);
+        if (!s.nt) a.row_lse = reinterpret_cast<float*>(base + s.row_lse);
         a.logits = reinterpret_cast<float*>(base + s.logits);
         a.weights = weights;
         a.ws[0] = w_strides[0];
@@ -724,15 +891,24 @@ extern "C" int minf_kv8_attention(
         }
     }
     cudaStream_t st = static_cast<cudaStream_t>(stream);
-    const cudaError_t e = launch_attention(a, s, st);
+    cudaError_t e = launch_attention(a, s, st);
     if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_attention_kernel failed: %s", cudaGetErrorString(e));
-    if (s.splits > 1) {
-        kv8_combine_kernel<<<(unsigned)((size_t)cache->batch * cache->heads * a.rows), 128, 0, st>>>(a);
-        MINF_LAUNCH_OK("kv8_combine_kernel");
+    const long long pairs = (long long)cache->batch * cache->heads, rows = pairs * a.rows;
+    const long long chunks = weights ? ((long long)max_length + kFinishTokens - 1) / kFinishTokens : 0;
+    if (s.nt) {
+        const dim3 grid((unsigned)(rows + pairs * chunks));
+        e = narrow_warps(s.nt) == 8 ? launch_behind(kv8_finish_kernel<8>, grid, kFinishThreads, 0, st, a)
+                                    : launch_behind(kv8_finish_kernel<4>, grid, kFinishThreads, 0, st, a);
+        if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
+        return MINF_OK;
     }
-    if (weights && max_length > 0) {
-        kv8_weights_kernel<<<dim3((max_length + 255) / 256, cache->heads, cache->batch), 256, 0, st>>>(a);
-        MINF_LAUNCH_OK("kv8_weights_kernel");
+    if (s.splits > 1) {
+        e = launch_behind(kv8_finish_kernel<0>, dim3((unsigned)rows), kFinishThreads, 0, st, a);
+        if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
+    }
+    if (chunks) {
+        e = launch_behind(kv8_weights_kernel, dim3((unsigned)chunks, cache->heads, cache->batch), kFinishThreads, 0, st, a);
+        if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_weights_kernel failed: %s", cudaGetErrorString(e));
     }
     return MINF_OK;
 }

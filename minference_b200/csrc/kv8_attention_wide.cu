@@ -166,6 +166,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
     const int count = j_hi - j_lo;                  // this CTA's tiles
     const bool has_tail = j_hi == (n + kWideTile - 1) / kWideTile && n % kKv8Block && count > 0;
 
+    dependents_launch();
     auto bar = [&](const unsigned long long* p) { return smem_u32(p); };
     volatile int* abort_flag = &ctl->abort;
     if (threadIdx.x == 0) {
