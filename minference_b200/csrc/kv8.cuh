@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <cstdint>
+#include <utility>
 
 #include "common.h"
 
@@ -77,6 +78,25 @@ __device__ __forceinline__ int kv8_length(const int32_t* lengths, int all, int b
     }
     return n;
 }
+
+// A kernel that may start while the one before it in the stream ends: its launch is hidden behind that one's last CTAs.  It
+// waits for the other's results itself (dependents_wait); the other says that it may be launched (dependents_launch).
+template <class... Params, class... Args>
+cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, cudaStream_t stream, Args&&... args) {
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = shared;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
+}
+__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 // Host-side check of a cache descriptor; MINF_OK or a negative code with its message set.
 int kv8_check(const minf_kv8_cache* c);

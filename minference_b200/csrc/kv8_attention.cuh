@@ -1,7 +1,5 @@
 // Arguments shared by the kernels of the attention over an 8-bit cache (kv8_attention.cu, kv8_attention_wide.cu).
 #pragma once
-#include <utility>
-
 #include "kv8.cuh"
 
 namespace minf {
@@ -34,24 +32,5 @@ struct Kv8AttnArgs {
 
 constexpr int kWideRows = 128;      // query rows of a CTA of the wide kernel
 cudaError_t launch_attention_wide(const Kv8AttnArgs& a, int tiles, cudaStream_t stream);
-
-// A kernel that may start while the one before it in the stream ends: its launch is hidden behind that one's last CTAs.  It
-// waits for the other's results itself (dependents_wait); the other says that it may be launched (dependents_launch).
-template <class... Params, class... Args>
-cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, int threads, size_t shared, cudaStream_t stream, Args&&... args) {
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cudaLaunchConfig_t cfg{};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = shared;
-    cfg.stream = stream;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    return cudaLaunchKernelEx(&cfg, kernel, std::forward<Args>(args)...);
-}
-__device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
-__device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
 }  // namespace minf

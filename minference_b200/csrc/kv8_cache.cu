@@ -11,6 +11,8 @@
 
 #include <cooperative_groups.h>
 
+#include <algorithm>
+
 #include "sm100_ptx.cuh"
 
 namespace minf {
@@ -216,6 +218,7 @@ struct SelectArgsKv8 {
     const float* weights;           // [batch, heads, >= max_length] with the strides below, tokens contiguous
     long long w_stride[2];
     int budget, recent, sink;
+    int cached;                     // keys a CTA has room for
     int32_t* kept;                  // [batch, heads, budget]
 };
 
@@ -228,10 +231,10 @@ __device__ __forceinline__ uint32_t weight_key(float w) {
 
 constexpr int kSelectThreads = 1024;
 constexpr int kSelectWarps = kSelectThreads / 32;
-constexpr int kSelectCluster = 8;                           // CTAs that share a head's tokens
+constexpr int kSelectCluster = 8;                           // CTAs at most that share a head's tokens
+constexpr int kSelectPart = 8192;                           // tokens from which on one more is worth its barriers
 constexpr int kSelectBins = 2048;
-constexpr int kSelectCached = 40960;                        // keys a CTA keeps in shared memory
-constexpr int kSelectSmem = (kSelectBins + kSelectCached) * 4;
+constexpr int kSelectCached = 40960;                        // keys a CTA keeps in shared memory at most
 
 // A cluster per (sequence, head), each CTA a contiguous part of the candidates, whose keys it reads once and keeps in
 // shared memory (beyond 8 x 40960 candidates it reads them again from L2 in each pass).  Three passes of 11, 11 and 10
@@ -239,8 +242,7 @@ constexpr int kSelectSmem = (kSelectBins + kSelectCached) * 4;
 // shared memory and every CTA takes the same digit.  Then the warps, each with a contiguous stretch, count what they
 // keep and write it at the offset of everything before them: ascending order without a sort, equal keys by position.
 // What bounds it: the barriers of the three passes (two across the cluster each), not the 4 B a token it reads.
-__global__ void __cluster_dims__(kSelectCluster, 1, 1) __launch_bounds__(kSelectThreads)
-kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
+__global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
     extern __shared__ uint32_t dyn[];
     uint32_t* hist = dyn;
     uint32_t* cached = dyn + kSelectBins;
@@ -250,24 +252,30 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
     __shared__ uint32_t cta_above, cta_equal;
     namespace cg = cooperative_groups;
     cg::cluster_group cluster = cg::this_cluster();
-    const int part = blockIdx.x % kSelectCluster, h = blockIdx.x / kSelectCluster, b = blockIdx.y;
+    const int parts = cluster.num_blocks(), part = blockIdx.x % parts, h = blockIdx.x / parts, b = blockIdx.y;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.c.status);
+    dependents_launch();
     const float* w = a.weights + b * a.w_stride[0] + h * a.w_stride[1];
     int32_t* kept = a.kept + ((size_t)b * a.c.heads + h) * a.budget;
     if (n <= a.budget) {                                    // everything stays (the whole cluster leaves here)
-        for (int i = part * kSelectThreads + tid; i < a.budget; i += kSelectCluster * kSelectThreads) kept[i] = i < n ? i : -1;
+        for (int i = part * kSelectThreads + tid; i < a.budget; i += parts * kSelectThreads) kept[i] = i < n ? i : -1;
         return;
     }
     const int lo = a.sink, hi = n - a.recent;
-    for (int i = part * kSelectThreads + tid; i < a.sink + a.recent; i += kSelectCluster * kSelectThreads)
+    for (int i = part * kSelectThreads + tid; i < a.sink + a.recent; i += parts * kSelectThreads)
         kept[i < a.sink ? i : a.budget - a.recent + (i - a.sink)] = i < a.sink ? i : hi + (i - a.sink);
     uint32_t need = a.budget - a.sink - a.recent;           // of hi - lo > need candidates
     if (need == 0) return;
-    const int chunk = ((hi - lo + kSelectCluster - 1) / kSelectCluster + 31) / 32 * 32;
+    const int chunk = ((hi - lo + parts - 1) / parts + 31) / 32 * 32;
     const int c0 = min(hi, lo + part * chunk), c1 = min(hi, c0 + chunk), count = c1 - c0;
-    const bool in_smem = count <= kSelectCached;
+    const bool in_smem = count <= a.cached;
     auto key_at = [&](int i) { return in_smem ? cached[i] : weight_key(w[c0 + i]); };
+
+    auto sync = [&] {
+        if (parts > 1) cluster.sync();
+        else __syncthreads();
+    };
 
     uint32_t prefix = 0;
 #pragma unroll 1
@@ -289,18 +297,15 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
                 const int i = i0 + u * kSelectThreads + tid;
                 const bool live = i < count && (pass == 0 || (key[u] >> (shift + bits)) == prefix);
                 if (pass == 0 && in_smem && i < count) cached[i] = key[u];
-                const uint32_t bin = live ? (key[u] >> shift) & mask : 0xffffffffu;
-                // weights share their exponents: one addition for all lanes of a warp that hit the same bin
-                const uint32_t same = __match_any_sync(0xffffffffu, bin);
-                if (live && (__ffs(same) - 1) == lane) atomicAdd(&hist[bin], __popc(same));
+                if (live) atomicAdd(&hist[(key[u] >> shift) & mask], 1u);
             }
         }
-        cluster.sync();
+        sync();
         // thread t sums bins 2046 - 2t and 2047 - 2t over the cluster: a scan over the threads runs from the largest key down
         const int bin = kSelectBins - 2 - 2 * tid;
         uint32_t x1 = 0, x0 = 0;
-#pragma unroll
-        for (int r = 0; r < kSelectCluster; ++r) {
+#pragma unroll 1
+        for (int r = 0; r < parts; ++r) {
             const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
             x0 += v.x;
             x1 += v.y;
@@ -313,8 +318,7 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
         }
         if (lane == 31) warp_sum[warp] = scan;
         __syncthreads();
-        uint32_t before = scan - x0 - x1;
-        for (int i = 0; i < warp; ++i) before += warp_sum[i];
+        uint32_t before = scan - x0 - x1 + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
         if (before < need && need <= before + x1) {
             sh_digit = bin + 1;
             sh_need = need - before;
@@ -322,7 +326,7 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
             sh_digit = bin;
             sh_need = need - before - x1;
         }
-        cluster.sync();                                     // digit and histograms: read by all before the next pass clears them
+        sync();                                             // digit and histograms: read by all before the next pass clears them
         prefix = (prefix << bits) | sh_digit;
         need = sh_need;
     }
@@ -349,16 +353,15 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
             cta_equal = ce;
         }
     }
-    cluster.sync();
-    uint32_t gt = 0, eq = 0;                                // before this warp's stretch
-    for (int r = 0; r < part; ++r) {
-        gt += *cluster.map_shared_rank(&cta_above, r);
-        eq += *cluster.map_shared_rank(&cta_equal, r);
+    sync();
+    // before this warp's stretch: the parts before this one, the warps before this one
+    uint32_t gt = lane < warp ? warp_above[lane] : 0u, eq = lane < warp ? warp_equal[lane] : 0u;
+    if (lane < part) {
+        gt += *cluster.map_shared_rank(&cta_above, lane);
+        eq += *cluster.map_shared_rank(&cta_equal, lane);
     }
-    for (int i = 0; i < warp; ++i) {
-        gt += warp_above[i];
-        eq += warp_equal[i];
-    }
+    gt = __reduce_add_sync(0xffffffffu, gt);
+    eq = __reduce_add_sync(0xffffffffu, eq);
     const uint32_t below_lane = (1u << lane) - 1u;
     for (int i0 = s0; i0 < s1; i0 += 32) {
         const int i = i0 + lane;
@@ -373,7 +376,7 @@ kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
         gt += __popc(bg);
         eq += __popc(be);
     }
-    cluster.sync();                                         // the counts are read by the others
+    sync();                                                 // the counts are read by the others
 }
 
 struct GatherArgs {
@@ -397,6 +400,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_gather_kernel(const __grid_
     const int m = min(n, a.budget);
     const size_t bh = (size_t)b * a.src.heads + h;
     const int32_t* kept = a.kept + bh * a.budget;
+    dependents_wait();
     if (which == 0 && threadIdx.x < kKv8Block) {
         const int slot = blk * kKv8Block + threadIdx.x;
         float w = 0.f;
@@ -534,9 +538,26 @@ extern "C" int minf_kv8_evict(
     a.recent = recent;
     a.sink = sink;
     a.kept = kept;
-    MINF_CUDA_OK(cudaFuncSetAttribute(kv8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSelectSmem));
-    kv8_select_kernel<<<dim3(src->heads * kSelectCluster, src->batch), kSelectThreads, kSelectSmem, s>>>(a);
-    MINF_LAUNCH_OK("kv8_select_kernel");
+    // a CTA for every kSelectPart tokens, a power of two of them
+    int parts = 1;
+    while (parts < kSelectCluster && (long long)max_length > (long long)parts * kSelectPart) parts *= 2;
+    a.cached = std::min(kSelectCached, (max_length / parts + 64) / 32 * 32);
+    const size_t shared = (size_t)(kSelectBins + a.cached) * 4;
+    MINF_CUDA_OK(cudaFuncSetAttribute(kv8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSelectBins + kSelectCached) * 4));
+    {
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = parts;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cudaLaunchConfig_t cfg{};
+        cfg.gridDim = dim3(src->heads * parts, src->batch);
+        cfg.blockDim = dim3(kSelectThreads);
+        cfg.dynamicSmemBytes = shared;
+        cfg.stream = s;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        MINF_CUDA_OK(cudaLaunchKernelEx(&cfg, kv8_select_kernel, a));
+    }
     GatherArgs g{};
     g.src = *src;
     g.dst = *dst;
@@ -551,8 +572,7 @@ extern "C" int minf_kv8_evict(
     g.weights_out = weights_out;
     g.lengths_out = lengths_out;
     dim3 grid(dst->capacity / kKv8Block, 2 * src->heads, src->batch);
-    if (src->format == MINF_KV8_E4M3) kv8_gather_kernel<MINF_KV8_E4M3><<<grid, kStoreThreads, 0, s>>>(g);
-    else kv8_gather_kernel<MINF_KV8_INT8><<<grid, kStoreThreads, 0, s>>>(g);
-    MINF_LAUNCH_OK("kv8_gather_kernel");
+    MINF_CUDA_OK(src->format == MINF_KV8_E4M3 ? launch_behind(kv8_gather_kernel<MINF_KV8_E4M3>, grid, kStoreThreads, 0, s, g)
+                                              : launch_behind(kv8_gather_kernel<MINF_KV8_INT8>, grid, kStoreThreads, 0, s, g));
     return MINF_OK;
 }

@@ -12,7 +12,6 @@ The reference has no counterpart (its quantised cache is a 2-bit one of another 
 """
 from __future__ import annotations
 
-import contextlib
 import ctypes
 import functools
 
@@ -33,10 +32,22 @@ def _scratch_bytes(batch: int, hq: int, heads: int, n_q: int, max_length: int, w
     return _cabi.lib().minf_kv8_attention_scratch_bytes(batch, hq, heads, n_q, max_length, with_weights)
 
 
-def _on_device(cache):
-    """Context in which a launch goes to the cache's device: nothing to switch in the usual case (a decoding step is a few
-    microseconds of work, and the context manager costs one of them)."""
-    return contextlib.nullcontext() if torch.cuda.current_device() == cache.device.index else torch.cuda.device(cache.device)
+# the current stream's handle without a Stream object around it, where torch offers that (2 us less a call)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
+
+
+def _launch(entry: str, cache, *args) -> None:
+    """Call a C entry point with the current stream of the cache's device appended.  The device is switched only where it
+    is not the current one: a decoding step is a few microseconds of work."""
+    index = cache.device.index
+    fn = getattr(_cabi.lib(), entry)
+    if torch.cuda.current_device() == index:
+        rc = fn(*args, _raw_stream(index))
+    else:
+        with torch.cuda.device(index):
+            rc = fn(*args, _raw_stream(index))
+    if rc:
+        _cabi.check(rc)
 
 
 def _fail(msg: str):
@@ -66,12 +77,24 @@ class KV8Cache:
                 _fail("cache tensors must be contiguous and 16-byte aligned")
             if t.device != k.device:
                 _fail("cache tensors must be on one device")
-        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail = k, v, k_scale, v_scale, k_tail, v_tail
-        self.batch, self.kv_heads, self.capacity, self.dtype, self.device = b, h, cap, k.dtype, k.device
-        self.status = _cabi.new_status(k.device)
-        p = [t.data_ptr() for t in (k, v, k_scale, v_scale, k_tail, v_tail, self.status)]
-        self._desc = _cabi.Kv8Desc(*p, b, h, cap, _FORMATS[k.dtype])
+        self._set(k, v, k_scale, v_scale, k_tail, v_tail, _cabi.new_status(k.device))
+
+    def _set(self, k, v, k_scale, v_scale, k_tail, v_tail, status):
+        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.status = k, v, k_scale, v_scale, k_tail, v_tail, status
+        self.batch, self.kv_heads, self.capacity, _ = k.shape
+        self.dtype, self.device = k.dtype, k.device
+        self._desc = _cabi.Kv8Desc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
+                                   status.data_ptr(), self.batch, self.kv_heads, self.capacity, _FORMATS[k.dtype])
         self._ref = ctypes.byref(self._desc)
+
+    def _smaller(self, capacity: int):
+        """An empty cache like this one; it reports into this one's status."""
+        b, h, cap = self.batch, self.kv_heads, (capacity + BLOCK - 1) // BLOCK * BLOCK
+        new = KV8Cache.__new__(KV8Cache)
+        new._set(self.k.new_empty((b, h, cap, HEAD_DIM)), self.k.new_empty((b, h, cap, HEAD_DIM)),
+                 self.k_scale.new_empty((b, h, cap // BLOCK)), self.k_scale.new_empty((b, h, cap // BLOCK)),
+                 torch.empty_like(self.k_tail), torch.empty_like(self.k_tail), self.status)
+        return new
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, dtype=torch.float8_e4m3fn, device="cuda"):
@@ -121,10 +144,6 @@ def _strides(t: torch.Tensor):
     return _I64x3(*t.stride()[:3])
 
 
-def _stream(cache: KV8Cache) -> int:
-    return torch.cuda.current_stream(cache.device).cuda_stream
-
-
 def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
     """Append tokens ``key, value [B, Hkv, n, 128]`` (bf16) behind the ``start`` tokens each sequence holds (an int or an
     int32 tensor ``[B]``); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
@@ -139,9 +158,7 @@ def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, co
             _fail("counts must be an int32 tensor")
         dev_counts, _ = _per_sequence(cache, counts, "counts", 0, n)
     dev_start, start = _per_sequence(cache, start, "start", 0, cache.capacity - (n if counts is None else 0))
-    with _on_device(cache):
-        _cabi.check(_cabi.lib().minf_kv8_store(cache._ref, key.data_ptr(), value.data_ptr(), _strides(key), _strides(value),
-                                               n, dev_start, start, dev_counts, _stream(cache)))
+    _launch("minf_kv8_store", cache, cache._ref, key.data_ptr(), value.data_ptr(), _strides(key), _strides(value), n, dev_start, start, dev_counts)
 
 
 def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
@@ -154,11 +171,8 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    with _on_device(cache):
-        _cabi.check(_cabi.lib().minf_kv8_load(cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr(),
-                                              _stream(cache)))
+    k, v = cache.k_tail.new_empty(shape), cache.k_tail.new_empty(shape)
+    _launch("minf_kv8_load", cache, cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr())
     return k, v
 
 
@@ -202,17 +216,16 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
         if weights is None:
             _fail("add_to without weights")
         _weights_arg(add_to, "add_to", cache, longest)
-    out = torch.empty((b, hq, s, d), dtype=query.dtype, device=cache.device)
-    lse = torch.empty((b, hq, s), dtype=torch.float32, device=cache.device) if return_lse else None
+    out = query.new_empty((b, hq, s, d))
+    lse = cache.k_scale.new_empty((b, hq, s)) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
-    scratch = torch.empty(nbytes, dtype=torch.uint8, device=cache.device) if nbytes else None
-    with _on_device(cache):
-        _cabi.check(_cabi.lib().minf_kv8_attention(
-            cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _strides(out), hq, s, dev_n, n, longest,
+    scratch = cache.k_scale.new_empty(nbytes // 4) if nbytes else None      # (in words of four bytes)
+    _launch("minf_kv8_attention", cache,
+            cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _I64x3(hq * s * d, s * d, d), hq, s, dev_n, n, longest,
             d ** -0.5 if sm_scale is None else float(sm_scale), lse.data_ptr() if return_lse else None,
             weights.data_ptr() if weights is not None else None, _strides(weights) if weights is not None else None,
             add_to.data_ptr() if add_to is not None else None, _strides(add_to) if add_to is not None else None,
-            scratch.data_ptr() if nbytes else None, _stream(cache)))
+            scratch.data_ptr() if nbytes else None)
     return (out, lse) if return_lse else out
 
 
@@ -222,8 +235,8 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     [B, Hkv, >= max_length]`` (fp32, as ``kv8_attention`` sums them up) of the others; equal weights: the earlier token.
     Sequences of ``budget`` tokens or fewer are copied.
 
-    Writes into ``out`` (another cache of the same type, batch and heads; a new one with room for ``budget`` tokens if not
-    given) and returns ``(out, lengths int32 [B], weights fp32 [B, Hkv, out.capacity] -- zeros behind the last --, kept int32
+    Writes into ``out`` (another cache of the same type, batch and heads; a new one with room for ``budget`` tokens, which
+    reports into this cache's status, if not given) and returns ``(out, lengths int32 [B], weights fp32 [B, Hkv, out.capacity] -- zeros behind the last --, kept int32
     [B, Hkv, budget] -- old positions, ascending, -1 behind the last)``.  Keys keep the rotary phase they were stored
     with: the caller goes on counting positions from the full sequence."""
     budget, recent, sink = int(budget), int(recent), int(sink)
@@ -233,15 +246,12 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     dev_n, n = _per_sequence(cache, lengths, "lengths", 0, longest)
     _weights_arg(weights, "weights", cache, longest)
     if out is None:
-        out = KV8Cache.empty(cache.batch, cache.kv_heads, budget, cache.dtype, cache.device)
+        out = cache._smaller(budget)
     elif out is cache or (out.batch, out.kv_heads, out.dtype, out.device) != (cache.batch, cache.kv_heads, cache.dtype, cache.device) or out.capacity < budget:
         _fail("out must be another cache of the same batch, heads, type and device with room for the budget")
-    dev = cache.device
-    kept = torch.empty((cache.batch, cache.kv_heads, budget), dtype=torch.int32, device=dev)
-    weights_out = torch.empty((cache.batch, cache.kv_heads, out.capacity), dtype=torch.float32, device=dev)
-    lengths_out = torch.empty((cache.batch,), dtype=torch.int32, device=dev)
-    with _on_device(cache):
-        _cabi.check(_cabi.lib().minf_kv8_evict(
-            cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides(weights), budget, recent, sink,
-            kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr(), _stream(cache)))
+    kept = cache.status.new_empty((cache.batch, cache.kv_heads, budget))
+    weights_out = cache.k_scale.new_empty((cache.batch, cache.kv_heads, out.capacity))
+    lengths_out = cache.status.new_empty((cache.batch,))
+    _launch("minf_kv8_evict", cache, cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides(weights), budget, recent, sink,
+            kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr())
     return out, lengths_out, weights_out, kept
