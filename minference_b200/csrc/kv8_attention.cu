@@ -203,18 +203,26 @@ __device__ __forceinline__ long long total_units(const Kv8AttnArgs& a, bool repo
 // CTAs that get work: every warp of one a unit, as far as there are
 template <int W>
 __device__ __forceinline__ int pieces_ctas(long long units, int ctas) {
-    return (int)min((long long)ctas, (units + W - 1) / W);
+    return units >= (long long)ctas * W ? ctas : (int)((units + W - 1) / W);
+}
+// x * y / z of non-negative numbers; 64-bit division takes a few hundred cycles, so it is left to products that need it
+__device__ __forceinline__ long long mul_div(long long x, int y, long long z) {
+    const long long p = x * y;
+    return (p | z) >> 32 ? p / z : (long long)((unsigned)p / (unsigned)z);
 }
 // the CTA that has a unit
-__device__ __forceinline__ long long owner_of(long long unit, long long units, int ctas) { return ((unit + 1) * ctas - 1) / units; }
+__device__ __forceinline__ long long owner_of(long long unit, long long units, int ctas) {
+    const long long p = (unit + 1) * ctas - 1;
+    return (p | units) >> 32 ? p / units : (long long)((unsigned)p / (unsigned)units);
+}
 
 template <int W>
 __device__ __forceinline__ Place locate(const Kv8AttnArgs& a, long long at) {
     const int lane = threadIdx.x & 31;
     if (!a.lengths) {
         const int per = units_of<W>(a.length_all);
-        const int bh = (int)(at / per);
-        return {bh / a.c.heads, bh % a.c.heads, (int)(at % per), a.length_all};
+        const int bh = (int)mul_div(at, 1, per);
+        return {bh / a.c.heads, bh % a.c.heads, (int)(at - (long long)bh * per), a.length_all};
     }
     for (int b0 = 0;; b0 += 32) {
         const int n = b0 + lane < a.c.batch ? clipped_length(a, b0 + lane) : 0;
@@ -231,7 +239,8 @@ __device__ __forceinline__ Place locate(const Kv8AttnArgs& a, long long at) {
             const int nb = __shfl_sync(0xffffffffu, n, src);
             const long long rest = at - __shfl_sync(0xffffffffu, upto - mine, src);        // within the sequence's heads
             const int per = units_of<W>(nb);
-            return {b0 + src, (int)(rest / per), (int)(rest % per), nb};
+            const int head = (int)mul_div(rest, 1, per);
+            return {b0 + src, head, (int)(rest - (long long)head * per), nb};
         }
         if (b0 + 32 >= a.c.batch) return {0, 0, 0, 0};          // (not reached: `at` is below the total)
         at -= __shfl_sync(0xffffffffu, upto, 31);
@@ -264,8 +273,8 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     const long long all_units = total_units<kAttnWarps>(a, blockIdx.x == 0);
     const int ctas = pieces_ctas<kAttnWarps>(all_units, a.splits);
     if ((int)blockIdx.x >= ctas) return;
-    long long at = all_units * blockIdx.x / ctas;
-    const long long stop = all_units * (blockIdx.x + 1) / ctas;
+    long long at = mul_div(all_units, blockIdx.x, ctas);
+    const long long stop = mul_div(all_units, blockIdx.x + 1, ctas);
 #pragma unroll 1
     while (at < stop) {                             // a piece: units of one sequence and head
     const Place place = locate<kAttnWarps>(a, at);
@@ -279,6 +288,14 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     const bool whole = x_lo == 0 && x_hi == units;  // nothing to join: the output is written here
     const size_t piece = blockIdx.x + bh;           // pieces are numbered so: both grow along the units, one of them at each new piece
     at += x_hi - x_lo;
+    if (takes_tail && n % kKv8Block) {              // the tail is wanted at the end: on its way to L2 from here
+        const char* kt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.k_tail) + bh * kKv8Block * kKv8Dim);
+        const char* vt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.v_tail) + bh * kKv8Block * kKv8Dim);
+        for (int i = threadIdx.x * 128; i < kKv8Block * kKv8Dim * 2; i += kAttnThreads * 128) {
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(kt + i));
+            asm volatile("prefetch.global.L2 [%0];" ::"l"(vt + i));
+        }
+    }
     const int all_see = n - a.n_q + 1;              // tokens below this are seen by every row
 
     // The warp's own ring of three slots of 4 KB: keys of a unit, values of it, keys of its next unit, ...; two copies

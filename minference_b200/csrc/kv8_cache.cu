@@ -75,12 +75,17 @@ __device__ __forceinline__ uint2 values_to_codes(const float (&x)[8], float scal
             c[i] = (uint32_t)lo | ((uint32_t)hi << 16);
         }
     } else {
+        // x / scale rounded to an integer: by the reciprocal, which is right unless the quotient lies next to a half (its
+        // error is below 127 * 2^-22), and there by the division the definition has
+        const float inv = __fdiv_rn(1.f, scale);
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
             uint32_t w = 0;
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float q = rintf(__fdiv_rn(x[4 * i + j], scale));
+                const float y = x[4 * i + j] * inv;
+                float q = rintf(y);
+                if (fabsf(fabsf(y - q) - 0.5f) < 1e-4f) q = rintf(__fdiv_rn(x[4 * i + j], scale));
                 const int r = q != q ? 0 : (int)fminf(fmaxf(q, -127.f), 127.f);
                 w |= (uint32_t)(r & 0xff) << (8 * j);
             }
@@ -304,11 +309,21 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid
         // thread t sums bins 2046 - 2t and 2047 - 2t over the cluster: a scan over the threads runs from the largest key down
         const int bin = kSelectBins - 2 - 2 * tid;
         uint32_t x1 = 0, x0 = 0;
-#pragma unroll 1
-        for (int r = 0; r < parts; ++r) {
-            const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
-            x0 += v.x;
-            x1 += v.y;
+        if (parts == kSelectCluster) {
+            uint2 v[kSelectCluster];                        // all on their way at once
+#pragma unroll
+            for (int r = 0; r < kSelectCluster; ++r) v[r] = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
+#pragma unroll
+            for (int r = 0; r < kSelectCluster; ++r) {
+                x0 += v[r].x;
+                x1 += v[r].y;
+            }
+        } else {
+            for (int r = 0; r < parts; ++r) {
+                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
+                x0 += v.x;
+                x1 += v.y;
+            }
         }
         uint32_t scan = x0 + x1;
 #pragma unroll
@@ -393,7 +408,7 @@ struct GatherArgs {
 
 // One CTA per (block of the new cache, head, keys or values): the kept tokens' values, quantised again as a block.
 template <int FMT>
-__global__ void __launch_bounds__(kStoreThreads) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
+__global__ void __launch_bounds__(kStoreThreads, 6) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
     __shared__ float red[kStoreThreads / 32];
     const int b = blockIdx.z, h = blockIdx.y >> 1, which = blockIdx.y & 1, blk = blockIdx.x;
     const int n = kv8_length(a.lengths, a.length_all, b, a.max_length, a.src.status);
@@ -414,32 +429,64 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_gather_kernel(const __grid_
     if (blk * kKv8Block >= m) return;
     const bool complete = (blk + 1) * kKv8Block <= m;
     const int chunk = threadIdx.x & 15, row0 = threadIdx.x >> 4;
-    float x[4][8];
-    float top = 0.f;
+    // A row's eight values as they lie in the source (codes, or bf16 of the tail) and their scale: turned into numbers
+    // twice, for the maximum and for the new codes, because few registers -- many blocks on an SM -- hide the two
+    // dependent reads this kernel waits for.
+    const int whole = n / kKv8Block * kKv8Block;
+    const uint8_t* src_codes = static_cast<const uint8_t*>(which ? a.src.v : a.src.k) + bh * a.src.capacity * kKv8Dim + chunk * 8;
+    const __nv_bfloat16* src_tail = static_cast<const __nv_bfloat16*>(which ? a.src.v_tail : a.src.k_tail) + bh * (kKv8Block * kKv8Dim) + chunk * 8;
+    const float* src_scale = (which ? a.src.v_scale : a.src.k_scale) + bh * (a.src.capacity / kKv8Block);
+    uint4 raw[4];
+    float scale_in[4];
+    unsigned coded = 0;                                     // bit i: row i is codes, else bf16 (or nothing: zeros)
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         const int slot = blk * kKv8Block + row0 + 16 * i;
         const int t = slot < m ? kept[slot] : -1;
-#pragma unroll
-        for (int j = 0; j < 8; ++j) x[i][j] = 0.f;
-        if (t >= 0 && t < n) token_values<FMT>(a.src, which, bh, t, n, chunk, x[i]);
-#pragma unroll
-        for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[i][j]));
+        raw[i] = make_uint4(0u, 0u, 0u, 0u);
+        scale_in[i] = 0.f;
+        if (t >= 0 && t < whole) {
+            const uint2 c = *reinterpret_cast<const uint2*>(src_codes + (size_t)t * kKv8Dim);
+            raw[i].x = c.x;
+            raw[i].y = c.y;
+            scale_in[i] = src_scale[t / kKv8Block];
+            coded |= 1u << i;
+        } else if (t >= whole && t < n) {
+            raw[i] = *reinterpret_cast<const uint4*>(src_tail + (t - whole) * kKv8Dim);
+        }
     }
+    auto values = [&](int i, float (&x)[8]) {
+        if (coded >> i & 1u) codes_to_values<FMT>(make_uint2(raw[i].x, raw[i].y), scale_in[i], x);
+        else bf16x8_to_values(raw[i], x);
+    };
     if (complete) {
+        float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            float x[8];
+            values(i, x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+        }
         top = block_max<kStoreThreads>(top, red);
         const float scale = scale_of<FMT>(top);
         uint8_t* codes = static_cast<uint8_t*>(which ? a.dst.v : a.dst.k) + (bh * a.dst.capacity + (size_t)blk * kKv8Block) * kKv8Dim;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint2*>(codes + (row0 + 16 * i) * kKv8Dim + chunk * 8) = values_to_codes<FMT>(x[i], scale);
+        for (int i = 0; i < 4; ++i) {
+            float x[8];
+            values(i, x);
+            *reinterpret_cast<uint2*>(codes + (row0 + 16 * i) * kKv8Dim + chunk * 8) = values_to_codes<FMT>(x, scale);
+        }
         if (threadIdx.x == 0) (which ? a.dst.v_scale : a.dst.k_scale)[bh * (a.dst.capacity / kKv8Block) + blk] = scale;
     } else {
         __nv_bfloat16* tail = static_cast<__nv_bfloat16*>(which ? a.dst.v_tail : a.dst.k_tail) + bh * (kKv8Block * kKv8Dim);
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (blk * kKv8Block + row0 + 16 * i < m)
-                *reinterpret_cast<uint4*>(tail + (row0 + 16 * i) * kKv8Dim + chunk * 8) = pack_bf16x8(x[i]);
+            if (blk * kKv8Block + row0 + 16 * i < m) {
+                float x[8];
+                values(i, x);
+                *reinterpret_cast<uint4*>(tail + (row0 + 16 * i) * kKv8Dim + chunk * 8) = pack_bf16x8(x);
+            }
     }
 }
 
