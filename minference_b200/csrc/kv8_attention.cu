@@ -42,6 +42,15 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], uint32_t a0, uint32_t a1
         : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
         : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
+// Codes are read once a call: they leave L2 before the logits and partial results that the second kernel reads.
+__device__ __forceinline__ uint64_t stream_policy() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void cp_async_16_stream(uint32_t dst, const void* src, uint64_t policy) {
+    asm volatile("cp.async.cg.shared.global.L2::cache_hint [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "l"(policy) : "memory");
+}
 __device__ __forceinline__ uint32_t transpose8x8(uint32_t x) {
     uint32_t y;
     asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
@@ -303,11 +312,12 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     unsigned char* const ring = ring_all + warp * (kRingSlots * kSlotBytes);
     const uint32_t ring_u = smem_u32(ring);
     const uint32_t put0 = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4), put1 = (lane >> 3) * 128 + (((lane & 7) ^ ((lane >> 3) + 4)) << 4);
+    const uint64_t stream = stream_policy();
     auto fetch = [&](int slot, const uint8_t* src) {
         src += lane * 16;
         const uint32_t dst = ring_u + slot * kSlotBytes;
 #pragma unroll
-        for (int i = 0; i < kSlotBytes / 512; ++i) cp_async_16(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i);
+        for (int i = 0; i < kSlotBytes / 512; ++i) cp_async_16_stream(dst + 512 * i + ((i & 1) ? put1 : put0), src + 512 * i, stream);
     };
     const float* ks = a.c.k_scale + bh * (a.c.capacity / kKv8Block);
     const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
@@ -653,21 +663,50 @@ __device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r
 constexpr int kFinishThreads = 256;
 constexpr int kFinishTokens = 1024;                 // tokens of a CTA that sums weights
 
-// weights of tokens [t0, t0 + kFinishTokens) of a head: the probabilities of its rows, summed in their order
+// Weights of tokens [t0, t0 + kFinishTokens) of a head: the probabilities of its rows, summed in their order.  A thread has
+// four tokens, whose logits it reads together.
+__device__ __forceinline__ float weight_of(float logit, float lse) { return logit == -CUDART_INF_F ? 0.f : fast_exp2(logit - lse); }
 __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, int n, int t0, const float* row_lse) {
+    constexpr int kEach = kFinishTokens / kFinishThreads;
     const size_t bh = (size_t)b * a.c.heads + h;
-    for (int t = t0 + threadIdx.x; t < min(n, t0 + kFinishTokens); t += kFinishThreads) {
-        const float* x = a.logits + ((long long)bh * a.tokens + t) * a.pitch;
-        const float was = a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f;
-        float sum = 0.f;
-#pragma unroll 4
-        for (int r = 0; r < a.rows; r += 2) {
-            const float2 l = *reinterpret_cast<const float2*>(x + r);
-            sum += l.x == -CUDART_INF_F ? 0.f : exp2f(l.x - row_lse[r]);
-            if (r + 1 < a.rows) sum += l.y == -CUDART_INF_F ? 0.f : exp2f(l.y - row_lse[r + 1]);
-        }
-        a.weights[b * a.ws[0] + h * a.ws[1] + t] = was + sum;
+    const float* x = a.logits + ((long long)bh * a.tokens + t0 + threadIdx.x) * a.pitch;
+    const float* add = a.add_to ? a.add_to + b * a.as[0] + h * a.as[1] + t0 + threadIdx.x : nullptr;
+    const int left = n - t0 - (int)threadIdx.x;     // token k of this thread: k * kFinishThreads < left
+    float was[kEach], sum[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) {
+        was[k] = add && k * kFinishThreads < left ? add[k * kFinishThreads] : 0.f;
+        sum[k] = 0.f;
     }
+    int r = 0;
+    for (; r + 4 <= a.pitch; r += 4) {              // (a pitch of 2, or a multiple of 4)
+        float4 l[kEach];
+#pragma unroll
+        for (int k = 0; k < kEach; ++k)
+            l[k] = k * kFinishThreads < left ? *reinterpret_cast<const float4*>(x + (long long)k * kFinishThreads * a.pitch + r)
+                                             : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
+        const float e0 = row_lse[r], e1 = r + 1 < a.rows ? row_lse[r + 1] : 0.f, e2 = r + 2 < a.rows ? row_lse[r + 2] : 0.f, e3 = r + 3 < a.rows ? row_lse[r + 3] : 0.f;
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            sum[k] += weight_of(l[k].x, e0);
+            if (r + 1 < a.rows) sum[k] += weight_of(l[k].y, e1);
+            if (r + 2 < a.rows) sum[k] += weight_of(l[k].z, e2);
+            if (r + 3 < a.rows) sum[k] += weight_of(l[k].w, e3);
+        }
+    }
+    if (a.pitch == 2) {
+#pragma unroll
+        for (int k = 0; k < kEach; ++k) {
+            if (k * kFinishThreads >= left) continue;
+            const float2 l = *reinterpret_cast<const float2*>(x + k * kFinishThreads * 2);
+            sum[k] += weight_of(l.x, row_lse[0]);
+            if (a.rows > 1) sum[k] += weight_of(l.y, row_lse[1]);
+        }
+    }
+    float* w = a.weights + b * a.ws[0] + h * a.ws[1] + t0 + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < kEach; ++k)
+        if (k * kFinishThreads < left) w[k * kFinishThreads] = was[k] + sum[k];
 }
 
 // The first CTAs join the parts of one row each: eight warps take every eighth part, a lane four dims.  The others (narrow
@@ -797,7 +836,7 @@ static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_
         }
         parts = s.splits > 1 ? pairs * rows * s.splits : 0;
     }
-    s.pitch = (int)((rows + 1) / 2 * 2);
+    s.pitch = rows <= 2 ? 2 : (int)((rows + 3) / 4 * 4);
     s.tokens = max_length;
     auto up = [](size_t x) { return (x + 255) / 256 * 256; };
     size_t at = 0;
