@@ -10,6 +10,8 @@ reference makes before its per-head loop (modules/forward.py:128-132) does not e
 Prefill calls (query length == key length > 1) run the sparse path of the configured attention type; decode
 steps go to the stock scaled-dot-product function, and so does a prefill the kernels cannot serve (another
 logit scale, sliding-window layers, batch above 1, another dtype or head size) -- with a warning, once.
+With ``past_key_values=KV8HFCache(...)`` (modules/kv8_decode.py) the keys and values stay in an 8-bit cache and decoding
+steps run this library's attention over it.
 """
 from __future__ import annotations
 
@@ -17,6 +19,7 @@ import torch
 
 import warnings
 
+from ._cabi import MInferB200Error
 from .modules.flexprefill import flexprefill_forward
 from .modules.minference_forward import minference_prefill_forward, static_prefill_forward
 from .modules.tri_mix import tri_mix_forward, tri_mix_minference_forward
@@ -62,6 +65,18 @@ def _make_attention_function(config):
     attn_kwargs = config.attn_kwargs
 
     def minference_attention(module, query, key, value, attention_mask=None, dropout=0.0, scaling=None, **kwargs):
+        kv8 = getattr(key, "minf_kv8", None)         # the 8-bit cache that holds this layer's tokens, these included
+        if kv8 is not None:
+            if kv8.seen > query.shape[2]:
+                if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None:
+                    raise MInferB200Error("sliding-window or soft-capped layers cannot attend over an 8-bit cache")
+                return kv8.attend(query, scaling).transpose(1, 2), None
+            out = prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs)
+            kv8.after_prompt(query, key)
+            return out
+        return prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs)
+
+    def prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs):
         from transformers.integrations.sdpa_attention import sdpa_attention_forward
 
         why = _sparse_path_refusal(query, key, scaling, kwargs)

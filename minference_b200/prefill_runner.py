@@ -9,7 +9,7 @@ rotary embedding in the half-rotation convention, grouped-query attention, SwiGL
 
 Dense projections and the MLP are library GEMMs (``torch.matmul``); attention of every layer goes
 through ``minference_prefill_forward`` with the per-head pattern table, exactly as the patched model
-would call it.  Under a process group the prompt is sequence-sharded in zigzag chunks: the dense
+would call it.  The prompt's keys and values may be kept in 8-bit caches, from which ``decode`` and ``generate`` go on.  Under a process group the prompt is sequence-sharded in zigzag chunks: the dense
 parts are token-parallel and need no exchange, attention runs as the vertical-slash ring.
 """
 from __future__ import annotations
@@ -68,13 +68,14 @@ class LlamaPrefill:
 
     @torch.no_grad()
     def prefill(self, ids: torch.Tensor, attn_forward_config: dict, chunk: int = 16384,
-                positions: torch.Tensor | None = None, attention=None, timing: dict | None = None) -> torch.Tensor:
+                positions: torch.Tensor | None = None, attention=None, timing: dict | None = None, kv: list | None = None) -> torch.Tensor:
         """``ids [N]`` (this rank's tokens) -> fp32 logits ``[vocab]`` of the last local token.
 
         ``positions [N]`` are the tokens' positions in the whole prompt (default 0..N-1).
         ``attention(q, k, v, layer_idx)`` replaces the single-GPU operator (the ring passes one).
         ``timing``: a dict that receives CUDA-event pairs, ``"gemm"`` around every projection / MLP product and
         ``"attention"`` around every layer's attention (see ``split_times``).
+        ``kv``: one ``KV8Layer`` per layer (``new_kv``), which keep the prompt's keys and values for ``decode``.
         """
         s = self.shape
         n = ids.numel()
@@ -116,6 +117,10 @@ class LlamaPrefill:
                 o = timed("attention", lambda: minference_prefill_forward(
                     q, k, v, {"attention_mask": None, "layer_idx": li, "num_hidden_layers": s.layers,
                               "attn_forward_config": attn_forward_config}))
+            if kv is not None:
+                kv[li].reset()
+                kv[li].append(k, v)
+                kv[li].after_prompt(q, k)
             for c0 in range(0, n, chunk):
                 c1 = min(c0 + chunk, n)
                 o_rows = o[0, :, c0:c1].transpose(0, 1).reshape(c1 - c0, nq)
@@ -126,6 +131,42 @@ class LlamaPrefill:
                 x[c0:c1] += timed("gemm", lambda: act @ L["w_down"])
             del o
         return (self._rms(x[-1:], self.final_norm) @ self.lm_head)[0].float()
+
+    def new_kv(self, **options) -> list:
+        """An 8-bit cache per layer for ``prefill(kv=...)`` and ``decode``; options as in ``KV8Layer``."""
+        from .modules.kv8_decode import KV8Layer
+
+        return [KV8Layer(**options) for _ in self.layers]
+
+    @torch.no_grad()
+    def decode(self, ids: torch.Tensor, kv: list) -> torch.Tensor:
+        """Logits (fp32 ``[S, vocab]``) behind each of the new tokens ``ids [S]``, which follow the tokens ``kv`` has seen and
+        are added to it: a decoding step (S = 1), proposed tokens to check, or a follow-up prompt."""
+        s = self.shape
+        n, nq, nk = ids.numel(), s.q_heads * s.head_dim, s.kv_heads * s.head_dim
+        cos, sin = rope_cos_sin(n, s.head_dim, s.rope_theta, self.device, start=kv[0].seen)
+        cos, sin = cos[:, None, :], sin[:, None, :]
+        x = self.embed[ids.to(self.device)]
+        for L, layer_kv in zip(self.layers, kv):
+            qkv = self._rms(x, L["attn_norm"]) @ L["wqkv"]
+            q = apply_rope(qkv[:, :nq].view(n, s.q_heads, s.head_dim).float(), cos, sin).to(self.dtype).transpose(0, 1)[None]
+            k = apply_rope(qkv[:, nq:nq + nk].view(n, s.kv_heads, s.head_dim).float(), cos, sin).to(self.dtype).transpose(0, 1)[None]
+            v = qkv[:, nq + nk:].view(n, s.kv_heads, s.head_dim).transpose(0, 1)[None]
+            layer_kv.append(k, v)
+            x = x + layer_kv.attend(q)[0].transpose(0, 1).reshape(n, nq) @ L["wo"]
+            gu = self._rms(x, L["mlp_norm"]) @ L["w_gate_up"]
+            x = x + (torch.nn.functional.silu(gu[:, :s.ffn]) * gu[:, s.ffn:]) @ L["w_down"]
+        return (self._rms(x, self.final_norm) @ self.lm_head).float()
+
+    def generate(self, ids: torch.Tensor, new_tokens: int, attn_forward_config: dict, kv: list | None = None, **options) -> torch.Tensor:
+        """``new_tokens`` greedy tokens behind the prompt ``ids [N]``: sparse prefill, then decoding over 8-bit caches."""
+        kv = self.new_kv(**options) if kv is None else kv
+        nxt = self.prefill(ids, attn_forward_config, kv=kv).argmax()[None]
+        out = [nxt]
+        for _ in range(new_tokens - 1):
+            nxt = self.decode(nxt, kv)[-1].argmax()[None]
+            out.append(nxt)
+        return torch.cat(out)
 
 
 def split_times(timing: dict, total_ms: float, layers: int) -> dict:

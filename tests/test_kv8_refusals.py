@@ -88,3 +88,20 @@ def test_no_cpu_path(cabi):
 
     with pytest.raises(cabi.MInferB200Error):
         KV8Cache.empty(1, 1, 64, device="cpu")
+
+
+def test_decode_layer_refusals(cabi):
+    from minference_b200 import KV8HFCache, KV8Layer
+
+    for kw in (dict(budget=0), dict(budget=8, recent=6, sink=4), dict(budget=8, sink=-1), dict(budget=8, slack=0)):
+        with pytest.raises(cabi.MInferB200Error):
+            KV8Layer(**kw)
+        with pytest.raises(cabi.MInferB200Error):
+            KV8HFCache(**kw)
+    past = KV8HFCache()
+    two = torch.zeros(2, 1, 4, 128, dtype=torch.bfloat16)
+    with pytest.raises(cabi.MInferB200Error, match="one sequence"):
+        past.update(two, two, 0)
+    with pytest.raises(cabi.MInferB200Error):
+        past.update(two[:1], two[:1], 0)                    # CPU tensors
+    assert past.get_seq_length() == 0
