@@ -2,17 +2,17 @@
 // the splitting of kv8_attention.cu, on the tcgen05 tensor cores.
 //
 // One CTA owns 128 rows of a head and a stretch of its tokens, in tiles of 128.  Warp roles:
-//   warps 0-3, 4-7       softmax: two threads per row, one for each block of 64 tokens of the tile (each block has its own
-//                        scales); the threads of a row exchange their maxima through shared memory, everything else is
-//                        their own, and P of the first block is on the tensor cores while the second is computed
-//   warps 8-11, 12-15    turn codes into f16 operands, one team the keys', one the values': cp.async into two 16 KB tiles,
+//   warps 0-3, 4-7       softmax of the even / odd tiles, a thread per row.  Each group keeps its own maximum, sum and output
+//                        (O and S in TMEM, P written over S as f16), so that the loads and exchanges of one tile run under
+//                        the exponentials of the other; the two results are joined at the end
+//   warps 8-10, 11-13    turn codes into f16 operands, one team the keys', one the values': cp.async into two 16 KB tiles,
 //                        the next one in flight while one is converted into the team's two 128-byte-swizzled stages.  A
 //                        thread converts what it copied itself, so the copies need no barrier
-//   warp 16              issues the MMAs
-// (Five warps share a scheduler at most, so a thread may hold 96 registers: a row's 128 logits in one thread would not fit,
-// and read from TMEM twice in small pieces they took 3700 cycles a tile.)
-// TMEM: O, two tiles of S (P is written over S as f16) and Q, 128 + 2 x 128 + 64 columns.  The products of tile i + 1 run
-// under the softmax of tile i.
+//   warp 14              issues the MMAs
+// (Four warps share a scheduler at most, so a thread may hold 128 registers: half a row of S.)  Built and measured as well:
+// two threads a row and one group (3070 cycles a tile, all of it one chain), conversion by one team of four warps (its
+// 2200 cycles a tile bound the rest).
+// TMEM: O and S of the two groups, 4 x 128 columns.
 //
 // The tail's bf16 values become f16 by a power of two for the block (what is lost lies 2^-33 below its largest value).
 // In tiles that some row does not see to its end, values that are infinite or NaN are left out of the product (zero
@@ -32,15 +32,14 @@ constexpr int kWideTile = 128;                      // tokens of a tile
 constexpr uint32_t kOperand = 128 * 256;            // 128 rows x 128 f16
 constexpr uint32_t kRawTile = 128 * 128;            // codes of a tile
 constexpr int kRawSlots = 2;                        // per team
-constexpr uint32_t kWKOff = 0, kWVOff = 2 * kOperand, kWRawOff = 4 * kOperand;
+constexpr uint32_t kWQOff = 0, kWKOff = kOperand, kWVOff = 3 * kOperand, kWRawOff = 5 * kOperand;
 constexpr uint32_t kWCtlOff = kWRawOff + 2 * kRawSlots * kRawTile;
-constexpr int kConvWarps = 4, kMmaWarp = 8 + 2 * kConvWarps;
+constexpr int kConvWarps = 3, kMmaWarp = 8 + 2 * kConvWarps;
 constexpr int kWideThreads = (kMmaWarp + 1) * 32;
 constexpr int kConvThreads = kConvWarps * 32;
-constexpr int kConvParts = kRawTile / (16 * kConvThreads);    // 16-byte pieces of a tile a thread converts
-
-// TMEM columns
-constexpr uint32_t kTmO = 0, kTmS = 128, kTmQ = 384;        // S of tile i at kTmS + 128 (i & 1)
+constexpr int kRowHop = kConvThreads / 8;                      // rows that a team takes at a time
+constexpr int kConvParts = (128 + kRowHop - 1) / kRowHop;      // 16-byte pieces of a tile a thread converts (the last one: some threads)
+static_assert(kRowHop % 4 == 0 && kRowHop % 8 != 0, "rows kRowHop apart differ in bit 2 of r & 7");
 
 struct WideCtl {
     unsigned long long k_full[2], k_empty[2], v_full[2], v_empty[2], s_full[2], p_half[2][2], tail_ready, o_done;
@@ -50,8 +49,7 @@ struct WideCtl {
     float tail_scale[2];            // of the tail's keys and values
     float red[2][kConvWarps];
     float unit[kWideRows];          // power of two a query row was divided by
-    float top[2][2][kWideRows];     // maxima of a tile's two blocks, alternating tiles
-    float sum[2][kWideRows];        // the blocks' parts of the denominator
+    float lse[kWideRows];
 };
 static_assert(kWCtlOff + sizeof(WideCtl) <= 232448, "shared memory of one CTA");
 
@@ -110,8 +108,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             mbar_init(bar(&ctl->k_empty[s]), 1);
             mbar_init(bar(&ctl->v_empty[s]), 1);
             mbar_init(bar(&ctl->s_full[s]), 1);
-            mbar_init(bar(&ctl->p_half[s][0]), 4);      // the block's warps
-            mbar_init(bar(&ctl->p_half[s][1]), 4);
+            mbar_init(bar(&ctl->p_half[s][0]), 128);    // the rows' threads
+            mbar_init(bar(&ctl->p_half[s][1]), 128);
         }
         mbar_init(bar(&ctl->tail_ready), 2 * kConvWarps);
         mbar_init(bar(&ctl->o_done), 1);
@@ -123,17 +121,17 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         tmem_alloc(smem_u32(&ctl->tmem_base), 512);
         tmem_relinquish();
     }
-    __syncthreads();
-    const uint32_t tmem = ctl->tmem_base;
-    if (warp < 4) {                                 // the query rows, a thread each, into TMEM
+    if (warp < 4) {                                 // the query rows, a thread each
         const int r = row0 + threadIdx.x;
-        const uint32_t t_q = tmem + kTmQ + ((uint32_t)(32 * warp) << 16);
         const uint4* q = r < a.rows ? reinterpret_cast<const uint4*>(a.q + b * a.qs[0] + (long long)(h * a.group + r / a.n_q) * a.qs[1] + (long long)(r % a.n_q) * a.qs[2]) : nullptr;
+        uint4 x[16];
         float top = 0.f;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) x[i] = q ? q[i] : make_uint4(0u, 0u, 0u, 0u);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float v[8];
-            bf16x8_to_values(q ? q[i] : make_uint4(0u, 0u, 0u, 0u), v);
+            bf16x8_to_values(x[i], v);
 #pragma unroll
             for (int k = 0; k < 8; ++k) {
                 const float m = fabsf(v[k]);
@@ -146,22 +144,18 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         const float inv = a.scale_log2 < 0.f ? -exp2f((float)-e) : exp2f((float)-e);
         ctl->unit[threadIdx.x] = exp2f((float)e);
 #pragma unroll
-        for (int c = 0; c < 4; ++c) {               // 32 dims, read again (from L1) rather than kept
-            uint32_t x[16];
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                float v[8];
-                bf16x8_to_values(q ? q[4 * c + i] : make_uint4(0u, 0u, 0u, 0u), v);
-#pragma unroll
-                for (int k = 0; k < 4; ++k) x[4 * i + k] = pack_half2_rn(v[2 * k] * inv, v[2 * k + 1] * inv);
-            }
-            tmem_st16(t_q + 16 * c, x);
+        for (int i = 0; i < 16; ++i) {
+            float v[8];
+            bf16x8_to_values(x[i], v);
+            st_shared_16(smem_base + kWQOff + operand_at(threadIdx.x, i), pack_half2_rn(v[0] * inv, v[1] * inv), pack_half2_rn(v[2] * inv, v[3] * inv),
+                         pack_half2_rn(v[4] * inv, v[5] * inv), pack_half2_rn(v[6] * inv, v[7] * inv));
         }
-        tmem_wait_st();
+        fence_proxy_async_smem();
     }
     tc_fence_before();
     __syncthreads();
     tc_fence_after();
+    const uint32_t tmem = ctl->tmem_base;
 
     float m_ref = -CUDART_INF_F, l_sum = 0.f;       // of a softmax thread's row
     bool ok = true;
@@ -174,11 +168,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             ok = ok && wait(&ctl->k_full[i & 1], (i >> 1) & 1);
             if (!ok) return;
             constexpr uint32_t idesc = umma_idesc(128, 128, false, false, false);
-            const uint32_t d = tmem + kTmS + (i & 1) * 128;
-            const uint32_t k_lo = ((smem_base + kWKOff + (i & 1) * kOperand) >> 4) | (1u << 16);
+            const uint32_t d = tmem + (i & 1) * 256 + 128;
+            const uint32_t q_lo = ((smem_base + kWQOff) >> 4) | (1u << 16), k_lo = ((smem_base + kWKOff + (i & 1) * kOperand) >> 4) | (1u << 16);
             if (elect_one()) {
 #pragma unroll
-                for (int kk = 0; kk < 8; ++kk) umma_ts(d, tmem + kTmQ + kk * 8, desc(k_lo + (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4)), idesc, kk > 0);
+                for (int kk = 0; kk < 8; ++kk) {
+                    const uint32_t adv = (kk >> 2) * (16384 >> 4) + (kk & 3) * (32 >> 4);
+                    umma_ss(d, desc(q_lo + adv), desc(k_lo + adv), idesc, kk > 0);
+                }
                 umma_commit(bar(&ctl->s_full[i & 1]));
                 umma_commit(bar(&ctl->k_empty[i & 1]));
             }
@@ -186,7 +183,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         auto issue_pv = [&](int i) {
             ok = ok && wait(&ctl->v_full[i & 1], (i >> 1) & 1);
             constexpr uint32_t idesc = umma_idesc(128, 128, false, false, true);
-            const uint32_t d = tmem + kTmO, p = tmem + kTmS + (i & 1) * 128;
+            const uint32_t d = tmem + (i & 1) * 256, p = d + 128;
             const uint32_t v_lo = ((smem_base + kWVOff + (i & 1) * kOperand) >> 4) | ((16384u >> 4) << 16);
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
@@ -196,7 +193,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                 if (elect_one()) {
 #pragma unroll
                     for (int kk = 4 * half; kk < 4 * half + 4; ++kk)
-                        umma_ts(d, p + kk * 8, desc(v_lo + kk * (2048 >> 4)), idesc, (i > 0 || kk > 0) ? 1u : 0u);
+                        umma_ts(d, p + kk * 8, desc(v_lo + kk * (2048 >> 4)), idesc, (i > 1 || kk > 0) ? 1u : 0u);
                     if (half) umma_commit(bar(&ctl->v_empty[i & 1]));
                 }
             }
@@ -213,10 +210,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         }
     } else if (warp >= 8) {
         // ---------------------------------------------------------------------------------------- conversion
-        const int which = warp >= 8 + kConvWarps, dw = warp & 3, tid = threadIdx.x & (kConvThreads - 1);
+        const int which = warp >= 8 + kConvWarps, dw = (warp - 8) % kConvWarps, tid = threadIdx.x - 256 - which * kConvThreads;
         const uint8_t* codes = static_cast<const uint8_t*>(which ? a.c.v : a.c.k) + bh * a.c.capacity * kKv8Dim;
         const __nv_bfloat16* tail = static_cast<const __nv_bfloat16*>(which ? a.c.v_tail : a.c.k_tail) + bh * kKv8Block * kKv8Dim;
-        constexpr int kRowHop = kConvThreads / 8, kPartBytes = kConvThreads * 16;
+        constexpr int kPartBytes = kConvThreads * 16;
         // Rows row + kRowHop u, 16 codes from 16 ch.  Eight neighbouring lanes have chunks 0-3 of a row and 4-7 of its
         // neighbour: so their operand chunks lie in different banks (the upper 64 dims lie 16 KB behind the lower).
         const int quad = (tid >> 2) & 3;
@@ -229,15 +226,10 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                 const int t0 = (j_lo + i) * kWideTile;
                 const uint8_t* src = codes + (size_t)t0 * kKv8Dim + mine;
                 const uint32_t dst = raw + (i & 1) * kRawTile;
-                const int rows = full * kKv8Block - t0 - row;           // rows of complete blocks from this thread's on
-                if (rows > kRowHop * (kConvParts - 1)) {
+                const int rows = min(full * kKv8Block - t0, kWideTile) - row;       // rows of complete blocks from this thread's on
 #pragma unroll
-                    for (int u = 0; u < kConvParts; ++u) cp_async_16(dst + u * kPartBytes, src + u * kPartBytes);
-                } else {
-#pragma unroll 1
-                    for (int u = 0; u < kConvParts; ++u)
-                        if (kRowHop * u < rows) cp_async_16(dst + u * kPartBytes, src + u * kPartBytes);
-                }
+                for (int u = 0; u < kConvParts; ++u)
+                    if (kRowHop * u < rows) cp_async_16(dst + u * kPartBytes, src + u * kPartBytes);
             }
             cp_async_commit();
         };
@@ -245,9 +237,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         fetch(1);
         if (has_tail) {                             // the tail's scale, before its tile is due
             float top = 0.f;
-#pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int r = (tid >> 4) + 8 * u;
+#pragma unroll 4
+            for (int r = tid >> 4; r < kKv8Block; r += kConvThreads / 16) {
                 if (full * kKv8Block + r < n) {
                     float v[8];
                     bf16x8_to_values(*reinterpret_cast<const uint4*>(tail + r * kKv8Dim + (tid & 15) * 8), v);
@@ -279,18 +270,22 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             const uint32_t src = raw + (i & 1) * kRawTile, dst = smem_base + (which ? kWVOff : kWKOff) + (i & 1) * kOperand;
             uint4 c[kConvParts];
 #pragma unroll
-            for (int u = 0; u < kConvParts; ++u) c[u] = ld_shared_16(src + u * kPartBytes);
+            for (int u = 0; u < kConvParts; ++u)
+                c[u] = u < kConvParts - 1 || row + kRowHop * u < kWideTile ? ld_shared_16(src + u * kPartBytes) : make_uint4(0u, 0u, 0u, 0u);
             if (i >= 2) {
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(&empty_bar[i & 1]), ((i >> 1) - 1) & 1, abort_flag));
                 if (!ok) break;
             }
             const bool masked = t0 + kWideTile > all_see;
             bool bad = false;
+            // rows kRowHop apart differ in bit 2 of r & 7, which the chunks' places are xored with: 64 bytes on or back
             const uint32_t d0 = dst + operand_at(row, 2 * ch), d1 = dst + operand_at(row, 2 * ch + 1);
-            auto put = [&](int u, const uint32_t (&x)[8]) {             // (rows kRowHop apart: the same row & 7)
-                const uint32_t at = u * kRowHop * 128;
-                st_shared_16(d0 + at, x[0], x[1], x[2], x[3]);
-                st_shared_16(d1 + at, x[4], x[5], x[6], x[7]);
+            auto put = [&](int u, const uint32_t (&x)[8]) {
+                const uint32_t at = u * kRowHop * 128, flip = (u & 1) * 64;
+                if (u < kConvParts - 1 || row + kRowHop * u < kWideTile) {
+                    st_shared_16((d0 ^ flip) + at, x[0], x[1], x[2], x[3]);
+                    st_shared_16((d1 ^ flip) + at, x[4], x[5], x[6], x[7]);
+                }
             };
             auto halves = [&](const uint4& w, uint32_t (&x)[8]) {
                 codes_to_half<FMT>(w.x, x[0], x[1]);
@@ -298,15 +293,15 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                 codes_to_half<FMT>(w.z, x[4], x[5]);
                 codes_to_half<FMT>(w.w, x[6], x[7]);
             };
-            // Shared memory is read in order: once the last piece is used, all are in registers, and the next tile but one may be
-            // copied over them.
+            // Shared memory is read in order: once the last pieces are used, all are in registers, and the next tile but one may
+            // be copied over them.
             if (!masked && t0 + kWideTile <= full * kKv8Block) {
 #pragma unroll
                 for (int u = kConvParts - 1; u >= 0; --u) {
                     uint32_t x[8];
                     halves(c[u], x);
                     put(u, x);
-                    if (u == kConvParts - 1) fetch(i + 2);
+                    if (u == kConvParts - 2) fetch(i + 2);
                 }
             } else {
 #pragma unroll
@@ -327,8 +322,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             if (has_tail && i == count - 1) {
                 const float inv = __fdiv_rn(1.f, ctl->tail_scale[which]);
 #pragma unroll 1
-                for (int u = 0; u < 8; ++u) {               // (unrolled once: the last tile only)
-                    const int r = (tid >> 4) + 8 * u, c16 = tid & 15;
+                for (int r = tid >> 4; r < kKv8Block; r += kConvThreads / 16) {
+                    const int c16 = tid & 15;
                     uint32_t x[4] = {0u, 0u, 0u, 0u};
                     if (full * kKv8Block + r < n) {
                         float v[8];
@@ -350,9 +345,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         cp_async_wait<0>();
     } else {
         // ------------------------------------------------------------------------------------------- softmax
-        const int half = warp >> 2, r = threadIdx.x & 127, gr = row0 + r;
-        const uint32_t lanes = (uint32_t)(32 * (warp & 3)) << 16;
-        const uint32_t t_o = tmem + kTmO + 64 * half + lanes;
+        const int grp = warp >> 2, r = threadIdx.x & 127, gr = row0 + r;
+        const uint32_t t_o = tmem + grp * 256 + ((uint32_t)(32 * (warp & 3)) << 16), t_s = t_o + 128;
         const bool live = gr < a.rows;
         const int lim = live ? all_see + gr % a.n_q : 0x7fffffff;      // (rows behind the last: anything, they are dropped)
         const float mul = fabsf(a.scale_log2) * ctl->unit[r];
@@ -360,75 +354,85 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         const float* vs = a.c.v_scale + bh * (a.c.capacity / kKv8Block);
         float* logits = LOGITS && live ? a.logits + (long long)bh * a.tokens * a.pitch + gr : nullptr;
         const bool warp_live = row0 + 32 * (warp & 3) < a.rows;         // rows behind the last: P of zeros, nothing else
-        float next_k = 1.f, next_v = 1.f;
-        auto scales = [&](int i) {                  // of this thread's block, read a tile ahead
-            const int blk = (j_lo + i) * 2 + half;
-            if (i < count && blk < full) {
-                next_k = ks[blk];
-                next_v = vs[blk];
-            } else {
-                next_k = next_v = 1.f;
+        float next_k[2], next_v[2];
+        auto scales = [&](int i) {                  // of a tile's two blocks, read a turn ahead
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                const int blk = (j_lo + i) * 2 + x;
+                const bool there = i < count && blk < full;
+                next_k[x] = there ? ks[blk] : 1.f;
+                next_v[x] = there ? vs[blk] : 1.f;
             }
         };
-        scales(0);
-        for (int i = 0; i < count; ++i) {
-            const int t0 = (j_lo + i) * kWideTile + 64 * half;          // this thread's block
-            float f = next_k, inv_v = next_v;
-            if (t0 == full * kKv8Block && n % kKv8Block) {
+        scales(grp);
+        for (int i = grp; i < count; i += 2) {
+            const int t0 = (j_lo + i) * kWideTile;
+            float f[2] = {next_k[0], next_k[1]}, inv_v[2] = {next_v[0], next_v[1]}, lv[2];
+            if (t0 + kWideTile > full * kKv8Block && n % kKv8Block) {   // the tail is one of the blocks
                 ok = __all_sync(0xffffffffu, mbar_wait(bar(&ctl->tail_ready), 0, abort_flag));
                 if (!ok) break;
-                f = ctl->tail_scale[0];
-                inv_v = ctl->tail_scale[1];
+                const int x = full & 1;
+                f[0] = x == 0 ? ctl->tail_scale[0] : f[0];
+                f[1] = x == 1 ? ctl->tail_scale[0] : f[1];
+                inv_v[0] = x == 0 ? ctl->tail_scale[1] : inv_v[0];
+                inv_v[1] = x == 1 ? ctl->tail_scale[1] : inv_v[1];
             }
-            scales(i + 1);
-            f *= mul;
-            const float lv = log2f(inv_v);
-            inv_v = 1.f / inv_v;
-            ok = __all_sync(0xffffffffu, mbar_wait(bar(&ctl->s_full[i & 1]), (i >> 1) & 1, abort_flag));
+            scales(i + 2);
+#pragma unroll
+            for (int x = 0; x < 2; ++x) {
+                f[x] *= mul;
+                lv[x] = __log2f(inv_v[x]);
+                inv_v[x] = __fdividef(1.f, inv_v[x]);
+            }
+            ok = __all_sync(0xffffffffu, mbar_wait(bar(&ctl->s_full[grp]), (i >> 1) & 1, abort_flag));
             if (!ok) break;
             tc_fence_after();
-            if (!warp_live) {                       // (both warps of these rows)
+            if (!warp_live) {
                 uint32_t z[8];
 #pragma unroll
                 for (int k = 0; k < 8; ++k) z[k] = 0u;
 #pragma unroll 1
-                for (int c = 0; c < 4; ++c) tmem_st8(tmem + kTmS + (i & 1) * 128 + 32 * half + 8 * c + lanes, z);
+                for (int c = 0; c < 8; ++c) tmem_st8(t_s + 8 * c, z);
                 tmem_wait_st();
                 tc_fence_before();
-                __syncwarp();
-                if (lane == 0) mbar_arrive(bar(&ctl->p_half[i & 1][half]));
+                mbar_arrive(bar(&ctl->p_half[grp][0]));
+                mbar_arrive(bar(&ctl->p_half[grp][1]));
                 continue;
             }
-            const uint32_t t_s = tmem + kTmS + (i & 1) * 128 + 64 * half + lanes, t_p = tmem + kTmS + (i & 1) * 128 + 32 * half + lanes;
-            // P of the second block goes over columns 32-63 of S, which belong to the first: its warps have read them
-            // when the maxima are exchanged
-            uint32_t s[2][32];
-            tmem_ld32(t_s, s[0]);
-            tmem_ld32(t_s + 32, s[1]);
-            tmem_wait_ld();
-            const int seen = lim - t0;                                  // of this block's tokens
-            if (seen < 64) {
-#pragma unroll
-                for (int c = 0; c < 2; ++c) {
-                    const int left = seen - 32 * c;
-                    const uint32_t cm = left >= 32 ? 0xffffffffu : left <= 0 ? 0u : (1u << left) - 1u;
+            const int seen = lim - t0;              // of this tile's tokens
+            // Columns 32 c .. of S, -inf where the row does not see the token.
+            auto hide = [&](int c, uint32_t (&x)[32]) {
+                const int left = seen - 32 * c;
+                if (left < 32) {
+                    const uint32_t cm = left <= 0 ? 0u : (1u << left) - 1u;
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
-                        if (!((cm >> k) & 1u)) s[c][k] = 0xff800000u;   // -inf
+                        if (!((cm >> k) & 1u)) x[k] = 0xff800000u;
                 }
-            }
-            float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
+            };
+            auto largest = [&](const uint32_t (&x)[32]) {
+                float m4[4] = {-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F};
 #pragma unroll
-            for (int c = 0; c < 2; ++c)
-#pragma unroll
-                for (int k = 0; k < 32; k += 2) m4[(k >> 1) & 3] = max3(m4[(k >> 1) & 3], __uint_as_float(s[c][k]), __uint_as_float(s[c][k + 1]));
-            const float m = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
-            const float mine = m == -CUDART_INF_F ? m : fmaf(m, f, lv);         // (-inf times a scale of zero would be NaN)
-            ctl->top[i & 1][half][r] = mine;
-            tc_fence_before();
-            asm volatile("bar.sync %0, 64;" ::"r"(4 + (warp & 3)) : "memory");  // the row's two warps
-            tc_fence_after();
-            const float mx = fmaxf(mine, ctl->top[i & 1][half ^ 1][r]);
+                for (int k = 0; k < 32; k += 2) m4[(k >> 1) & 3] = max3(m4[(k >> 1) & 3], __uint_as_float(x[k]), __uint_as_float(x[k + 1]));
+                return fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3]));
+            };
+            // The maximum first, of the second block and then of the first, which stays in registers: its P goes over the
+            // columns it came from, and is on the tensor cores while the second block is read again.
+            uint32_t s0[32], s1[32];
+            tmem_ld32(t_s + 64, s0);
+            tmem_ld32(t_s + 96, s1);
+            tmem_wait_ld();
+            hide(2, s0);
+            float mb = largest(s0);
+            tmem_ld32(t_s, s0);
+            hide(3, s1);
+            mb = fmaxf(mb, largest(s1));
+            tmem_ld32(t_s + 32, s1);
+            tmem_wait_ld();
+            hide(0, s0);
+            hide(1, s1);
+            const float ma = fmaxf(largest(s0), largest(s1));
+            const float mx = fmaxf(ma == -CUDART_INF_F ? ma : fmaf(ma, f[0], lv[0]), mb == -CUDART_INF_F ? mb : fmaf(mb, f[1], lv[1]));   // (-inf times zero)
             float alpha = 1.f;
             if (mx > m_ref + 8.f) {                 // the reference is raised on a jump of more than 2^8: P stays far below f16's largest
                 alpha = fast_exp2(m_ref - mx);
@@ -436,13 +440,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                 m_ref = mx;
             }
             const float ref = m_ref == -CUDART_INF_F ? 0.f : m_ref;
-            if (i > 0 && __any_sync(0xffffffffu, alpha != 1.f)) {
-                // O is at rest once the last tile's product is through (and this tile's waits for the P below)
-                ok = __all_sync(0xffffffffu, mbar_wait(bar(&ctl->v_empty[(i - 1) & 1]), ((i - 1) >> 1) & 1, abort_flag));
-                if (!ok) break;
-                tc_fence_after();
+            if (i > 1 && __any_sync(0xffffffffu, alpha != 1.f)) {       // (O is at rest: this tile's S came behind its last product)
 #pragma unroll 1
-                for (int c = 0; c < 8; ++c) {
+                for (int c = 0; c < 16; ++c) {
                     uint32_t o[8];
                     tmem_ld8(t_o + 8 * c, o);
                     tmem_wait_ld();
@@ -451,48 +451,60 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                     tmem_st8(t_o + 8 * c, o);
                 }
             }
-            if (LOGITS && logits) {
-                float* to = logits + (long long)t0 * a.pitch;
-#pragma unroll
-                for (int c = 0; c < 2; ++c)
+            // P of 32 tokens of block x, columns 32 c of S; the sum of the numerators
+            auto numerators = [&](int c, int x, uint32_t (&sc)[32]) {
+                if (LOGITS && logits) {
+                    float* to = logits + (long long)(t0 + 32 * c) * a.pitch;
 #pragma unroll
                     for (int k = 0; k < 32; ++k)
-                        if (t0 + 32 * c + k < n) to[(long long)(32 * c + k) * a.pitch] = 32 * c + k < seen ? __uint_as_float(s[c][k]) * f : -CUDART_INF_F;
-            }
-            const uint64_t f2 = pack_f32x2(f, f), d2 = pack_f32x2(lv - ref, lv - ref);
-            uint64_t sum2[2] = {0ull, 0ull};
-            const bool zero = f == 0.f && seen < 64;    // (the only masked logits that the product below would not leave at -inf)
-#pragma unroll
-            for (int c = 0; c < 4; ++c) {
-                uint32_t p[8];
-#pragma unroll
-                for (int k = 0; k < 16; k += 2) {
-                    const int kk = 16 * (c & 1) + k;
-                    float x0, x1;
-                    unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(s[c >> 1][kk]), __uint_as_float(s[c >> 1][kk + 1])), f2, d2), x0, x1);
-                    x0 = fast_exp2(x0);
-                    x1 = fast_exp2(x1);
-                    if (zero) {
-                        if (16 * c + k >= seen) x0 = 0.f;
-                        if (16 * c + k + 1 >= seen) x1 = 0.f;
-                    }
-                    sum2[(k >> 1) & 1] = add_f32x2(sum2[(k >> 1) & 1], pack_f32x2(x0, x1));
-                    p[k >> 1] = pack_half2_rn(x0, x1);
+                        if (t0 + 32 * c + k < n) to[(long long)k * a.pitch] = 32 * c + k < seen ? __uint_as_float(sc[k]) * f[x] : -CUDART_INF_F;
                 }
-                tmem_st8(t_p + 8 * c, p);
-            }
-            float a0, a1;
-            unpack_f32x2(add_f32x2(sum2[0], sum2[1]), a0, a1);
-            l_sum = fmaf(a0 + a1, inv_v, l_sum);
+                const float d = lv[x] - ref;
+                const uint64_t f2 = pack_f32x2(f[x], f[x]), d2 = pack_f32x2(d, d);
+                uint64_t sum2[2] = {0ull, 0ull};
+                const bool zero = f[x] == 0.f && seen < 32 * c + 32;    // (the only masked logits the product would not leave at -inf)
+#pragma unroll
+                for (int hf = 0; hf < 2; ++hf) {
+                    uint32_t p[8];
+#pragma unroll
+                    for (int k = 0; k < 16; k += 2) {
+                        const int kk = 16 * hf + k;
+                        float x0, x1;
+                        unpack_f32x2(fma_f32x2(pack_f32x2(__uint_as_float(sc[kk]), __uint_as_float(sc[kk + 1])), f2, d2), x0, x1);
+                        x0 = fast_exp2(x0);
+                        x1 = fast_exp2(x1);
+                        if (zero) {
+                            if (32 * c + kk >= seen) x0 = 0.f;
+                            if (32 * c + kk + 1 >= seen) x1 = 0.f;
+                        }
+                        sum2[(k >> 1) & 1] = add_f32x2(sum2[(k >> 1) & 1], pack_f32x2(x0, x1));
+                        p[k >> 1] = pack_half2_rn(x0, x1);
+                    }
+                    tmem_st8(t_s + 16 * c + 8 * hf, p);
+                }
+                float a0, a1;
+                unpack_f32x2(add_f32x2(sum2[0], sum2[1]), a0, a1);
+                return a0 + a1;
+            };
+            float sum = numerators(0, 0, s0);
+            tmem_ld32(t_s + 64, s0);
+            sum += numerators(1, 0, s1);
+            l_sum = fmaf(sum, inv_v[0], l_sum);
+            tmem_wait_ld();
+            tmem_ld32(t_s + 96, s1);
             tmem_wait_st();
             tc_fence_before();
-            __syncwarp();
-            if (lane == 0) mbar_arrive(bar(&ctl->p_half[i & 1][half]));
+            mbar_arrive(bar(&ctl->p_half[grp][0]));
+            hide(2, s0);
+            sum = numerators(2, 1, s0);
+            tmem_wait_ld();
+            hide(3, s1);
+            sum += numerators(3, 1, s1);
+            l_sum = fmaf(sum, inv_v[1], l_sum);
+            tmem_wait_st();
+            tc_fence_before();
+            mbar_arrive(bar(&ctl->p_half[grp][1]));
         }
-        if (ok) ctl->sum[half][r] = l_sum;
-        // A warp that gave up a wait will not come to the exchange of the maxima: its partner, which may wait there, goes on to a
-        // wait that gives up too.
-        else asm volatile("bar.arrive %0, 64;" ::"r"(4 + (warp & 3)) : "memory");
     }
     // every wait of this kernel ends within its limit: all warps come here
     if (warp < 8) {
@@ -502,12 +514,34 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
     __syncthreads();
     if (!ctl->abort) {
         tc_fence_after();
-        if (warp < 8) {                             // each thread 64 dims of its row
-            const int half = warp >> 2, r = threadIdx.x & 127, gr = row0 + r;
-            const uint32_t t_o = tmem + kTmO + 64 * half + ((uint32_t)(32 * (warp & 3)) << 16);
-            const float sum = ctl->sum[0][r] + ctl->sum[1][r];
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            const float lse = sum == 0.f ? -CUDART_INF_F : m_ref == -CUDART_INF_F ? sum : m_ref + log2f(sum);
+        // join the two groups: the odd tiles' through shared memory (the operands are done with), a column of 128 rows at a time
+        float* other = reinterpret_cast<float*>(smem);
+        const int r = threadIdx.x & 127, grp = warp >> 2;
+        const uint32_t t_o = tmem + (grp & 1) * 256 + ((uint32_t)(32 * (warp & 3)) << 16);
+        const bool any = (grp == 0 && count > 0) || (grp == 1 && count > 1);
+        const float mine = l_sum == 0.f ? -CUDART_INF_F : (m_ref == -CUDART_INF_F ? l_sum : m_ref + log2f(l_sum));
+        if (grp == 1) {
+            ctl->lse[r] = mine;
+            const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
+#pragma unroll 1
+            for (int c = 0; c < 8; ++c) {
+                uint32_t o[16];
+                if (any) {
+                    tmem_ld16(t_o + 16 * c, o);
+                    tmem_wait_ld();
+                }
+#pragma unroll
+                for (int k = 0; k < 16; ++k) other[(16 * c + k) * kWideRows + r] = any && l_sum != 0.f ? __uint_as_float(o[k]) * inv : 0.f;
+            }
+        }
+        __syncthreads();
+        if (grp == 0) {
+            const int gr = row0 + r;
+            const float theirs = ctl->lse[r], top = fmaxf(mine, theirs);
+            const float e0 = mine == -CUDART_INF_F ? 0.f : exp2f(mine - top), e1 = theirs == -CUDART_INF_F ? 0.f : exp2f(theirs - top);
+            const float sum = e0 + e1;
+            const float w0 = e0 == 0.f ? 0.f : e0 / (sum * l_sum), w1 = e1 == 0.f ? 0.f : e1 / sum;
+            const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
             const size_t row = bh * a.rows + gr;
             const int hq = h * a.group + gr / a.n_q, t = gr % a.n_q;
             const bool live = gr < a.rows;
@@ -516,17 +550,20 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             const uint8_t* vc = static_cast<const uint8_t*>(a.c.v) + bh * a.c.capacity * kKv8Dim;
             const __nv_bfloat16* vt = static_cast<const __nv_bfloat16*>(a.c.v_tail) + bh * kKv8Block * kKv8Dim;
 #pragma unroll 1
-            for (int c = 0; c < 4; ++c) {
+            for (int c = 0; c < 8; ++c) {
                 uint32_t o[16];
-                if (count > 0) {
+                if (any) {
                     tmem_ld16(t_o + 16 * c, o);
                     tmem_wait_ld();
                 }
                 float x[16];
 #pragma unroll
-                for (int k = 0; k < 16; ++k) x[k] = count > 0 && inv != 0.f ? __uint_as_float(o[k]) * inv : 0.f;
+                for (int k = 0; k < 16; ++k) {
+                    x[k] = w1 == 0.f ? 0.f : other[(16 * c + k) * kWideRows + r] * w1;
+                    if (any && w0 != 0.f) x[k] = fmaf(__uint_as_float(o[k]), w0, x[k]);
+                }
                 if (!live) continue;
-                const int d = 64 * half + 16 * c;
+                const int d = 16 * c;
                 if (ctl->bad) {
                     for (int tt = bad_lo; tt < bad_hi; ++tt)
 #pragma unroll
@@ -547,7 +584,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                     for (int k = 0; k < 4; ++k) dst[k] = make_uint2(pack_bf16x2(x[4 * k], x[4 * k + 1]), pack_bf16x2(x[4 * k + 2], x[4 * k + 3]));
                 }
             }
-            if (live && half == 0) {
+            if (live) {
                 if (a.splits > 1) {
                     a.part_lse[row * a.splits + split] = lse;
                 } else {
