@@ -28,7 +28,9 @@ namespace minf {
 constexpr int kUnit = 32;                           // tokens a warp takes at a time: half a block
 constexpr int kSlotBytes = kUnit * kKv8Dim;         // their keys or values
 constexpr int kRingSlots = 3;
-constexpr int kNarrowRows = 32;                     // rows per cache head this kernel takes
+// Rows per cache head this kernel takes; more go to the wide one.  At 131072 tokens of 8 heads (e4m3, device time): 24 rows 76 us
+// here and 85 us there, 32 rows (a fourth group, since removed) 97 and 90; four sequences of 16384: 32 rows 78 and 57.
+constexpr int kNarrowRows = 24;
 // warps of a CTA: two CTAs fit an SM with 128 registers a thread for one group of rows, twice that for more
 __host__ __device__ constexpr int narrow_warps(int nt) { return nt == 1 ? 8 : 4; }
 
@@ -191,28 +193,40 @@ __device__ __forceinline__ int clipped_length(const Kv8AttnArgs& a, int b) {
     const int n = a.lengths ? a.lengths[b] : a.length_all;
     return max(0, min(n, a.max_length));
 }
+struct Share {
+    long long units;                // of all sequences and heads
+    int ctas;                       // that get some: every warp of one a unit, as far as there are
+};
 template <int W>
-__device__ __forceinline__ long long total_units(const Kv8AttnArgs& a, bool report) {
-    if (!a.lengths) return (long long)a.c.batch * a.c.heads * units_of<W>(a.length_all);
-    const int lane = threadIdx.x & 31;
-    long long sum = 0;
-    for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-        int x = 0;
-        if (b0 + lane < a.c.batch) {
-            const int n = clipped_length(a, b0 + lane);
-            if (report && threadIdx.x < 32 && n != a.lengths[b0 + lane]) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
-            x = units_of<W>(n);
-        }
+__device__ __forceinline__ Share share_of(const Kv8AttnArgs& a, bool report) {
+    const int pairs = a.c.batch * a.c.heads;
+    long long units = 0;
+    bool same = true;               // sequences of one length
+    if (!a.lengths) {
+        units = (long long)pairs * units_of<W>(a.length_all);
+    } else {
+        const int lane = threadIdx.x & 31, first = units_of<W>(clipped_length(a, 0));
+        for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
+            int x = 0;
+            if (b0 + lane < a.c.batch) {
+                const int n = clipped_length(a, b0 + lane);
+                if (report && threadIdx.x < 32 && n != a.lengths[b0 + lane]) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
+                x = units_of<W>(n);
+                same = same && x == first;
+            }
 #pragma unroll
-        for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        sum += x;
+            for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+            units += x;
+        }
+        same = __all_sync(0xffffffffu, same);
+        units *= a.c.heads;
     }
-    return sum * a.c.heads;
-}
-// CTAs that get work: every warp of one a unit, as far as there are
-template <int W>
-__device__ __forceinline__ int pieces_ctas(long long units, int ctas) {
-    return units >= (long long)ctas * W ? ctas : (int)((units + W - 1) / W);
+    int ctas = a.splits;
+    // a whole number of CTAs per head where that leaves few of them idle: then none works on two pieces, which costs it a new
+    // start and a second joining (about 5 us)
+    if (same && pairs <= ctas && ctas / pairs * pairs * 10 >= ctas * 9) ctas = ctas / pairs * pairs;
+    if (units < (long long)ctas * W) ctas = (int)((units + W - 1) / W);
+    return {units, ctas};
 }
 // x * y / z of non-negative numbers; 64-bit division takes a few hundred cycles, so it is left to products that need it
 __device__ __forceinline__ long long mul_div(long long x, int y, long long z) {
@@ -279,8 +293,9 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     extern __shared__ __align__(128) unsigned char ring_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     dependents_launch();
-    const long long all_units = total_units<kAttnWarps>(a, blockIdx.x == 0);
-    const int ctas = pieces_ctas<kAttnWarps>(all_units, a.splits);
+    const Share share = share_of<kAttnWarps>(a, blockIdx.x == 0);
+    const long long all_units = share.units;
+    const int ctas = share.ctas;
     if ((int)blockIdx.x >= ctas) return;
     long long at = mul_div(all_units, blockIdx.x, ctas);
     const long long stop = mul_div(all_units, blockIdx.x + 1, ctas);
@@ -650,13 +665,63 @@ __device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r
         return {(bh * a.rows + r) * a.splits, 1, a.splits};
     } else {
         const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
-        const long long all = total_units<W>(a, false);
-        const int ctas = pieces_ctas<W>(all, a.splits);
+        const Share share = share_of<W>(a, false);
+        const long long all = share.units;
+        const int ctas = share.ctas;
         const int per = units_of<W>(a.lengths ? clipped_length(a, b) : a.length_all);
         if (per == 0) return {0, 0, 0};
         const long long start = units_before<W>(a, b) + (long long)h * per;
         const long long lo = owner_of(start, all, ctas), hi = owner_of(start + per - 1, all, ctas);
         return {((size_t)lo + bh) * a.rows + r, (size_t)a.rows, (int)(hi - lo + 1)};
+    }
+}
+
+// The parts of one row joined and written: `WARPS` warps of the CTA take every WARPS-th part, a lane four dims.
+template <int WARPS>
+__device__ __forceinline__ void join_row(const Kv8AttnArgs& a, const Parts& p, size_t row, int warp, int lane, float4 (*sm)[32], float* sm_sum) {
+    float top = -CUDART_INF_F;
+    for (int k = lane; k < p.count; k += 32) top = fmaxf(top, a.part_lse[p.base + k * p.step]);
+#pragma unroll
+    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+    float sum = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 4
+    for (int k = warp; k < p.count; k += WARPS) {
+        const float e = a.part_lse[p.base + k * p.step];
+        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p.base + k * p.step) * kKv8Dim + 4 * lane);
+        const float f = e == -CUDART_INF_F ? 0.f : exp2f(e - top);     // (a part that saw nothing holds zeros)
+        sum += f;
+        acc.x = fmaf(f, x.x, acc.x);
+        acc.y = fmaf(f, x.y, acc.y);
+        acc.z = fmaf(f, x.z, acc.z);
+        acc.w = fmaf(f, x.w, acc.w);
+    }
+    if constexpr (WARPS > 1) {
+        sm[warp][lane] = acc;
+        if (lane == 0) sm_sum[warp] = sum;
+        __syncthreads();
+        if (warp) return;
+        sum = 0.f;
+        acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) {
+            const float4 x = sm[w][lane];
+            sum += sm_sum[w];
+            acc.x += x.x;
+            acc.y += x.y;
+            acc.z += x.z;
+            acc.w += x.w;
+        }
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    const int bh = (int)(row / a.rows), r = (int)(row % a.rows), b = bh / a.c.heads, h = bh % a.c.heads;
+    const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
+    __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + 4 * lane;
+    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+    if (lane == 0) {
+        const float e = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+        if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = e;
+        if (a.row_lse) a.row_lse[row] = e;
     }
 }
 
@@ -709,8 +774,8 @@ __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, 
         if (k * kFinishThreads < left) w[k * kFinishThreads] = was[k] + sum[k];
 }
 
-// The first CTAs join the parts of one row each: eight warps take every eighth part, a lane four dims.  The others (narrow
-// kernel) sum the weights, for which they join the log-sum-exps of their head's rows themselves: no second wait.
+// The first CTAs join the parts of a row each (narrow kernel: up to a few dozen parts, eight warps) or of eight rows (wide
+// kernel).  The others (narrow kernel) sum the weights, for which they join the log-sum-exps of their head's rows themselves: no second wait.
 template <int W>
 __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid_constant__ Kv8AttnArgs a) {
     __shared__ float4 sm[8][32];
@@ -747,52 +812,18 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
         }
         return;
     }
+    if constexpr (W == 0) {                         // the wide kernel's few splits: a warp per row
+        const size_t row = (size_t)blockIdx.x * 8 + warp;
+        dependents_wait();
+        if (row < rows) join_row<1>(a, {row * a.splits, 1, a.splits}, row, 0, lane, nullptr, nullptr);
+        return;
+    }
     const size_t bh = blockIdx.x / a.rows;
-    const int r = (int)(blockIdx.x % a.rows), b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+    const int r = (int)(blockIdx.x % a.rows);
     const Parts p = parts_of<W>(a, bh, r);
     dependents_wait();
     if (W > 0 && p.count == 1) return;              // the attention kernel wrote this row itself
-    float top = -CUDART_INF_F;
-    for (int k = lane; k < p.count; k += 32) top = fmaxf(top, a.part_lse[p.base + k * p.step]);
-#pragma unroll
-    for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
-    float sum = 0.f;
-    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = warp; k < p.count; k += 8) {
-        const float e = a.part_lse[p.base + k * p.step];
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p.base + k * p.step) * kKv8Dim + 4 * lane);
-        const float f = e == -CUDART_INF_F ? 0.f : exp2f(e - top);     // (a part that saw nothing holds zeros)
-        sum += f;
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
-    }
-    sm[warp][lane] = acc;
-    if (lane == 0) sm_sum[warp] = sum;
-    __syncthreads();
-    if (warp) return;
-    sum = 0.f;
-    acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int w = 0; w < 8; ++w) {
-        const float4 x = sm[w][lane];
-        sum += sm_sum[w];
-        acc.x += x.x;
-        acc.y += x.y;
-        acc.z += x.z;
-        acc.w += x.w;
-    }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
-    const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
-    __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + 4 * lane;
-    *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
-    if (lane == 0) {
-        const float e = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
-        if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = e;
-        if (W == 0 && a.row_lse) a.row_lse[bh * a.rows + r] = e;
-    }
+    join_row<8>(a, p, bh * a.rows + r, warp, lane, sm, sm_sum);
 }
 
 // Weights after the wide kernel: its rows' log-sum-exps are joined by then.
@@ -871,8 +902,7 @@ static cudaError_t launch_narrow(const Kv8AttnArgs& a, int nt, cudaStream_t stre
     switch (nt) {
         case 1: return launch_narrow<FMT, 1, LOGITS>(a, stream);
         case 2: return launch_narrow<FMT, 2, LOGITS>(a, stream);
-        case 3: return launch_narrow<FMT, 3, LOGITS>(a, stream);
-        default: return launch_narrow<FMT, 4, LOGITS>(a, stream);
+        default: return launch_narrow<FMT, 3, LOGITS>(a, stream);
     }
 }
 
@@ -959,7 +989,7 @@ extern "C" int minf_kv8_attention(
         return MINF_OK;
     }
     if (s.splits > 1) {
-        e = launch_behind(kv8_finish_kernel<0>, dim3((unsigned)rows), kFinishThreads, 0, st, a);
+        e = launch_behind(kv8_finish_kernel<0>, dim3((unsigned)((rows + 7) / 8)), kFinishThreads, 0, st, a);
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
     }
     if (chunks) {
