@@ -726,7 +726,8 @@ __device__ __forceinline__ void join_row(const Kv8AttnArgs& a, const Parts& p, s
 }
 
 constexpr int kFinishThreads = 256;
-constexpr int kFinishTokens = 1024;                 // tokens of a CTA that sums weights
+constexpr int kFinishTokens = 1024;                 // tokens that a CTA sums weights of at a time
+constexpr int kFinishCtas = 8 * kSMs;               // CTAs of that kind worth starting: resident at once, each with some microseconds of start
 
 // Weights of tokens [t0, t0 + kFinishTokens) of a head: the probabilities of its rows, summed in their order.  A thread has
 // four tokens, whose logits it reads together.
@@ -786,14 +787,14 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
     dependents_launch();
     if (blockIdx.x >= rows) {
         if constexpr (W > 0) {
-            const int chunks = (int)((a.tokens + kFinishTokens - 1) / kFinishTokens);
+            const int chunks = (int)((a.tokens + a.chunk - 1) / a.chunk);
             const int i = (int)(blockIdx.x - rows), chunk = i % chunks;
             const size_t bh = i / chunks;
             const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
             const int n = clipped_length(a, b);
             const Parts p = parts_of<W>(a, bh, 0);
             dependents_wait();
-            if (chunk * kFinishTokens >= n) return;
+            if ((long long)chunk * a.chunk >= n) return;
             for (int r = warp; r < a.rows; r += 8) {
                 float top = -CUDART_INF_F, sum = 0.f;
                 for (int k = lane; k < p.count; k += 32) top = fmaxf(top, a.part_lse[p.base + r + k * p.step]);
@@ -808,7 +809,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
                 if (lane == 0) sm_lse[r] = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
             }
             __syncthreads();
-            sum_weights(a, b, h, n, chunk * kFinishTokens, sm_lse);
+            for (int t0 = chunk * a.chunk; t0 < min((long long)n, (chunk + 1ll) * a.chunk); t0 += kFinishTokens) sum_weights(a, b, h, n, t0, sm_lse);
         }
         return;
     }
@@ -980,7 +981,8 @@ extern "C" int minf_kv8_attention(
     cudaError_t e = launch_attention(a, s, st);
     if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_attention_kernel failed: %s", cudaGetErrorString(e));
     const long long pairs = (long long)cache->batch * cache->heads, rows = pairs * a.rows;
-    const long long chunks = weights ? ((long long)max_length + kFinishTokens - 1) / kFinishTokens : 0;
+    a.chunk = kFinishTokens * (int)std::max(1ll, std::min(16ll, pairs * (max_length / kFinishTokens) / kFinishCtas));
+    const long long chunks = weights ? ((long long)max_length + a.chunk - 1) / a.chunk : 0;
     if (s.nt) {
         const dim3 grid((unsigned)(rows + pairs * chunks));
         e = narrow_warps(s.nt) == 8 ? launch_behind(kv8_finish_kernel<8>, grid, kFinishThreads, 0, st, a)
@@ -993,7 +995,7 @@ extern "C" int minf_kv8_attention(
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
     }
     if (chunks) {
-        e = launch_behind(kv8_weights_kernel, dim3((unsigned)chunks, cache->heads, cache->batch), kFinishThreads, 0, st, a);
+        e = launch_behind(kv8_weights_kernel, dim3((unsigned)((max_length + kFinishTokens - 1) / kFinishTokens), cache->heads, cache->batch), kFinishThreads, 0, st, a);
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_weights_kernel failed: %s", cudaGetErrorString(e));
     }
     return MINF_OK;

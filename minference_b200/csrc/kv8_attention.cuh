@@ -24,6 +24,7 @@ struct Kv8AttnArgs {
     float* logits;                  // [batch*heads][tokens][pitch], or NULL
     int pitch;
     long long tokens;               // rows of `logits` per head
+    int chunk;                      // tokens of a CTA that sums weights
     float* weights;
     long long ws[2];
     const float* add_to;

@@ -97,7 +97,7 @@ __device__ __forceinline__ uint2 values_to_codes(const float (&x)[8], float scal
 
 // ------------------------------------------------------------------------------------------------- store
 // One CTA per (block of 64 tokens that gets new ones, head, keys or values).  256 threads hold the block in
-// registers, eight values of four rows each: one read of the new tokens, one write of the codes.
+// registers, sixteen values of two rows each: one read of the new tokens, one write of the codes.
 // Bound by HBM: 4 B read and 2 B written per (key, value) pair of elements.
 struct StoreArgs {
     minf_kv8_cache c;
@@ -132,34 +132,53 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(const __grid_c
     const __nv_bfloat16* src = a.src[which] + b * a.stride[which][0] + h * a.stride[which][1];
     const long long row_stride = a.stride[which][2];
     __nv_bfloat16* tail = static_cast<__nv_bfloat16*>(which ? a.c.v_tail : a.c.k_tail) + bh * (kKv8Block * kKv8Dim);
-    const int chunk = threadIdx.x & 15, row0 = threadIdx.x >> 4;
-    auto new_row = [&](int t) { return *reinterpret_cast<const uint4*>(src + (t - start) * row_stride + chunk * 8); };
-    auto tail_row = [&](int r) { return reinterpret_cast<uint4*>(tail + r * kKv8Dim + chunk * 8); };
+    const int chunk = threadIdx.x & 7, row0 = threadIdx.x >> 3;        // 16 values of rows row0 and row0 + 32
+    auto new_row = [&](int t) { return reinterpret_cast<const uint4*>(src + (t - start) * row_stride + chunk * 16); };
+    auto tail_row = [&](int r) { return reinterpret_cast<uint4*>(tail + r * kKv8Dim + chunk * 16); };
 
     if (complete) {
-        float x[4][8];
+        uint4 raw[2][2];
         float top = 0.f;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int r = row0 + 16 * i, t = blk * kKv8Block + r;
-            bf16x8_to_values(t < start ? *tail_row(r) : new_row(t), x[i]);
+        for (int i = 0; i < 2; ++i) {
+            const int r = row0 + 32 * i, t = blk * kKv8Block + r;
+            if (t < start) {
+                raw[i][0] = tail_row(r)[0];
+                raw[i][1] = tail_row(r)[1];
+            } else {
+                raw[i][0] = __ldcs(new_row(t));
+                raw[i][1] = __ldcs(new_row(t) + 1);
+            }
+        }
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[i][j]));
+        for (int i = 0; i < 4; ++i) {
+            float x[8];
+            bf16x8_to_values(raw[i >> 1][i & 1], x);
+#pragma unroll
+            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[j]));
         }
         top = block_max<kStoreThreads>(top, red);           // (its barrier also ends the reads of the tail)
         const float scale = scale_of<FMT>(top);
         uint8_t* codes = static_cast<uint8_t*>(which ? a.c.v : a.c.k) + (bh * a.c.capacity + (size_t)blk * kKv8Block) * kKv8Dim;
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            *reinterpret_cast<uint2*>(codes + (row0 + 16 * i) * kKv8Dim + chunk * 8) = values_to_codes<FMT>(x[i], scale);
+        for (int i = 0; i < 2; ++i) {
+            float x[8], y[8];
+            bf16x8_to_values(raw[i][0], x);
+            bf16x8_to_values(raw[i][1], y);
+            const uint2 lo = values_to_codes<FMT>(x, scale), hi = values_to_codes<FMT>(y, scale);
+            *reinterpret_cast<uint4*>(codes + (row0 + 32 * i) * kKv8Dim + chunk * 16) = make_uint4(lo.x, lo.y, hi.x, hi.y);
+        }
         if (threadIdx.x == 0) (which ? a.c.v_scale : a.c.k_scale)[bh * (a.c.capacity / kKv8Block) + blk] = scale;
     }
     if (blk == blk0 && end % kKv8Block) {                   // the tokens behind the last complete block
         const int t0 = max(start, last * kKv8Block);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int t = last * kKv8Block + row0 + 16 * i;
-            if (t >= t0 && t < end) *tail_row(row0 + 16 * i) = new_row(t);
+        for (int i = 0; i < 2; ++i) {
+            const int t = last * kKv8Block + row0 + 32 * i;
+            if (t >= t0 && t < end) {
+                tail_row(row0 + 32 * i)[0] = new_row(t)[0];
+                tail_row(row0 + 32 * i)[1] = new_row(t)[1];
+            }
         }
     }
 }
@@ -175,19 +194,6 @@ struct LoadArgs {
     __nv_bfloat16* out[2];
 };
 
-// Eight values of token t (0 <= t < n) of one head.
-template <int FMT>
-__device__ __forceinline__ void token_values(const minf_kv8_cache& c, int which, size_t bh, int t, int n, int chunk, float (&v)[8]) {
-    if (t < n / kKv8Block * kKv8Block) {
-        const uint8_t* codes = static_cast<const uint8_t*>(which ? c.v : c.k) + (bh * c.capacity + t) * kKv8Dim + chunk * 8;
-        const float scale = (which ? c.v_scale : c.k_scale)[bh * (c.capacity / kKv8Block) + t / kKv8Block];
-        codes_to_values<FMT>(*reinterpret_cast<const uint2*>(codes), scale, v);
-    } else {
-        const __nv_bfloat16* tail = static_cast<const __nv_bfloat16*>(which ? c.v_tail : c.k_tail) + bh * (kKv8Block * kKv8Dim);
-        bf16x8_to_values(*reinterpret_cast<const uint4*>(tail + (t % kKv8Block) * kKv8Dim + chunk * 8), v);
-    }
-}
-
 __device__ __forceinline__ uint4 pack_bf16x8(const float (&v)[8]) {
     return make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]), pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
 }
@@ -198,20 +204,34 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_load_kernel(const __grid_co
     const int n = kv8_length(a.lengths, a.length_all, b, a.c.capacity, a.c.status);
     const long long first = a.first ? a.first[b] : a.first_all;
     const size_t bh = (size_t)b * a.c.heads + h;
-    const int chunk = threadIdx.x & 15;
-    __nv_bfloat16* out = a.out[which] + bh * a.count * kKv8Dim + chunk * 8;
+    const int chunk = threadIdx.x & 7;                      // 16 values of two rows
+    const int whole = n / kKv8Block * kKv8Block;
+    const uint8_t* codes = static_cast<const uint8_t*>(which ? a.c.v : a.c.k) + bh * a.c.capacity * kKv8Dim + chunk * 16;
+    const float* scales = (which ? a.c.v_scale : a.c.k_scale) + bh * (a.c.capacity / kKv8Block);
+    const __nv_bfloat16* tail = static_cast<const __nv_bfloat16*>(which ? a.c.v_tail : a.c.k_tail) + bh * (kKv8Block * kKv8Dim) + chunk * 16;
+    __nv_bfloat16* out = a.out[which] + bh * a.count * kKv8Dim + chunk * 16;
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        const int r = blockIdx.x * kKv8Block + (threadIdx.x >> 4) + 16 * i;
+    for (int i = 0; i < 2; ++i) {
+        const int r = blockIdx.x * kKv8Block + (threadIdx.x >> 3) + 32 * i;
         if (r >= a.count) break;
         const long long t = first + r;
-        uint4 w = make_uint4(0u, 0u, 0u, 0u);
-        if (t >= 0 && t < n) {
+        uint4 lo = make_uint4(0u, 0u, 0u, 0u), hi = lo;
+        if (t >= 0 && t < whole) {
+            const uint4 c = *reinterpret_cast<const uint4*>(codes + (size_t)t * kKv8Dim);
+            const float scale = scales[t / kKv8Block];
             float v[8];
-            token_values<FMT>(a.c, which, bh, (int)t, n, chunk, v);
-            w = pack_bf16x8(v);
+            codes_to_values<FMT>(make_uint2(c.x, c.y), scale, v);
+            lo = pack_bf16x8(v);
+            codes_to_values<FMT>(make_uint2(c.z, c.w), scale, v);
+            hi = pack_bf16x8(v);
+        } else if (t >= whole && t < n) {
+            const uint4* x = reinterpret_cast<const uint4*>(tail + (t - whole) * kKv8Dim);
+            lo = x[0];
+            hi = x[1];
         }
-        *reinterpret_cast<uint4*>(out + (size_t)r * kKv8Dim) = w;
+        uint4* to = reinterpret_cast<uint4*>(out + (size_t)r * kKv8Dim);
+        to[0] = lo;
+        to[1] = hi;
     }
 }
 

@@ -91,9 +91,8 @@ class KV8Cache:
         """An empty cache like this one; it reports into this one's status."""
         b, h, cap = self.batch, self.kv_heads, (capacity + BLOCK - 1) // BLOCK * BLOCK
         new = KV8Cache.__new__(KV8Cache)
-        new._set(self.k.new_empty((b, h, cap, HEAD_DIM)), self.k.new_empty((b, h, cap, HEAD_DIM)),
-                 self.k_scale.new_empty((b, h, cap // BLOCK)), self.k_scale.new_empty((b, h, cap // BLOCK)),
-                 torch.empty_like(self.k_tail), torch.empty_like(self.k_tail), self.status)
+        new._set(*self.k.new_empty((2, b, h, cap, HEAD_DIM)).unbind(0), *self.k_scale.new_empty((2, b, h, cap // BLOCK)).unbind(0),
+                 *self.k_tail.new_empty((2, b, h, BLOCK, HEAD_DIM)).unbind(0), self.status)
         return new
 
     @classmethod
@@ -171,7 +170,7 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
-    k, v = cache.k_tail.new_empty(shape), cache.k_tail.new_empty(shape)
+    k, v = cache.k_tail.new_empty((2, *shape)).unbind(0)
     _launch("minf_kv8_load", cache, cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr())
     return k, v
 
