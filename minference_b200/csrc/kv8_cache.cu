@@ -585,8 +585,21 @@ extern "C" int minf_kv8_evict(
     if (!weights || !w_strides || !kept || !weights_out || !lengths_out) return fail(MINF_E_ARG, "null pointer argument");
     if (src->format != dst->format || src->batch != dst->batch || src->heads != dst->heads)
         return fail(MINF_E_ARG, "the two caches must have one format, batch and head count");
-    if (src->k == dst->k || src->v == dst->v || src->k_tail == dst->k_tail || src->v_tail == dst->v_tail)
-        return fail(MINF_E_ARG, "eviction writes into another cache than it reads");
+    {
+        auto overlap = [](const void* p, size_t np, const void* q, size_t nq) {
+            const uintptr_t a = reinterpret_cast<uintptr_t>(p), b = reinterpret_cast<uintptr_t>(q);
+            return a < b + nq && b < a + np;
+        };
+        const size_t pairs = (size_t)src->batch * src->heads, tails = pairs * kKv8Block * kKv8Dim * 2;
+        const void* from[6] = {src->k, src->v, src->k_scale, src->v_scale, src->k_tail, src->v_tail};
+        const void* to[6] = {dst->k, dst->v, dst->k_scale, dst->v_scale, dst->k_tail, dst->v_tail};
+        auto bytes = [&](const minf_kv8_cache* c, int i) {
+            return i < 2 ? pairs * c->capacity * kKv8Dim : i < 4 ? pairs * (c->capacity / kKv8Block) * sizeof(float) : tails;
+        };
+        for (int i = 0; i < 6; ++i)
+            for (int j = 0; j < 6; ++j)
+                if (overlap(from[i], bytes(src, i), to[j], bytes(dst, j))) return fail(MINF_E_ARG, "eviction writes into another cache than it reads");
+    }
     if (budget < 1 || recent < 0 || sink < 0 || (long long)recent + sink > budget)
         return fail(MINF_E_ARG, "budget %d must hold the %d first and %d last tokens", budget, sink, recent);
     if (budget > dst->capacity) return fail(MINF_E_ARG, "budget %d does not fit a cache of %d tokens", budget, dst->capacity);

@@ -91,8 +91,9 @@ class KV8Cache:
         """An empty cache like this one; it reports into this one's status."""
         b, h, cap = self.batch, self.kv_heads, (capacity + BLOCK - 1) // BLOCK * BLOCK
         new = KV8Cache.__new__(KV8Cache)
-        new._set(*self.k.new_empty((2, b, h, cap, HEAD_DIM)).unbind(0), *self.k_scale.new_empty((2, b, h, cap // BLOCK)).unbind(0),
-                 *self.k_tail.new_empty((2, b, h, BLOCK, HEAD_DIM)).unbind(0), self.status)
+        new._set(self.k.new_empty((b, h, cap, HEAD_DIM)), self.k.new_empty((b, h, cap, HEAD_DIM)),
+                 self.k_scale.new_empty((b, h, cap // BLOCK)), self.k_scale.new_empty((b, h, cap // BLOCK)),
+                 self.k_tail.new_empty((b, h, BLOCK, HEAD_DIM)), self.k_tail.new_empty((b, h, BLOCK, HEAD_DIM)), self.status)
         return new
 
     @classmethod
@@ -112,7 +113,7 @@ class KV8Cache:
         if bits:
             self.status.zero_()
             _fail(f"8-bit cache: device reported error bits {bits:#x} (16 = a length or position outside the cache of "
-                  f"{self.capacity} tokens, or outside max_length)")
+                  f"{self.capacity} tokens, or outside max_length; 1 = an abandoned wait)")
 
     def nbytes(self) -> int:
         return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
@@ -170,7 +171,7 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
-    k, v = cache.k_tail.new_empty((2, *shape)).unbind(0)
+    k, v = cache.k_tail.new_empty(shape), cache.k_tail.new_empty(shape)
     _launch("minf_kv8_load", cache, cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -180,6 +181,21 @@ def _weights_arg(t, what: str, cache: KV8Cache, max_length: int):
         _fail(f"{what} must be fp32 [{cache.batch}, {cache.kv_heads}, >= {max_length}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
     if t.stride(2) != 1 and t.shape[2] > 1:
         _fail(f"{what} must be contiguous along its tokens")
+
+
+def _extent(t: torch.Tensor):
+    """First and last byte address of a tensor's elements."""
+    return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
+
+
+def _check_written(weights: torch.Tensor, add_to: torch.Tensor | None) -> None:
+    """No element of ``weights`` may be written twice, or be read as ``add_to`` of another token."""
+    if (weights.shape[0] > 1 and weights.stride(0) == 0) or (weights.shape[1] > 1 and weights.stride(1) == 0):
+        _fail("weights must not be an expanded view: its elements are written")
+    if add_to is not None and add_to is not weights:
+        a, b = _extent(weights), _extent(add_to)
+        if a[0] < b[1] and b[0] < a[1] and (a[0] != b[0] or weights.stride() != add_to.stride()):
+            _fail("add_to overlaps weights without being the same view")
 
 
 def _max_length(cache: KV8Cache, lengths, max_length):
@@ -201,7 +217,9 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
     host (the capacity if not given), by which the work is split and scratch memory sized.
     ``weights [B, Hkv, >= max_length]`` fp32 receives the attention weight of each token -- the probabilities summed over
     the head's queries -- plus ``add_to`` (``add_to=weights`` sums up in place); entries behind a sequence's length are
-    left as they were.
+    left as they were.  It takes scratch memory of 4 bytes for every query row and token.
+    Forward only.  One to 24 rows per cache head (H / Hkv * S) and more take different kernels; both are within the
+    roundings of P to 16 bits of the exact result.
     """
     query = _rows(query, "query", cache)
     b, hq, s, d = query.shape
@@ -215,6 +233,8 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
         if weights is None:
             _fail("add_to without weights")
         _weights_arg(add_to, "add_to", cache, longest)
+    if weights is not None:
+        _check_written(weights, add_to)
     out = query.new_empty((b, hq, s, d))
     lse = cache.k_scale.new_empty((b, hq, s)) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)

@@ -416,6 +416,8 @@ def test_python_refusals():
            lambda: kv8_attention(q, cache, 5, max_length=4), lambda: kv8_attention(q, cache, 5, max_length=200),
            lambda: kv8_attention(q, cache, 5, add_to=w), lambda: kv8_attention(q, cache, 100, weights=w[..., :99]),
            lambda: kv8_attention(q, cache, 5, weights=w.double()), lambda: kv8_attention(q, cache, 5, weights=w.transpose(1, 2)),
+           lambda: kv8_attention(q, cache, 5, weights=w[:1].expand(2, 2, 128)), lambda: kv8_attention(q, cache, 5, weights=w[:, :1].expand(2, 2, 128)),
+           lambda: kv8_attention(q, cache, 5, max_length=100, weights=w[..., :100], add_to=w[..., 10:110]),
            lambda: kv8_attention(q.cpu(), cache, 1), lambda: kv8_attention(q[:, :, :0], cache, 1),
            lambda: kv8_attention(q, cache, torch.tensor([1, 1], dtype=torch.int32)), lambda: kv8_load(cache, 129), lambda: kv8_load(cache, 1, count=-1),
            lambda: kv8_evict(cache, 128, w, 0, recent=0), lambda: kv8_evict(cache, 128, w, 8, recent=6, sink=3),

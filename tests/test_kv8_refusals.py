@@ -72,11 +72,15 @@ def test_attention_checks(cabi):
 
 def test_evict_checks(cabi):
     lib = cabi.lib()
-    src, dst = _desc(cabi), _desc(cabi, k=1 << 20, v=2 << 20, k_tail=3 << 20, v_tail=4 << 20, capacity=64)
+    other = dict(k=1 << 20, v=2 << 20, k_scale=5 << 20, v_scale=6 << 20, k_tail=3 << 20, v_tail=4 << 20)
+    src = _desc(cabi, k=1 << 24, v=2 << 24, k_scale=5 << 24, v_scale=6 << 24, k_tail=3 << 24, v_tail=4 << 24)
+    dst = _desc(cabi, capacity=64, **other)
     w = (ctypes.c_int64 * 3)(128, 128, 0)
     def call(s=src, d=dst, n=128, longest=128, weights=256, budget=32, recent=8, sink=4, kept=256):
         return lib.minf_kv8_evict(ctypes.byref(s), ctypes.byref(d), None, n, longest, weights, w, budget, recent, sink, kept, 256, 256, None)
-    for kw, word in [(dict(d=src), b"another"), (dict(d=_desc(cabi, k=1 << 20, v=2 << 20, k_tail=3 << 20, v_tail=4 << 20, format=1)), b"format"),
+    inside = dict(other, v=(1 << 24) + 32 * 128, capacity=64)      # its values in the middle of the source's keys
+    for kw, word in [(dict(d=src), b"another"), (dict(d=_desc(cabi, **inside)), b"another"),
+                     (dict(d=_desc(cabi, **dict(other, k_scale=(5 << 24) + 4))), b"another"), (dict(d=_desc(cabi, format=1, **other)), b"format"),
                      (dict(budget=0), b"budget"), (dict(recent=30), b"budget"), (dict(sink=-1), b"budget"), (dict(recent=-1), b"budget"),
                      (dict(budget=65), b"fit"), (dict(n=129), b"outside"), (dict(longest=129), b"max_length"), (dict(weights=0), b"null"),
                      (dict(kept=0), b"null")]:
