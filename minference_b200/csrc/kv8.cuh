@@ -12,6 +12,7 @@
 #include <cuda_fp16.h>
 #include <cuda_runtime.h>
 
+#include <atomic>
 #include <cstdint>
 #include <utility>
 
@@ -97,6 +98,19 @@ cudaError_t launch_behind(void (*kernel)(Params...), dim3 grid, int threads, siz
 }
 __device__ __forceinline__ void dependents_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 __device__ __forceinline__ void dependents_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+// Lets a kernel use `bytes` of dynamic shared memory, once per device (`done`: a bit for each device, one word per kernel).
+template <class Kernel>
+cudaError_t allow_shared(Kernel kernel, int bytes, std::atomic<unsigned long long>& done) {
+    int device = 0;
+    cudaError_t e = cudaGetDevice(&device);
+    if (e != cudaSuccess) return e;
+    const unsigned long long bit = device < 64 ? 1ull << device : 0ull;
+    if (done.load(std::memory_order_relaxed) & bit) return cudaSuccess;
+    e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e == cudaSuccess) done.fetch_or(bit, std::memory_order_relaxed);
+    return e;
+}
 
 // Host-side check of a cache descriptor; MINF_OK or a negative code with its message set.
 int kv8_check(const minf_kv8_cache* c);

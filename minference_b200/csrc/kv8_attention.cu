@@ -222,6 +222,7 @@ __device__ __forceinline__ Share share_of(const Kv8AttnArgs& a, bool report) {
         units *= a.c.heads;
     }
     int ctas = a.splits;
+    if (a.single) return {units, pairs};            // (not looked at: CTA i has head i)
     // a whole number of CTAs per head where that leaves few of them idle: then none works on two pieces, which costs it a new
     // start and a second joining (about 5 us)
     if (same && pairs <= ctas && ctas / pairs * pairs * 10 >= ctas * 9) ctas = ctas / pairs * pairs;
@@ -297,21 +298,22 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     const long long all_units = share.units;
     const int ctas = share.ctas;
     if ((int)blockIdx.x >= ctas) return;
-    long long at = mul_div(all_units, blockIdx.x, ctas);
-    const long long stop = mul_div(all_units, blockIdx.x + 1, ctas);
+    long long at = a.single ? 0 : mul_div(all_units, blockIdx.x, ctas);
+    const long long stop = a.single ? 1 : mul_div(all_units, blockIdx.x + 1, ctas);
 #pragma unroll 1
     while (at < stop) {                             // a piece: units of one sequence and head
-    const Place place = locate<kAttnWarps>(a, at);
+    const Place place = a.single ? Place{(int)blockIdx.x / a.c.heads, (int)blockIdx.x % a.c.heads, 0, clipped_length(a, blockIdx.x / a.c.heads)}
+                                 : locate<kAttnWarps>(a, at);
     const int h = place.h, b = place.b, n = place.n;
     const size_t bh = (size_t)b * a.c.heads + h;
     const int full = n / kKv8Block;                 // complete blocks
     const int full_u = full * (kKv8Block / kUnit), units = units_of<kAttnWarps>(n);
-    const int x_lo = place.u, x_hi = (int)min((long long)units, x_lo + (stop - at));
+    const int x_lo = place.u, x_hi = a.single ? units : (int)min((long long)units, x_lo + (stop - at));
     const int u_lo = min(full_u, x_lo), u_hi = min(full_u, x_hi);
     const bool takes_tail = x_hi == units;          // the tail's units: its last one's piece takes all of it
     const bool whole = x_lo == 0 && x_hi == units;  // nothing to join: the output is written here
-    const size_t piece = blockIdx.x + bh;           // pieces are numbered so: both grow along the units, one of them at each new piece
-    at += x_hi - x_lo;
+    const size_t piece = a.single ? bh : blockIdx.x + bh;       // pieces are numbered so: both grow along the units, one of them at each new piece
+    at = a.single ? stop : at + (x_hi - x_lo);
     if (takes_tail && n % kKv8Block) {              // the tail is wanted at the end: on its way to L2 from here
         const char* kt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.k_tail) + bh * kKv8Block * kKv8Dim);
         const char* vt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.v_tail) + bh * kKv8Block * kKv8Dim);
@@ -665,6 +667,7 @@ __device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r
         return {(bh * a.rows + r) * a.splits, 1, a.splits};
     } else {
         const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
+        if (a.single) return {bh * a.rows + r, (size_t)a.rows, 1};
         const Share share = share_of<W>(a, false);
         const long long all = share.units;
         const int ctas = share.ctas;
@@ -838,6 +841,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_weights_kernel(const __gri
 // ---------------------------------------------------------------------------------------------------- host
 struct AttnShape {
     int nt;                         // column groups of the narrow kernel, 0: the wide kernel
+    bool single;                    // narrow kernel: a CTA per head
     int tiles, splits, pitch;
     long long tokens;
     size_t part_o, part_lse, row_lse, logits, bytes;
@@ -852,8 +856,10 @@ static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_
     if (s.nt) {
         const int warps = narrow_warps(s.nt);
         const long long units = (long long)(max_length / kKv8Block) * (kKv8Block / kUnit) + warps;
-        s.splits = (int)std::min<long long>(2 * kSMs, (pairs * units + warps - 1) / warps);
-        parts = (s.splits + pairs) * rows;
+        // Short sequences, a unit for every warp and the tail: a CTA per head, and no second kernel unless the weights need one
+        s.single = units <= 2 * warps;
+        s.splits = s.single ? (int)std::min<long long>(pairs, 0x7fffffff) : (int)std::min<long long>(2 * kSMs, (pairs * units + warps - 1) / warps);
+        parts = (s.single ? pairs : s.splits + pairs) * rows;
     } else {
         // one CTA an SM: the number of splits (of two tiles of tokens at least) that wastes least of its last wave; each
         // costs about as much again as two tiles (its start, its end and the joining)
@@ -891,8 +897,8 @@ static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_le
 template <int FMT, int NT, bool LOGITS>
 static cudaError_t launch_narrow(const Kv8AttnArgs& a, cudaStream_t stream) {
     constexpr int bytes = narrow_warps(NT) * kRingSlots * kSlotBytes + (NT > 2 ? NT * 2048 : 0);
-    // per device, and cheap: every call sets it
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_kernel<FMT, NT, LOGITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_shared(kv8_attention_kernel<FMT, NT, LOGITS>, bytes, allowed);
     if (e != cudaSuccess) return e;
     kv8_attention_kernel<FMT, NT, LOGITS><<<a.splits, narrow_warps(NT) * 32, bytes, stream>>>(a);
     return cudaGetLastError();
@@ -959,6 +965,7 @@ extern "C" int minf_kv8_attention(
     a.max_length = max_length;
     a.scale_log2 = sm_scale * 1.4426950408889634f;
     a.splits = s.splits;
+    a.single = s.single;
     char* base = static_cast<char*>(scratch);
     a.part_o = reinterpret_cast<float*>(base + s.part_o);
     a.part_lse = reinterpret_cast<float*>(base + s.part_lse);
@@ -983,6 +990,7 @@ extern "C" int minf_kv8_attention(
     const long long pairs = (long long)cache->batch * cache->heads, rows = pairs * a.rows;
     a.chunk = kFinishTokens * (int)std::max(1ll, std::min(16ll, pairs * (max_length / kFinishTokens) / kFinishCtas));
     const long long chunks = weights ? ((long long)max_length + a.chunk - 1) / a.chunk : 0;
+    if (s.nt && s.single && !chunks) return MINF_OK;
     if (s.nt) {
         const dim3 grid((unsigned)(rows + pairs * chunks));
         e = narrow_warps(s.nt) == 8 ? launch_behind(kv8_finish_kernel<8>, grid, kFinishThreads, 0, st, a)

@@ -606,7 +606,8 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
 template <int FMT, bool LOGITS>
 static cudaError_t launch_wide(const Kv8AttnArgs& a, int tiles, cudaStream_t stream) {
     constexpr int bytes = kWCtlOff + sizeof(WideCtl);
-    const cudaError_t e = cudaFuncSetAttribute(kv8_attention_wide_kernel<FMT, LOGITS>, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    static std::atomic<unsigned long long> allowed{0};
+    const cudaError_t e = allow_shared(kv8_attention_wide_kernel<FMT, LOGITS>, bytes, allowed);
     if (e != cudaSuccess) return e;
     kv8_attention_wide_kernel<FMT, LOGITS><<<dim3(a.splits, a.c.heads * tiles, a.c.batch), kWideThreads, bytes, stream>>>(a, tiles);
     return cudaGetLastError();

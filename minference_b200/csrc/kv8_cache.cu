@@ -623,7 +623,8 @@ extern "C" int minf_kv8_evict(
     while (parts < kSelectCluster && (long long)max_length > (long long)parts * kSelectPart) parts *= 2;
     a.cached = std::min(kSelectCached, (max_length / parts + 64) / 32 * 32);
     const size_t shared = (size_t)(kSelectBins + a.cached) * 4;
-    MINF_CUDA_OK(cudaFuncSetAttribute(kv8_select_kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (kSelectBins + kSelectCached) * 4));
+    static std::atomic<unsigned long long> allowed{0};
+    MINF_CUDA_OK(allow_shared(kv8_select_kernel, (kSelectBins + kSelectCached) * 4, allowed));
     {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -14,6 +14,7 @@ from __future__ import annotations
 
 import ctypes
 import functools
+import math
 
 import torch
 
@@ -80,21 +81,41 @@ class KV8Cache:
         self._set(k, v, k_scale, v_scale, k_tail, v_tail, _cabi.new_status(k.device))
 
     def _set(self, k, v, k_scale, v_scale, k_tail, v_tail, status):
-        self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail, self.status = k, v, k_scale, v_scale, k_tail, v_tail, status
+        self._tensors = (k, v, k_scale, v_scale, k_tail, v_tail)
         self.batch, self.kv_heads, self.capacity, _ = k.shape
-        self.dtype, self.device = k.dtype, k.device
-        self._desc = _cabi.Kv8Desc(k.data_ptr(), v.data_ptr(), k_scale.data_ptr(), v_scale.data_ptr(), k_tail.data_ptr(), v_tail.data_ptr(),
-                                   status.data_ptr(), self.batch, self.kv_heads, self.capacity, _FORMATS[k.dtype])
+        self.dtype, self.device, self.status = k.dtype, k.device, status
+        self._desc = _cabi.Kv8Desc(*[t.data_ptr() for t in self._tensors], status.data_ptr(), self.batch, self.kv_heads, self.capacity, _FORMATS[k.dtype])
         self._ref = ctypes.byref(self._desc)
 
     def _smaller(self, capacity: int):
-        """An empty cache like this one; it reports into this one's status."""
+        """An empty cache like this one; it reports into this one's status.  Its tensors are views of one allocation, made when
+        somebody asks for them."""
         b, h, cap = self.batch, self.kv_heads, (capacity + BLOCK - 1) // BLOCK * BLOCK
+        codes, scales, tails = b * h * cap * HEAD_DIM, (b * h * cap // BLOCK * 4 + 15) // 16 * 16, b * h * BLOCK * HEAD_DIM * 2
         new = KV8Cache.__new__(KV8Cache)
-        new._set(self.k.new_empty((b, h, cap, HEAD_DIM)), self.k.new_empty((b, h, cap, HEAD_DIM)),
-                 self.k_scale.new_empty((b, h, cap // BLOCK)), self.k_scale.new_empty((b, h, cap // BLOCK)),
-                 self.k_tail.new_empty((b, h, BLOCK, HEAD_DIM)), self.k_tail.new_empty((b, h, BLOCK, HEAD_DIM)), self.status)
+        new.batch, new.kv_heads, new.capacity, new.dtype, new.device, new.status = b, h, cap, self.dtype, self.device, self.status
+        new._tensors = None
+        new._storage = self.status.new_empty((2 * (codes + scales + tails)) // 4)
+        at = new._storage.data_ptr()
+        new._places = (0, codes, 2 * codes, 2 * codes + scales, 2 * (codes + scales), 2 * (codes + scales) + tails)
+        new._desc = _cabi.Kv8Desc(*[at + x for x in new._places], self.status.data_ptr(), b, h, cap, _FORMATS[self.dtype])
+        new._ref = ctypes.byref(new._desc)
         return new
+
+    def _views(self):
+        if self._tensors is None:
+            b, h, cap, raw = self.batch, self.kv_heads, self.capacity, self._storage.view(torch.uint8)
+            shapes = [((b, h, cap, HEAD_DIM), self.dtype)] * 2 + [((b, h, cap // BLOCK), torch.float32)] * 2 + [((b, h, BLOCK, HEAD_DIM), torch.bfloat16)] * 2
+            self._tensors = tuple(raw[at: at + math.prod(shape) * dtype.itemsize].view(dtype).view(shape)
+                                  for at, (shape, dtype) in zip(self._places, shapes))
+        return self._tensors
+
+    k = property(lambda self: self._views()[0])
+    v = property(lambda self: self._views()[1])
+    k_scale = property(lambda self: self._views()[2])
+    v_scale = property(lambda self: self._views()[3])
+    k_tail = property(lambda self: self._views()[4])
+    v_tail = property(lambda self: self._views()[5])
 
     @classmethod
     def empty(cls, batch: int, kv_heads: int, capacity: int, dtype=torch.float8_e4m3fn, device="cuda"):
@@ -116,7 +137,7 @@ class KV8Cache:
                   f"{self.capacity} tokens, or outside max_length; 1 = an abandoned wait)")
 
     def nbytes(self) -> int:
-        return sum(t.numel() * t.element_size() for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
+        return sum(t.numel() * t.element_size() for t in self._views())
 
 
 def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
@@ -171,7 +192,8 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
-    k, v = cache.k_tail.new_empty(shape), cache.k_tail.new_empty(shape)
+    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
+    v = torch.empty_like(k)
     _launch("minf_kv8_load", cache, cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -236,9 +258,9 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
     if weights is not None:
         _check_written(weights, add_to)
     out = query.new_empty((b, hq, s, d))
-    lse = cache.k_scale.new_empty((b, hq, s)) if return_lse else None
+    lse = torch.empty((b, hq, s), dtype=torch.float32, device=cache.device) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
-    scratch = cache.k_scale.new_empty(nbytes // 4) if nbytes else None      # (in words of four bytes)
+    scratch = cache.status.new_empty(nbytes // 4) if nbytes else None       # (in words of four bytes)
     _launch("minf_kv8_attention", cache,
             cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _I64x3(hq * s * d, s * d, d), hq, s, dev_n, n, longest,
             d ** -0.5 if sm_scale is None else float(sm_scale), lse.data_ptr() if return_lse else None,
@@ -269,7 +291,7 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     elif out is cache or (out.batch, out.kv_heads, out.dtype, out.device) != (cache.batch, cache.kv_heads, cache.dtype, cache.device) or out.capacity < budget:
         _fail("out must be another cache of the same batch, heads, type and device with room for the budget")
     kept = cache.status.new_empty((cache.batch, cache.kv_heads, budget))
-    weights_out = cache.k_scale.new_empty((cache.batch, cache.kv_heads, out.capacity))
+    weights_out = torch.empty((cache.batch, cache.kv_heads, out.capacity), dtype=torch.float32, device=cache.device)
     lengths_out = cache.status.new_empty((cache.batch,))
     _launch("minf_kv8_evict", cache, cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides(weights), budget, recent, sink,
             kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr())
