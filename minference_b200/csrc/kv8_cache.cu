@@ -259,20 +259,27 @@ constexpr int kSelectWarps = kSelectThreads / 32;
 constexpr int kSelectCluster = 8;                           // CTAs at most that share a head's tokens
 constexpr int kSelectPart = 8192;                           // tokens from which on one more is worth its barriers
 constexpr int kSelectBins = 2048;
+constexpr int kSelectList = 2048;                           // keys of the first two passes' bin that a CTA lists
 constexpr int kSelectCached = 40960;                        // keys a CTA keeps in shared memory at most
+// shared memory in words: two histograms (of the even and the odd lanes), the cluster's sums of three passes, the list, the keys
+constexpr int kSelectWords = 2 * kSelectBins + 3 * kSelectBins + kSelectList;
 
 // A cluster per (sequence, head), each CTA a contiguous part of the candidates, whose keys it reads once and keeps in
 // shared memory (beyond 8 x 40960 candidates it reads them again from L2 in each pass).  Three passes of 11, 11 and 10
-// bits find the key of the last token that is kept; the histograms are summed over the cluster through distributed
-// shared memory and every CTA takes the same digit.  Then the warps, each with a contiguous stretch, count what they
-// keep and write it at the offset of everything before them: ascending order without a sort, equal keys by position.
-// What bounds it: the barriers of the three passes (two across the cluster each), not the 4 B a token it reads.
+// bits find the key of the last token that is kept: every CTA adds the bins it has to the first one's sums, which finds
+// the digit for all.  (Every CTA summing all histograms by itself moved 64 KB through distributed shared memory a pass:
+// 4800 cycles instead of 1300 and a barrier.)  Then the warps, each with a contiguous stretch, count what they keep and
+// write it at the offset of everything before them: ascending order without a sort, equal keys by position.
+// What bounds it at 131072 tokens: the first pass (4 B a token read, atomics on a few dozen hot bins) and seven barriers
+// across the cluster of 1500 cycles each.
 __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
     extern __shared__ uint32_t dyn[];
     uint32_t* hist = dyn;
-    uint32_t* cached = dyn + kSelectBins;
+    uint32_t* sums = dyn + 2 * kSelectBins;
+    uint32_t* list = sums + 3 * kSelectBins;
+    uint32_t* cached = dyn + kSelectWords;
     __shared__ uint32_t warp_sum[kSelectWarps];
-    __shared__ uint32_t sh_digit, sh_need;
+    __shared__ uint32_t sh_digit[3], sh_need[3], listed;
     __shared__ uint32_t warp_above[kSelectWarps], warp_equal[kSelectWarps];
     __shared__ uint32_t cta_above, cta_equal;
     namespace cg = cooperative_groups;
@@ -296,83 +303,116 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid
     const int c0 = min(hi, lo + part * chunk), c1 = min(hi, c0 + chunk), count = c1 - c0;
     const bool in_smem = count <= a.cached;
     auto key_at = [&](int i) { return in_smem ? cached[i] : weight_key(w[c0 + i]); };
-
     auto sync = [&] {
         if (parts > 1) cluster.sync();
         else __syncthreads();
     };
+    for (int i = tid; i < 3 * kSelectBins; i += kSelectThreads) sums[i] = 0;
+    if (tid == 0) listed = 0;
+    if (parts > 1) cluster.barrier_arrive();                // the first one's sums are clear before anybody adds to them
 
     uint32_t prefix = 0;
 #pragma unroll 1
     for (int pass = 0; pass < 3; ++pass) {
         const int shift = pass == 0 ? 21 : pass == 1 ? 10 : 0, bits = pass == 2 ? 10 : 11;
         const uint32_t mask = (1u << bits) - 1u;
-        hist[tid] = 0;
-        hist[tid + kSelectThreads] = 0;
+        for (int i = tid; i < 2 * kSelectBins; i += kSelectThreads) hist[i] = 0;
         __syncthreads();
-        for (int i0 = 0; i0 < count; i0 += 8 * kSelectThreads) {
-            uint32_t key[8];
+        auto add = [&](uint32_t key) { atomicAdd(&hist[2 * ((key >> shift) & mask) + (lane & 1)], 1u); };
+        if (pass == 2 && listed <= kSelectList) {
+            for (int i = tid; i < (int)listed; i += kSelectThreads)
+                if (list[i] >> 10 == prefix) add(list[i]);
+        } else {
+            for (int i0 = 0; i0 < count; i0 += 8 * kSelectThreads) {
+                uint32_t key[8];
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = i0 + u * kSelectThreads + tid;
-                if (i < count) key[u] = pass == 0 ? weight_key(w[c0 + i]) : key_at(i);
+                for (int u = 0; u < 8; ++u) {
+                    const int i = i0 + u * kSelectThreads + tid;
+                    key[u] = i >= count ? 0u : pass == 0 ? weight_key(w[c0 + i]) : key_at(i);
+                }
+#pragma unroll
+                for (int u = 0; u < 8; ++u) {
+                    const int i = i0 + u * kSelectThreads + tid;
+                    if (pass == 0) {
+                        if (i < count) {
+                            if (in_smem) cached[i] = key[u];
+                            add(key[u]);
+                        }
+                    } else {
+                        const bool live = i < count && key[u] >> (shift + bits) == prefix;
+                        const uint32_t who = __ballot_sync(0xffffffffu, live);
+                        if (who == 0) continue;
+                        if (live) add(key[u]);
+                        if (pass == 1) {                    // for the third pass
+                            uint32_t at = 0;
+                            if (lane == 0) at = atomicAdd(&listed, __popc(who));
+                            at = __shfl_sync(0xffffffffu, at, 0) + __popc(who & ((1u << lane) - 1u));
+                            if (live && at < kSelectList) list[at] = key[u];
+                        }
+                    }
+                }
             }
+        }
+        __syncthreads();
+        if (pass == 0 && parts > 1) cluster.barrier_wait();
+        uint32_t* total = sums + pass * kSelectBins;
+        uint32_t* to = parts > 1 ? cluster.map_shared_rank(total, 0) : total;
+        for (int i = tid; i < kSelectBins; i += kSelectThreads) {
+            const uint32_t x = hist[2 * i] + hist[2 * i + 1];
+            if (x) atomicAdd(to + i, x);
+        }
+        sync();
+        if (part == 0) {
+            // thread t has bins 2046 - 2t and 2047 - 2t: a scan over the threads runs from the largest key down
+            const int bin = kSelectBins - 2 - 2 * tid;
+            const uint32_t x0 = total[bin], x1 = total[bin + 1];
+            uint32_t scan = x0 + x1;
 #pragma unroll
-            for (int u = 0; u < 8; ++u) {
-                const int i = i0 + u * kSelectThreads + tid;
-                const bool live = i < count && (pass == 0 || (key[u] >> (shift + bits)) == prefix);
-                if (pass == 0 && in_smem && i < count) cached[i] = key[u];
-                if (live) atomicAdd(&hist[(key[u] >> shift) & mask], 1u);
+            for (int o = 1; o < 32; o <<= 1) {
+                const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
+                if (lane >= o) scan += y;
+            }
+            if (lane == 31) warp_sum[warp] = scan;
+            __syncthreads();
+            const uint32_t before = scan - x0 - x1 + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
+            if (before < need && need <= before + x1) {
+                sh_digit[pass] = bin + 1;
+                sh_need[pass] = need - before;
+            } else if (before + x1 < need && need <= before + x1 + x0) {
+                sh_digit[pass] = bin;
+                sh_need[pass] = need - before - x1;
             }
         }
         sync();
-        // thread t sums bins 2046 - 2t and 2047 - 2t over the cluster: a scan over the threads runs from the largest key down
-        const int bin = kSelectBins - 2 - 2 * tid;
-        uint32_t x1 = 0, x0 = 0;
-        if (parts == kSelectCluster) {
-            uint2 v[kSelectCluster];                        // all on their way at once
-#pragma unroll
-            for (int r = 0; r < kSelectCluster; ++r) v[r] = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
-#pragma unroll
-            for (int r = 0; r < kSelectCluster; ++r) {
-                x0 += v[r].x;
-                x1 += v[r].y;
-            }
-        } else {
-            for (int r = 0; r < parts; ++r) {
-                const uint2 v = *reinterpret_cast<const uint2*>(cluster.map_shared_rank(hist, r) + bin);
-                x0 += v.x;
-                x1 += v.y;
-            }
-        }
-        uint32_t scan = x0 + x1;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const uint32_t y = __shfl_up_sync(0xffffffffu, scan, o);
-            if (lane >= o) scan += y;
-        }
-        if (lane == 31) warp_sum[warp] = scan;
-        __syncthreads();
-        uint32_t before = scan - x0 - x1 + __reduce_add_sync(0xffffffffu, lane < warp ? warp_sum[lane] : 0u);
-        if (before < need && need <= before + x1) {
-            sh_digit = bin + 1;
-            sh_need = need - before;
-        } else if (before + x1 < need && need <= before + x1 + x0) {
-            sh_digit = bin;
-            sh_need = need - before - x1;
-        }
-        sync();                                             // digit and histograms: read by all before the next pass clears them
-        prefix = (prefix << bits) | sh_digit;
-        need = sh_need;
+        prefix = (prefix << bits) | (parts > 1 ? *cluster.map_shared_rank(&sh_digit[pass], 0) : sh_digit[pass]);
+        need = parts > 1 ? *cluster.map_shared_rank(&sh_need[pass], 0) : sh_need[pass];
     }
-    // keys above `prefix` are kept, and the first `need` that equal it
+    // Keys above `prefix` are kept, and the first `need` that equal it.  A warp takes its stretch 32 words of 32 tokens at a
+    // time: lane i has the words (above, equal) of tokens 32 i on.
     const int seg = ((count + kSelectWarps - 1) / kSelectWarps + 31) / 32 * 32;
     const int s0 = min(count, warp * seg), s1 = min(count, s0 + seg);
-    uint32_t above = 0, equal = 0;
-    for (int i = s0 + lane; i < s1; i += 32) {
-        const uint32_t k = key_at(i);
-        above += k > prefix;
-        equal += k == prefix;
+    auto words = [&](int base, uint32_t& gt, uint32_t& eq) {
+        gt = eq = 0;
+        for (int j = 0; j < 32 && base + 32 * j < s1; ++j) {
+            const int i = base + 32 * j + lane;
+            const uint32_t k = i < s1 ? key_at(i) : 0u;
+            const uint32_t bg = __ballot_sync(0xffffffffu, i < s1 && k > prefix), be = __ballot_sync(0xffffffffu, i < s1 && k == prefix);
+            if (lane == j) {
+                gt = bg;
+                eq = be;
+            }
+        }
+    };
+    uint32_t above = 0, equal = 0, first_gt = 0, first_eq = 0;
+    for (int base = s0; base < s1; base += 1024) {
+        uint32_t gt, eq;
+        words(base, gt, eq);
+        above += __popc(gt);
+        equal += __popc(eq);
+        if (base == s0) {
+            first_gt = gt;
+            first_eq = eq;
+        }
     }
     above = __reduce_add_sync(0xffffffffu, above);
     equal = __reduce_add_sync(0xffffffffu, equal);
@@ -390,26 +430,38 @@ __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid
     }
     sync();
     // before this warp's stretch: the parts before this one, the warps before this one
-    uint32_t gt = lane < warp ? warp_above[lane] : 0u, eq = lane < warp ? warp_equal[lane] : 0u;
+    uint32_t gt_before = lane < warp ? warp_above[lane] : 0u, eq_before = lane < warp ? warp_equal[lane] : 0u;
     if (lane < part) {
-        gt += *cluster.map_shared_rank(&cta_above, lane);
-        eq += *cluster.map_shared_rank(&cta_equal, lane);
+        gt_before += *cluster.map_shared_rank(&cta_above, lane);
+        eq_before += *cluster.map_shared_rank(&cta_equal, lane);
     }
-    gt = __reduce_add_sync(0xffffffffu, gt);
-    eq = __reduce_add_sync(0xffffffffu, eq);
-    const uint32_t below_lane = (1u << lane) - 1u;
-    for (int i0 = s0; i0 < s1; i0 += 32) {
-        const int i = i0 + lane;
-        const uint32_t k = i < s1 ? key_at(i) : 0u;
-        const bool is_gt = i < s1 && k > prefix, is_eq = i < s1 && k == prefix;
-        const uint32_t bg = __ballot_sync(0xffffffffu, is_gt), be = __ballot_sync(0xffffffffu, is_eq);
-        const uint32_t my_eq = eq + __popc(be & below_lane);
-        if (is_gt || (is_eq && my_eq < need)) {
-            const uint32_t at = a.sink + gt + __popc(bg & below_lane) + min(my_eq, need);
-            if (at < (uint32_t)a.budget) kept[at] = c0 + i;
+    gt_before = __reduce_add_sync(0xffffffffu, gt_before);
+    eq_before = __reduce_add_sync(0xffffffffu, eq_before);
+    for (int base = s0; base < s1; base += 1024) {
+        uint32_t gt = first_gt, eq = first_eq;
+        if (base != s0) words(base, gt, eq);
+        uint32_t gs = __popc(gt), es = __popc(eq);          // scans over the lanes' words
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const uint32_t x = __shfl_up_sync(0xffffffffu, gs, o), y = __shfl_up_sync(0xffffffffu, es, o);
+            if (lane >= o) {
+                gs += x;
+                es += y;
+            }
         }
-        gt += __popc(bg);
-        eq += __popc(be);
+        uint32_t g = gt_before + gs - __popc(gt), e = eq_before + es - __popc(eq);
+        gt_before += __shfl_sync(0xffffffffu, gs, 31);
+        eq_before += __shfl_sync(0xffffffffu, es, 31);
+        for (uint32_t both = gt | eq; both; both &= both - 1) {
+            const int bit = __ffs(both) - 1;
+            const bool is_gt = gt >> bit & 1u;
+            if (is_gt || e < need) {
+                const uint32_t at = a.sink + g + min(e, need);
+                if (at < (uint32_t)a.budget) kept[at] = c0 + base + 32 * lane + bit;
+            }
+            if (is_gt) ++g;
+            else ++e;
+        }
     }
     sync();                                                 // the counts are read by the others
 }
@@ -622,9 +674,9 @@ extern "C" int minf_kv8_evict(
     int parts = 1;
     while (parts < kSelectCluster && (long long)max_length > (long long)parts * kSelectPart) parts *= 2;
     a.cached = std::min(kSelectCached, (max_length / parts + 64) / 32 * 32);
-    const size_t shared = (size_t)(kSelectBins + a.cached) * 4;
+    const size_t shared = (size_t)(kSelectWords + a.cached) * 4;
     static std::atomic<unsigned long long> allowed{0};
-    MINF_CUDA_OK(allow_shared(kv8_select_kernel, (kSelectBins + kSelectCached) * 4, allowed));
+    MINF_CUDA_OK(allow_shared(kv8_select_kernel, (kSelectWords + kSelectCached) * 4, allowed));
     {
         cudaLaunchAttribute attr[1];
         attr[0].id = cudaLaunchAttributeClusterDimension;

@@ -33,6 +33,12 @@ def _scratch_bytes(batch: int, hq: int, heads: int, n_q: int, max_length: int, w
     return _cabi.lib().minf_kv8_attention_scratch_bytes(batch, hq, heads, n_q, max_length, with_weights)
 
 
+@functools.lru_cache(maxsize=None)
+def _like(device, dtype):
+    """An empty tensor to make others like: the cheapest way to allocate."""
+    return torch.empty(0, dtype=dtype, device=device)
+
+
 # the current stream's handle without a Stream object around it, where torch offers that (2 us less a call)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda index: torch.cuda.current_stream(index).cuda_stream)
 
@@ -192,8 +198,8 @@ def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)
-    k = torch.empty(shape, dtype=torch.bfloat16, device=cache.device)
-    v = torch.empty_like(k)
+    like = _like(cache.device, torch.bfloat16)
+    k, v = like.new_empty(shape), like.new_empty(shape)
     _launch("minf_kv8_load", cache, cache._ref, dev_n, n, dev_first, first, count, k.data_ptr(), v.data_ptr())
     return k, v
 
@@ -258,7 +264,7 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
     if weights is not None:
         _check_written(weights, add_to)
     out = query.new_empty((b, hq, s, d))
-    lse = torch.empty((b, hq, s), dtype=torch.float32, device=cache.device) if return_lse else None
+    lse = _like(cache.device, torch.float32).new_empty((b, hq, s)) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
     scratch = cache.status.new_empty(nbytes // 4) if nbytes else None       # (in words of four bytes)
     _launch("minf_kv8_attention", cache,
@@ -291,7 +297,7 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     elif out is cache or (out.batch, out.kv_heads, out.dtype, out.device) != (cache.batch, cache.kv_heads, cache.dtype, cache.device) or out.capacity < budget:
         _fail("out must be another cache of the same batch, heads, type and device with room for the budget")
     kept = cache.status.new_empty((cache.batch, cache.kv_heads, budget))
-    weights_out = torch.empty((cache.batch, cache.kv_heads, out.capacity), dtype=torch.float32, device=cache.device)
+    weights_out = _like(cache.device, torch.float32).new_empty((cache.batch, cache.kv_heads, out.capacity))
     lengths_out = cache.status.new_empty((cache.batch,))
     _launch("minf_kv8_evict", cache, cache._ref, out._ref, dev_n, n, longest, weights.data_ptr(), _strides(weights), budget, recent, sink,
             kept.data_ptr(), weights_out.data_ptr(), lengths_out.data_ptr())
