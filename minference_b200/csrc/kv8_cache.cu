@@ -150,14 +150,31 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(const __grid_c
                 raw[i][1] = __ldcs(new_row(t) + 1);
             }
         }
+        // the largest magnitude two values at a time (NaN is passed over); only if it is infinite, the finite ones one by one
+        __nv_bfloat162 top2 = __float2bfloat162_rn(0.f);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float x[8];
-            bf16x8_to_values(raw[i >> 1][i & 1], x);
+            const uint4& x = raw[i >> 1][i & 1];
+            const uint32_t words[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t m = words[j] & 0x7fff7fffu;
+                top2 = __hmax2(top2, *reinterpret_cast<const __nv_bfloat162*>(&m));
+            }
         }
-        top = block_max<kStoreThreads>(top, red);           // (its barrier also ends the reads of the tail)
+        top = block_max<kStoreThreads>(fmaxf(__low2float(top2), __high2float(top2)), red);     // (its barrier also ends the reads of the tail)
+        if (top == INFINITY) {                              // the same in every thread
+            top = 0.f;
+#pragma unroll 1
+            for (int i = 0; i < 4; ++i) {
+                float x[8];
+                bf16x8_to_values(raw[i >> 1][i & 1], x);
+#pragma unroll
+                for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+            }
+            __syncthreads();
+            top = block_max<kStoreThreads>(top, red);
+        }
         const float scale = scale_of<FMT>(top);
         uint8_t* codes = static_cast<uint8_t*>(which ? a.c.v : a.c.k) + (bh * a.c.capacity + (size_t)blk * kKv8Block) * kKv8Dim;
 #pragma unroll
