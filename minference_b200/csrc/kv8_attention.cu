@@ -830,12 +830,36 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
     join_row<8>(a, p, bh * a.rows + r, warp, lane, sm, sm_sum);
 }
 
-// Weights after the wide kernel: its rows' log-sum-exps are joined by then.
+// Weights after the wide kernel, whose rows' log-sum-exps are joined by then: a warp has sixteen tokens, its lanes the rows.
+constexpr int kWideTokens = 16 * kFinishThreads / 32;       // tokens of a CTA
 __global__ void __launch_bounds__(kFinishThreads) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    const int b = blockIdx.z, h = blockIdx.y, n = clipped_length(a, b);
+    const int b = blockIdx.z, h = blockIdx.y, n = clipped_length(a, b), lane = threadIdx.x & 31;
+    const int t0 = (blockIdx.x * (kFinishThreads / 32) + (threadIdx.x >> 5)) * 16;
     dependents_wait();
-    if ((int)blockIdx.x * kFinishTokens >= n) return;
-    sum_weights(a, b, h, n, blockIdx.x * kFinishTokens, a.row_lse + ((size_t)b * a.c.heads + h) * a.rows);
+    if (t0 >= n) return;
+    const size_t bh = (size_t)b * a.c.heads + h;
+    const float* x = a.logits + ((long long)bh * a.tokens + t0) * a.pitch;
+    const float* row_lse = a.row_lse + bh * a.rows;
+    float sum[16];
+#pragma unroll
+    for (int k = 0; k < 16; ++k) sum[k] = 0.f;
+    for (int r = lane; r < a.rows; r += 32) {
+        const float e = row_lse[r];
+        float l[16];
+#pragma unroll
+        for (int k = 0; k < 16; ++k) l[k] = t0 + k < n ? x[(long long)k * a.pitch + r] : -CUDART_INF_F;
+#pragma unroll
+        for (int k = 0; k < 16; ++k) sum[k] += weight_of(l[k], e);
+    }
+    float mine = 0.f;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
+        if (lane == k) mine = sum[k];
+    }
+    const int t = t0 + lane;
+    if (lane < 16 && t < n) a.weights[b * a.ws[0] + h * a.ws[1] + t] = (a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f) + mine;
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -1003,7 +1027,7 @@ extern "C" int minf_kv8_attention(
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
     }
     if (chunks) {
-        e = launch_behind(kv8_weights_kernel, dim3((unsigned)((max_length + kFinishTokens - 1) / kFinishTokens), cache->heads, cache->batch), kFinishThreads, 0, st, a);
+        e = launch_behind(kv8_weights_kernel, dim3((unsigned)((max_length + kWideTokens - 1) / kWideTokens), cache->heads, cache->batch), kFinishThreads, 0, st, a);
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_weights_kernel failed: %s", cudaGetErrorString(e));
     }
     return MINF_OK;
