@@ -90,7 +90,7 @@ struct Rows {
 template <int NT, int SUB, bool LOGITS>
 __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, float (&s)[SUB][NT][4], float k_scale, float v_scale,
                                              int t0, bool masked, int all_see, int end, size_t bh, int tg, int c) {
-    const float lv = log2f(v_scale), inv_v = 1.f / v_scale;
+    const float lv = __log2f(v_scale), inv_v = __fdividef(1.f, v_scale);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float f0 = R.mul[nt][0] * k_scale, f1 = R.mul[nt][1] * k_scale;
@@ -105,7 +105,7 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
         }
         if (masked) {
             const int r = 8 * nt + 2 * c;
-            const int lim0 = all_see + r % a.n_q, lim1 = all_see + (r + 1) % a.n_q;
+            const int lim0 = all_see + (a.n_q == 1 ? 0 : r % a.n_q), lim1 = all_see + (a.n_q == 1 ? 0 : (r + 1) % a.n_q);
 #pragma unroll
             for (int j = 0; j < SUB; ++j) {
                 float* x = s[j][nt];
@@ -196,38 +196,47 @@ __device__ __forceinline__ int clipped_length(const Kv8AttnArgs& a, int b) {
 struct Share {
     long long units;                // of all sequences and heads
     int ctas;                       // that get some: every warp of one a unit, as far as there are
+    // of sequence `lane`, for batches of up to 32: tokens, units of a head, units of a head of it and those before
+    int n, per, upto;
 };
 template <int W>
 __device__ __forceinline__ Share share_of(const Kv8AttnArgs& a, bool report) {
-    const int pairs = a.c.batch * a.c.heads;
-    long long units = 0;
+    const int pairs = a.c.batch * a.c.heads, lane = threadIdx.x & 31;
+    Share s{};
     bool same = true;               // sequences of one length
     if (!a.lengths) {
-        units = (long long)pairs * units_of<W>(a.length_all);
+        s.units = (long long)pairs * units_of<W>(a.length_all);
     } else {
-        const int lane = threadIdx.x & 31, first = units_of<W>(clipped_length(a, 0));
+        int first = 0;
         for (int b0 = 0; b0 < a.c.batch; b0 += 32) {
-            int x = 0;
-            if (b0 + lane < a.c.batch) {
-                const int n = clipped_length(a, b0 + lane);
-                if (report && threadIdx.x < 32 && n != a.lengths[b0 + lane]) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
-                x = units_of<W>(n);
-                same = same && x == first;
+            s.n = s.per = 0;
+            const bool there = b0 + lane < a.c.batch;
+            if (there) {
+                const int n = a.lengths[b0 + lane];
+                s.n = max(0, min(n, a.max_length));
+                s.per = units_of<W>(s.n);
+                if (report && threadIdx.x < 32 && n != s.n) atomicOr(a.c.status + MINF_ST_ERROR, MINF_ERR_KV8_RANGE);
             }
+            if (b0 == 0) first = __shfl_sync(0xffffffffu, s.per, 0);
+            same = same && (!there || s.per == first);
+            s.upto = s.per;         // below 2^31: 32 sequences of at most 2^25 units and a tail
 #pragma unroll
-            for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-            units += x;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, s.upto, o);
+                if (lane >= o) s.upto += y;
+            }
+            s.units += __shfl_sync(0xffffffffu, s.upto, 31);
         }
         same = __all_sync(0xffffffffu, same);
-        units *= a.c.heads;
+        s.units *= a.c.heads;
     }
-    int ctas = a.splits;
-    if (a.single) return {units, pairs};            // (not looked at: CTA i has head i)
+    s.ctas = a.splits;
+    if (a.single) return s;         // CTA i has head i
     // a whole number of CTAs per head where that leaves few of them idle: then none works on two pieces, which costs it a new
-    // start and a second joining (about 5 us)
-    if (same && pairs <= ctas && ctas / pairs * pairs * 10 >= ctas * 9) ctas = ctas / pairs * pairs;
-    if (units < (long long)ctas * W) ctas = (int)((units + W - 1) / W);
-    return {units, ctas};
+    // start and a second joining
+    if (same && pairs <= s.ctas && s.ctas / pairs * pairs * 10 >= s.ctas * 9) s.ctas = s.ctas / pairs * pairs;
+    if (s.units < (long long)s.ctas * W) s.ctas = (int)((s.units + W - 1) / W);
+    return s;
 }
 // x * y / z of non-negative numbers; 64-bit division takes a few hundred cycles, so it is left to products that need it
 __device__ __forceinline__ long long mul_div(long long x, int y, long long z) {
@@ -241,7 +250,7 @@ __device__ __forceinline__ long long owner_of(long long unit, long long units, i
 }
 
 template <int W>
-__device__ __forceinline__ Place locate(const Kv8AttnArgs& a, long long at) {
+__device__ __forceinline__ Place locate(const Kv8AttnArgs& a, const Share& share, long long at) {
     const int lane = threadIdx.x & 31;
     if (!a.lengths) {
         const int per = units_of<W>(a.length_all);
@@ -249,40 +258,51 @@ __device__ __forceinline__ Place locate(const Kv8AttnArgs& a, long long at) {
         return {bh / a.c.heads, bh % a.c.heads, (int)(at - (long long)bh * per), a.length_all};
     }
     for (int b0 = 0;; b0 += 32) {
-        const int n = b0 + lane < a.c.batch ? clipped_length(a, b0 + lane) : 0;
-        const long long mine = (long long)units_of<W>(n) * a.c.heads;
-        long long upto = mine;
+        int n = share.n, per = share.per, upto = share.upto;
+        if (a.c.batch > 32) {                       // the share has the last 32 only
+            n = b0 + lane < a.c.batch ? clipped_length(a, b0 + lane) : 0;
+            upto = per = units_of<W>(n);
 #pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const long long y = __shfl_up_sync(0xffffffffu, upto, o);
-            if (lane >= o) upto += y;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(0xffffffffu, upto, o);
+                if (lane >= o) upto += y;
+            }
         }
-        const unsigned here = __ballot_sync(0xffffffffu, at < upto);
+        const unsigned here = __ballot_sync(0xffffffffu, at < (long long)upto * a.c.heads);
         if (here) {
             const int src = __ffs(here) - 1;
-            const int nb = __shfl_sync(0xffffffffu, n, src);
-            const long long rest = at - __shfl_sync(0xffffffffu, upto - mine, src);        // within the sequence's heads
-            const int per = units_of<W>(nb);
-            const int head = (int)mul_div(rest, 1, per);
-            return {b0 + src, head, (int)(rest - (long long)head * per), nb};
+            const int nb = __shfl_sync(0xffffffffu, n, src), pb = __shfl_sync(0xffffffffu, per, src), ub = __shfl_sync(0xffffffffu, upto, src);
+            const long long rest = at - (long long)(ub - pb) * a.c.heads;       // within the sequence's heads
+            const int head = (int)mul_div(rest, 1, pb);
+            return {b0 + src, head, (int)(rest - (long long)head * pb), nb};
         }
         if (b0 + 32 >= a.c.batch) return {0, 0, 0, 0};          // (not reached: `at` is below the total)
-        at -= __shfl_sync(0xffffffffu, upto, 31);
+        at -= (long long)__shfl_sync(0xffffffffu, upto, 31) * a.c.heads;
     }
 }
-// units before sequence b
+// units of a head of sequence b, and of all heads of the sequences before it
 template <int W>
-__device__ __forceinline__ long long units_before(const Kv8AttnArgs& a, int b) {
-    if (!a.lengths) return (long long)b * a.c.heads * units_of<W>(a.length_all);
+__device__ __forceinline__ void units_before(const Kv8AttnArgs& a, const Share& share, int b, int& per, long long& before) {
+    if (!a.lengths) {
+        per = units_of<W>(a.length_all);
+        before = (long long)b * a.c.heads * per;
+        return;
+    }
+    if (a.c.batch <= 32) {
+        per = __shfl_sync(0xffffffffu, share.per, b);
+        before = (long long)(__shfl_sync(0xffffffffu, share.upto, b) - per) * a.c.heads;
+        return;
+    }
     const int lane = threadIdx.x & 31;
-    long long sum = 0;
+    per = units_of<W>(clipped_length(a, b));
+    before = 0;
     for (int b0 = 0; b0 < b; b0 += 32) {
         int x = b0 + lane < b ? units_of<W>(clipped_length(a, b0 + lane)) : 0;
 #pragma unroll
         for (int o = 16; o; o >>= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
-        sum += x;
+        before += x;
     }
-    return sum * a.c.heads;
+    before *= a.c.heads;
 }
 
 template <int FMT, int NT, bool LOGITS>
@@ -303,7 +323,7 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
 #pragma unroll 1
     while (at < stop) {                             // a piece: units of one sequence and head
     const Place place = a.single ? Place{(int)blockIdx.x / a.c.heads, (int)blockIdx.x % a.c.heads, 0, clipped_length(a, blockIdx.x / a.c.heads)}
-                                 : locate<kAttnWarps>(a, at);
+                                 : locate<kAttnWarps>(a, share, at);
     const int h = place.h, b = place.b, n = place.n;
     const size_t bh = (size_t)b * a.c.heads + h;
     const int full = n / kKv8Block;                 // complete blocks
@@ -354,52 +374,59 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     }
     cp_async_commit();
 
-    // Q^T fragments: column g of group nt, dims of step s: 64 (s / 4) + 16 c + 4 (s % 4) + {0, 1 | 2, 3}
+    // Q^T fragments: column g of group nt, dims of step s: 64 (s / 4) + 16 c + 4 (s % 4) + {0, 1 | 2, 3}.  Where they are
+    // shared, warp nt makes those of group nt.
     Rows<NT> R;
     uint32_t qf[kQShared ? 1 : NT][8][2];
     uint2* const q_sm = reinterpret_cast<uint2*>(ring_all + kRingBytes);        // [nt][step][lane]
-    float q_unit[NT];                               // power of two the row was divided by
-    // eight dims of row 8 nt + g from dim d on (zeros behind the last row)
-    auto q_load = [&](int nt, int d, float (&v)[8]) {
-        const int r = 8 * nt + g;
-        uint4 x = make_uint4(0u, 0u, 0u, 0u);
-        if (r < a.rows) x = *reinterpret_cast<const uint4*>(a.q + b * a.qs[0] + (long long)(h * a.group + r / a.n_q) * a.qs[1] + (long long)(r % a.n_q) * a.qs[2] + d);
-        bf16x8_to_values(x, v);
-    };
+    float* const unit_sm = reinterpret_cast<float*>(ring_all + kRingBytes + NT * 2048);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        float top = 0.f;
-        float x[4][8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            q_load(nt, 64 * (i >> 1) + 16 * c + 8 * (i & 1), x[i]);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float m = fabsf(x[i][e]);
-                if (m < CUDART_INF_F) top = fmaxf(top, m);
+        float unit = 1.f;                           // power of two the row was divided by
+        if (!kQShared || warp == nt) {
+            const int r = 8 * nt + g;
+            const uint4* q = nullptr;
+            if (r < a.rows) {
+                const int hq = h * a.group + (a.n_q == 1 ? r : r / a.n_q), t = a.n_q == 1 ? 0 : r % a.n_q;
+                q = reinterpret_cast<const uint4*>(a.q + b * a.qs[0] + (long long)hq * a.qs[1] + (long long)t * a.qs[2]);
             }
+            float top = 0.f;
+            float x[4][8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {           // eight dims from 64 (i / 2) + 16 c + 8 (i % 2) on; zeros behind the last row
+                bf16x8_to_values(q ? q[8 * (i >> 1) + 2 * c + (i & 1)] : make_uint4(0u, 0u, 0u, 0u), x[i]);
+#pragma unroll
+                for (int e = 0; e < 8; ++e) {
+                    const float m = fabsf(x[i][e]);
+                    if (m < CUDART_INF_F) top = fmaxf(top, m);
+                }
+            }
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+            int e = 0;
+            if (top > 0.f) frexpf(top, &e);         // top < 2^e: scaled to below 2^8, so that the smallest products count too
+            e = max(e - 8, -126);
+            const float inv = __uint_as_float((uint32_t)(127 - e) << 23);
+            unit = __uint_as_float((uint32_t)(127 + e) << 23);
+#pragma unroll
+            for (int st = 0; st < 8; ++st) {
+                const float* v = &x[st >> 1][4 * (st & 1)];
+                const uint32_t b0 = pack_half2(v[0] * inv, v[1] * inv), b1 = pack_half2(v[2] * inv, v[3] * inv);
+                if constexpr (kQShared) {
+                    q_sm[(nt * 8 + st) * 32 + lane] = make_uint2(b0, b1);
+                } else {
+                    qf[nt][st][0] = b0;
+                    qf[nt][st][1] = b1;
+                }
+            }
+            if (kQShared && c == 0) unit_sm[8 * nt + g] = unit;
         }
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-        top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-        int e = 0;
-        if (top > 0.f) frexpf(top, &e);             // top < 2^e: scaled to below 2^8, so that the smallest products count too
-        e = max(min(e - 8, 100), -100);
-        const float inv = exp2f((float)-e);
-        q_unit[nt] = exp2f((float)e);
+        if constexpr (!kQShared) {
 #pragma unroll
-        for (int st = 0; st < 8; ++st) {
-            const float* v = &x[st >> 1][4 * (st & 1)];
-            const uint32_t b0 = pack_half2(v[0] * inv, v[1] * inv), b1 = pack_half2(v[2] * inv, v[3] * inv);
-            if constexpr (kQShared) {
-                if (warp == 0) q_sm[(nt * 8 + st) * 32 + lane] = make_uint2(b0, b1);
-            } else {
-                qf[nt][st][0] = b0;
-                qf[nt][st][1] = b1;
-            }
+            for (int cc = 0; cc < 2; ++cc) R.mul[nt][cc] = a.scale_log2 * __shfl_sync(0xffffffffu, unit, 4 * (2 * c + cc));
         }
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-            R.mul[nt][cc] = a.scale_log2 * __shfl_sync(0xffffffffu, q_unit[nt], 4 * (2 * c + cc));
             R.m[nt][cc] = -CUDART_INF_F;
             R.l[nt][cc] = 0.f;
         }
@@ -408,7 +435,14 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
 #pragma unroll
             for (int k = 0; k < 4; ++k) R.o[nt][i][k] = 0.f;
     }
-    if (kQShared) __syncthreads();
+    if constexpr (kQShared) {
+        static_assert(NT <= kAttnWarps, "a warp for each group");
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+            for (int cc = 0; cc < 2; ++cc) R.mul[nt][cc] = a.scale_log2 * unit_sm[8 * nt + 2 * c + cc];
+    }
     auto q_frag = [&](int nt, int st) {
         if constexpr (kQShared) return q_sm[(nt * 8 + st) * 32 + lane];
         else return make_uint2(qf[nt][st][0], qf[nt][st][1]);
@@ -525,17 +559,19 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
         for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
             for (int e = 0; e < 4; ++e) s[0][nt][e] = 0.f;
+        auto to_bf16 = [](uint32_t x) {             // (eight bits of them at most: exact, but for what f16 has lost already)
+            const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&x));
+            return pack_bf16x2(f.x, f.y);
+        };
 #pragma unroll
         for (int i = 0; i < 4; ++i) {               // 16 dims of a lane quad: two steps
             const int d = 64 * (i >> 1) + 16 * c + 8 * (i & 1);
             const uint4 x = *reinterpret_cast<const uint4*>(kt + g * kKv8Dim + d), y = *reinterpret_cast<const uint4*>(kt + (g + 8) * kKv8Dim + d);
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt) {
-                float v[8];
-                q_load(nt, d, v);
-                const float inv = 1.f / q_unit[nt];
-                mma_bf16(s[0][nt], x.x, y.x, x.y, y.y, pack_bf16x2(v[0] * inv, v[1] * inv), pack_bf16x2(v[2] * inv, v[3] * inv));
-                mma_bf16(s[0][nt], x.z, y.z, x.w, y.w, pack_bf16x2(v[4] * inv, v[5] * inv), pack_bf16x2(v[6] * inv, v[7] * inv));
+                const uint2 q0 = q_frag(nt, 2 * i), q1 = q_frag(nt, 2 * i + 1);
+                mma_bf16(s[0][nt], x.x, y.x, x.y, y.y, to_bf16(q0.x), to_bf16(q0.y));
+                mma_bf16(s[0][nt], x.z, y.z, x.w, y.w, to_bf16(q1.x), to_bf16(q1.y));
             }
         }
         // tokens behind the last one must not count: no row sees them (all_see + n_q - 1 = n)
@@ -584,75 +620,90 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     // Join the warps, eight rows at a time.  In units that some row does not see to their end and in the tail, values that
     // are infinite or NaN were left out of the products (zero times them would not be zero) and are added here to the rows that see them.
     const bool any_bad = __syncthreads_or(bad);     // (and the rings are read out)
-    float (*sm_o)[8][kKv8Dim] = reinterpret_cast<float (*)[8][kKv8Dim]>(ring_all);
-    float (*sm_lse)[8] = reinterpret_cast<float (*)[8]>(ring_all + kAttnWarps * 8 * kKv8Dim * sizeof(float));
+    constexpr int kRows = 8 * NT;
+    float (*sm_o)[kRows][kKv8Dim] = reinterpret_cast<float (*)[kRows][kKv8Dim]>(ring_all);
+    static_assert(kAttnWarps * kRows * kKv8Dim * sizeof(float) <= kRingBytes, "the warps' outputs fit the rings");
+    __shared__ float2 sm_ml[kAttnWarps][kRows];     // maximum and denominator; then the warp's weight
 #pragma unroll
-    for (int nt = 0; nt < NT; ++nt) {
+    for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
             float l = R.l[nt][cc];
 #pragma unroll
             for (int o = 4; o < 32; o <<= 1) l += __shfl_xor_sync(0xffffffffu, l, o);
-            const float inv = l == 0.f ? 0.f : 1.f / l;
-            if (g == 0) sm_lse[warp][2 * c + cc] = l == 0.f ? -CUDART_INF_F : (R.m[nt][cc] == -CUDART_INF_F ? l : R.m[nt][cc] + log2f(l));
-            float* dst = &sm_o[warp][2 * c + cc][16 * g];
+            const int r = 8 * nt + 2 * c + cc;
+            if (g == 0) sm_ml[warp][r] = make_float2(R.m[nt][cc], l);
+            float* dst = &sm_o[warp][r][16 * g];
 #pragma unroll
             for (int i = 0; i < 4; ++i)
-                *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(R.o[nt][2 * i][cc] * inv, R.o[nt][2 * i][2 + cc] * inv,
-                                                                      R.o[nt][2 * i + 1][cc] * inv, R.o[nt][2 * i + 1][2 + cc] * inv);
+                *reinterpret_cast<float4*>(dst + 4 * i) = make_float4(R.o[nt][2 * i][cc], R.o[nt][2 * i][2 + cc], R.o[nt][2 * i + 1][cc], R.o[nt][2 * i + 1][2 + cc]);
         }
-        __syncthreads();
-#pragma unroll 1
-        for (int i = threadIdx.x; i < 8 * 32; i += kAttnThreads) {
-            const int rr = i >> 5, d = (i & 31) * 4, r = 8 * nt + rr;
-            if (r >= a.rows) continue;
-            float top = sm_lse[0][rr];
+    __syncthreads();
+    if (threadIdx.x < kRows) {                      // a row's log-sum-exp, and what each warp's output counts for in it
+        const int r = threadIdx.x;
+        float lse[kAttnWarps], l[kAttnWarps], top = -CUDART_INF_F;
 #pragma unroll
-            for (int w = 1; w < kAttnWarps; ++w) top = fmaxf(top, sm_lse[w][rr]);
-            float sum = 0.f;
-            float acc[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int w = 0; w < kAttnWarps; ++w) {
+            const float2 x = sm_ml[w][r];
+            l[w] = x.y;
+            lse[w] = x.y == 0.f ? -CUDART_INF_F : x.x == -CUDART_INF_F ? x.y : x.x + log2f(x.y);
+            top = fmaxf(top, lse[w]);
+        }
+        float sum = 0.f;
 #pragma unroll
-            for (int w = 0; w < kAttnWarps; ++w) {
-                const float e = sm_lse[w][rr];
-                if (e == -CUDART_INF_F) continue;
-                const float f = exp2f(e - top);
-                const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][rr][d]);
-                sum += f;
-                acc[0] = fmaf(f, x.x, acc[0]);
-                acc[1] = fmaf(f, x.y, acc[1]);
-                acc[2] = fmaf(f, x.z, acc[2]);
-                acc[3] = fmaf(f, x.w, acc[3]);
-            }
-            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+        for (int w = 0; w < kAttnWarps; ++w) {
+            lse[w] = lse[w] == -CUDART_INF_F ? 0.f : exp2f(lse[w] - top);
+            sum += lse[w];
+        }
 #pragma unroll
-            for (int k = 0; k < 4; ++k) acc[k] *= inv;
-            if (any_bad) {
-                const int lo = max(u_lo * kUnit, min(max(all_see, 0) / kUnit * kUnit, full * kKv8Block)), lim = all_see + r % a.n_q;
-                const int hi = min(takes_tail ? n : u_hi * kUnit, lim);
-                for (int t = lo; t < hi; ++t)
-                    for (int k = 0; k < 4; ++k) {
-                        float v = 0.f;
-                        if (t >= full * kKv8Block)
-                            v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.c.v_tail)[(bh * kKv8Block + t % kKv8Block) * kKv8Dim + d + k]);
-                        else if (FMT == MINF_KV8_E4M3 && (static_cast<const uint8_t*>(a.c.v)[(bh * a.c.capacity + t) * kKv8Dim + d + k] & 0x7f) == 0x7f)
-                            v = CUDART_NAN_F;
-                        if (!(fabsf(v) < CUDART_INF_F)) acc[k] += v;
-                    }
-            }
-            const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
-            const size_t row = piece * a.rows + r;
-            if (d == 0) a.part_lse[row] = lse;
-            if (!whole) {
-                *reinterpret_cast<float4*>(a.part_o + row * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
-            } else {
-                const int hq = h * a.group + r / a.n_q, t = r % a.n_q;
-                __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
-                *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
-                if (d == 0 && a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = lse;
+        for (int w = 0; w < kAttnWarps; ++w) sm_ml[w][r].x = lse[w] == 0.f ? 0.f : lse[w] / (sum * l[w]);
+        const float all = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+        if (r < a.rows) {
+            a.part_lse[piece * a.rows + r] = all;
+            if (whole && a.lse) {
+                const int hq = h * a.group + r / a.n_q;
+                a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + r % a.n_q] = all;
             }
         }
-        __syncthreads();
     }
+    __syncthreads();
+#pragma unroll 1
+    for (int i = threadIdx.x; i < kRows * 32; i += kAttnThreads) {
+        const int r = i >> 5, d = (i & 31) * 4;
+        if (r >= a.rows) break;
+        float acc[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int w = 0; w < kAttnWarps; ++w) {
+            const float f = sm_ml[w][r].x;
+            if (f == 0.f) continue;                 // (its output may be anything times zero)
+            const float4 x = *reinterpret_cast<const float4*>(&sm_o[w][r][d]);
+            acc[0] = fmaf(f, x.x, acc[0]);
+            acc[1] = fmaf(f, x.y, acc[1]);
+            acc[2] = fmaf(f, x.z, acc[2]);
+            acc[3] = fmaf(f, x.w, acc[3]);
+        }
+        if (any_bad) {
+            const int lo = max(u_lo * kUnit, min(max(all_see, 0) / kUnit * kUnit, full * kKv8Block)), lim = all_see + r % a.n_q;
+            const int hi = min(takes_tail ? n : u_hi * kUnit, lim);
+            for (int t = lo; t < hi; ++t)
+                for (int k = 0; k < 4; ++k) {
+                    float v = 0.f;
+                    if (t >= full * kKv8Block)
+                        v = __bfloat162float(static_cast<const __nv_bfloat16*>(a.c.v_tail)[(bh * kKv8Block + t % kKv8Block) * kKv8Dim + d + k]);
+                    else if (FMT == MINF_KV8_E4M3 && (static_cast<const uint8_t*>(a.c.v)[(bh * a.c.capacity + t) * kKv8Dim + d + k] & 0x7f) == 0x7f)
+                        v = CUDART_NAN_F;
+                    if (!(fabsf(v) < CUDART_INF_F)) acc[k] += v;
+                }
+        }
+        if (!whole) {
+            *reinterpret_cast<float4*>(a.part_o + (piece * a.rows + r) * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+        } else {
+            const int hq = h * a.group + (a.n_q == 1 ? r : r / a.n_q), t = a.n_q == 1 ? 0 : r % a.n_q;
+            __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
+            *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
+        }
+    }
+    __syncthreads();                                // before the next piece's copies
     }
 }
 
@@ -667,13 +718,15 @@ __device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r
         return {(bh * a.rows + r) * a.splits, 1, a.splits};
     } else {
         const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
-        if (a.single) return {bh * a.rows + r, (size_t)a.rows, 1};
+        if (a.single) return {bh * a.rows + r, (size_t)a.rows, 1};     // as numbered there
         const Share share = share_of<W>(a, false);
         const long long all = share.units;
         const int ctas = share.ctas;
-        const int per = units_of<W>(a.lengths ? clipped_length(a, b) : a.length_all);
+        int per;
+        long long start;
+        units_before<W>(a, share, b, per, start);
         if (per == 0) return {0, 0, 0};
-        const long long start = units_before<W>(a, b) + (long long)h * per;
+        start += (long long)h * per;
         const long long lo = owner_of(start, all, ctas), hi = owner_of(start + per - 1, all, ctas);
         return {((size_t)lo + bh) * a.rows + r, (size_t)a.rows, (int)(hi - lo + 1)};
     }
@@ -920,7 +973,7 @@ static bool attention_sizes_ok(int batch, int hq, int heads, int n_q, int max_le
 
 template <int FMT, int NT, bool LOGITS>
 static cudaError_t launch_narrow(const Kv8AttnArgs& a, cudaStream_t stream) {
-    constexpr int bytes = narrow_warps(NT) * kRingSlots * kSlotBytes + (NT > 2 ? NT * 2048 : 0);
+    constexpr int bytes = narrow_warps(NT) * kRingSlots * kSlotBytes + (NT > 2 ? NT * 2048 + NT * 8 * sizeof(float) : 0);
     static std::atomic<unsigned long long> allowed{0};
     const cudaError_t e = allow_shared(kv8_attention_kernel<FMT, NT, LOGITS>, bytes, allowed);
     if (e != cudaSuccess) return e;

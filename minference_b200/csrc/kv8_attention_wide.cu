@@ -140,9 +140,9 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         }
         int e = 0;
         if (top > 0.f) frexpf(top, &e);
-        e = max(min(e - 8, 100), -100);
-        const float inv = a.scale_log2 < 0.f ? -exp2f((float)-e) : exp2f((float)-e);
-        ctl->unit[threadIdx.x] = exp2f((float)e);
+        e = max(e - 8, -126);
+        const float inv = __uint_as_float(((uint32_t)(127 - e) << 23) | (a.scale_log2 < 0.f ? 0x80000000u : 0u));
+        ctl->unit[threadIdx.x] = __uint_as_float((uint32_t)(127 + e) << 23);
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float v[8];
@@ -258,7 +258,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
                 for (int i = 0; i < kConvWarps; ++i) t = fmaxf(t, ctl->red[which][i]);
                 int e = 0;
                 if (t > 0.f) frexpf(t, &e);
-                ctl->tail_scale[which] = exp2f((float)max(min(e - 9, 100), -100));
+                ctl->tail_scale[which] = __uint_as_float((uint32_t)(127 + max(e - 9, -126)) << 23);
             }
             asm volatile("bar.sync %0, %1;" ::"r"(1 + which), "n"(kConvThreads) : "memory");
             if (lane == 0) mbar_arrive(bar(&ctl->tail_ready));
