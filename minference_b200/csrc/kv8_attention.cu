@@ -707,6 +707,18 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     }
 }
 
+// Loads that stay in their order before their uses, several in flight: the compiler may move plain ones to their uses.
+__device__ __forceinline__ float load_now(const float* p) {
+    float x;
+    asm volatile("ld.global.f32 %0, [%1];" : "=f"(x) : "l"(p) : "memory");
+    return x;
+}
+__device__ __forceinline__ float4 load_now4(const float* p) {
+    float4 x;
+    asm volatile("ld.global.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "l"(p) : "memory");
+    return x;
+}
+
 // Parts of a row: `count` of them, the first at row `base` of part_o / part_lse, `step` rows apart.
 struct Parts {
     size_t base, step;
@@ -741,16 +753,25 @@ __device__ __forceinline__ void join_row(const Kv8AttnArgs& a, const Parts& p, s
     for (int o = 16; o; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
     float sum = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-    for (int k = warp; k < p.count; k += WARPS) {
-        const float e = a.part_lse[p.base + k * p.step];
-        const float4 x = *reinterpret_cast<const float4*>(a.part_o + (p.base + k * p.step) * kKv8Dim + 4 * lane);
-        const float f = e == -CUDART_INF_F ? 0.f : exp2f(e - top);     // (a part that saw nothing holds zeros)
-        sum += f;
-        acc.x = fmaf(f, x.x, acc.x);
-        acc.y = fmaf(f, x.y, acc.y);
-        acc.z = fmaf(f, x.z, acc.z);
-        acc.w = fmaf(f, x.w, acc.w);
+    const float ref = top == -CUDART_INF_F ? 0.f : top;
+    for (int k0 = warp; k0 < p.count; k0 += 4 * WARPS) {
+        float e[4];
+        float4 x[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {               // (behind the last part: that one again, for nothing)
+            const size_t at = p.base + min(k0 + u * WARPS, p.count - 1) * p.step;
+            e[u] = load_now(a.part_lse + at);
+            x[u] = load_now4(a.part_o + at * kKv8Dim + 4 * lane);
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const float f = k0 + u * WARPS < p.count ? exp2f(e[u] - ref) : 0.f;        // (a part that saw nothing holds zeros)
+            sum += f;
+            acc.x = fmaf(f, x[u].x, acc.x);
+            acc.y = fmaf(f, x[u].y, acc.y);
+            acc.z = fmaf(f, x[u].z, acc.z);
+            acc.w = fmaf(f, x[u].w, acc.w);
+        }
     }
     if constexpr (WARPS > 1) {
         sm[warp][lane] = acc;
@@ -787,17 +808,25 @@ constexpr int kFinishCtas = 8 * kSMs;               // CTAs of that kind worth s
 
 // Weights of tokens [t0, t0 + kFinishTokens) of a head: the probabilities of its rows, summed in their order.  A thread has
 // four tokens, whose logits it reads together.
-__device__ __forceinline__ float weight_of(float logit, float lse) { return logit == -CUDART_INF_F ? 0.f : fast_exp2(logit - lse); }
+// (no condition in it: one per element kept the loads from being in flight together, sixteen times the time)
+__device__ __forceinline__ float weight_of(float logit, float lse) { return fast_exp2(logit - lse); }
+// a row that sees nothing has logits of -inf: 2^(-inf - 0) = 0
+__device__ __forceinline__ float for_weights(float lse) { return lse == -CUDART_INF_F ? 0.f : lse; }
 __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, int n, int t0, const float* row_lse) {
     constexpr int kEach = kFinishTokens / kFinishThreads;
     const size_t bh = (size_t)b * a.c.heads + h;
     const float* x = a.logits + ((long long)bh * a.tokens + t0 + threadIdx.x) * a.pitch;
     const float* add = a.add_to ? a.add_to + b * a.as[0] + h * a.as[1] + t0 + threadIdx.x : nullptr;
     const int left = n - t0 - (int)threadIdx.x;     // token k of this thread: k * kFinishThreads < left
+    if (left <= 0) return;
+    // behind the last token: an earlier one again, dropped at the end
+    long long row[kEach];
+#pragma unroll
+    for (int k = 0; k < kEach; ++k) row[k] = (long long)(k * kFinishThreads < left ? k : 0) * kFinishThreads;
     float was[kEach], sum[kEach];
 #pragma unroll
     for (int k = 0; k < kEach; ++k) {
-        was[k] = add && k * kFinishThreads < left ? add[k * kFinishThreads] : 0.f;
+        was[k] = add ? load_now(add + row[k]) : 0.f;
         sum[k] = 0.f;
     }
     int r = 0;
@@ -805,22 +834,22 @@ __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, 
         float4 l[kEach];
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
-            l[k] = k * kFinishThreads < left ? *reinterpret_cast<const float4*>(x + (long long)k * kFinishThreads * a.pitch + r)
-                                             : make_float4(-CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F, -CUDART_INF_F);
-        const float e0 = row_lse[r], e1 = r + 1 < a.rows ? row_lse[r + 1] : 0.f, e2 = r + 2 < a.rows ? row_lse[r + 2] : 0.f, e3 = r + 3 < a.rows ? row_lse[r + 3] : 0.f;
+            l[k] = load_now4(x + row[k] * a.pitch + r);
+        // rows behind the last: +inf, so that whatever their columns hold counts nothing
+        const float e0 = row_lse[r], e1 = r + 1 < a.rows ? row_lse[r + 1] : CUDART_INF_F, e2 = r + 2 < a.rows ? row_lse[r + 2] : CUDART_INF_F,
+                    e3 = r + 3 < a.rows ? row_lse[r + 3] : CUDART_INF_F;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
             sum[k] += weight_of(l[k].x, e0);
-            if (r + 1 < a.rows) sum[k] += weight_of(l[k].y, e1);
-            if (r + 2 < a.rows) sum[k] += weight_of(l[k].z, e2);
-            if (r + 3 < a.rows) sum[k] += weight_of(l[k].w, e3);
+            sum[k] += weight_of(l[k].y, e1);
+            sum[k] += weight_of(l[k].z, e2);
+            sum[k] += weight_of(l[k].w, e3);
         }
     }
     if (a.pitch == 2) {
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
-            if (k * kFinishThreads >= left) continue;
-            const float2 l = *reinterpret_cast<const float2*>(x + k * kFinishThreads * 2);
+            const float2 l = *reinterpret_cast<const float2*>(x + row[k] * 2);
             sum[k] += weight_of(l.x, row_lse[0]);
             if (a.rows > 1) sum[k] += weight_of(l.y, row_lse[1]);
         }
@@ -862,7 +891,7 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
                 }
 #pragma unroll
                 for (int o = 16; o; o >>= 1) sum += __shfl_xor_sync(0xffffffffu, sum, o);
-                if (lane == 0) sm_lse[r] = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+                if (lane == 0) sm_lse[r] = for_weights(sum == 0.f ? -CUDART_INF_F : top + log2f(sum));
             }
             __syncthreads();
             for (int t0 = chunk * a.chunk; t0 < min((long long)n, (chunk + 1ll) * a.chunk); t0 += kFinishTokens) sum_weights(a, b, h, n, t0, sm_lse);
@@ -883,36 +912,61 @@ __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid
     join_row<8>(a, p, bh * a.rows + r, warp, lane, sm, sm_sum);
 }
 
-// Weights after the wide kernel, whose rows' log-sum-exps are joined by then: a warp has sixteen tokens, its lanes the rows.
-constexpr int kWideTokens = 16 * kFinishThreads / 32;       // tokens of a CTA
-__global__ void __launch_bounds__(kFinishThreads) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
-    const int b = blockIdx.z, h = blockIdx.y, n = clipped_length(a, b), lane = threadIdx.x & 31;
-    const int t0 = (blockIdx.x * (kFinishThreads / 32) + (threadIdx.x >> 5)) * 16;
+// Weights after the wide kernel, whose rows' log-sum-exps are joined by then: a warp has eight tokens and takes 128 rows of
+// them at a time through shared memory, four a lane.  (With plain loads, which the compiler put next to their uses, 448 rows of
+// 8000 tokens took 104 us instead of 20.)
+constexpr int kWideTokensWarp = 8, kWeightThreads = 128, kWideTokens = kWideTokensWarp * kWeightThreads / 32;
+__global__ void __launch_bounds__(kWeightThreads) kv8_weights_kernel(const __grid_constant__ Kv8AttnArgs a) {
+    __shared__ __align__(16) float4 tile[kWeightThreads / 32][2][kWideTokensWarp][32];
+    const int b = blockIdx.z, h = blockIdx.y, n = clipped_length(a, b), lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int t0 = (blockIdx.x * (kWeightThreads / 32) + warp) * kWideTokensWarp;
     dependents_wait();
     if (t0 >= n) return;
     const size_t bh = (size_t)b * a.c.heads + h;
     const float* x = a.logits + ((long long)bh * a.tokens + t0) * a.pitch;
     const float* row_lse = a.row_lse + bh * a.rows;
-    float sum[16];
+    const int steps = (a.rows + 127) / 128;
+    auto fetch = [&](int i) {
+        const int r = 128 * i + 4 * lane;
+        if (i < steps && r < a.pitch) {             // (the pitch is a multiple of four here)
 #pragma unroll
-    for (int k = 0; k < 16; ++k) sum[k] = 0.f;
-    for (int r = lane; r < a.rows; r += 32) {
-        const float e = row_lse[r];
-        float l[16];
+            for (int k = 0; k < kWideTokensWarp; ++k)
+                if (t0 + k < n) cp_async_16(smem_u32(&tile[warp][i & 1][k][lane]), x + (long long)k * a.pitch + r);
+        }
+        cp_async_commit();
+    };
+    float sum[kWideTokensWarp];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) l[k] = t0 + k < n ? x[(long long)k * a.pitch + r] : -CUDART_INF_F;
+    for (int k = 0; k < kWideTokensWarp; ++k) sum[k] = 0.f;
+    fetch(0);
+    for (int i = 0; i < steps; ++i) {
+        fetch(i + 1);
+        const int r = 128 * i + 4 * lane;
+        float e[4];
 #pragma unroll
-        for (int k = 0; k < 16; ++k) sum[k] += weight_of(l[k], e);
+        for (int j = 0; j < 4; ++j) e[j] = r + j < a.rows ? for_weights(row_lse[r + j]) : 0.f;
+        cp_async_wait<1>();
+        __syncwarp();
+#pragma unroll
+        for (int k = 0; k < kWideTokensWarp; ++k) {
+            const float4 l = tile[warp][i & 1][k][lane];
+            const float w0 = weight_of(l.x, e[0]), w1 = weight_of(l.y, e[1]), w2 = weight_of(l.z, e[2]), w3 = weight_of(l.w, e[3]);
+            sum[k] += r < a.rows ? w0 : 0.f;        // columns behind the last row hold anything
+            sum[k] += r + 1 < a.rows ? w1 : 0.f;
+            sum[k] += r + 2 < a.rows ? w2 : 0.f;
+            sum[k] += r + 3 < a.rows ? w3 : 0.f;
+        }
+        __syncwarp();
     }
     float mine = 0.f;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) {
+    for (int k = 0; k < kWideTokensWarp; ++k) {
 #pragma unroll
         for (int o = 16; o; o >>= 1) sum[k] += __shfl_xor_sync(0xffffffffu, sum[k], o);
         if (lane == k) mine = sum[k];
     }
     const int t = t0 + lane;
-    if (lane < 16 && t < n) a.weights[b * a.ws[0] + h * a.ws[1] + t] = (a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f) + mine;
+    if (lane < kWideTokensWarp && t < n) a.weights[b * a.ws[0] + h * a.ws[1] + t] = (a.add_to ? a.add_to[b * a.as[0] + h * a.as[1] + t] : 0.f) + mine;
 }
 
 // ---------------------------------------------------------------------------------------------------- host
@@ -1080,7 +1134,7 @@ extern "C" int minf_kv8_attention(
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_finish_kernel failed: %s", cudaGetErrorString(e));
     }
     if (chunks) {
-        e = launch_behind(kv8_weights_kernel, dim3((unsigned)((max_length + kWideTokens - 1) / kWideTokens), cache->heads, cache->batch), kFinishThreads, 0, st, a);
+        e = launch_behind(kv8_weights_kernel, dim3((unsigned)((max_length + kWideTokens - 1) / kWideTokens), cache->heads, cache->batch), kWeightThreads, 0, st, a);
         if (e != cudaSuccess) return fail(MINF_E_CUDA, "launch of kv8_weights_kernel failed: %s", cudaGetErrorString(e));
     }
     return MINF_OK;

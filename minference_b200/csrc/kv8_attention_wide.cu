@@ -455,9 +455,14 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             auto numerators = [&](int c, int x, uint32_t (&sc)[32]) {
                 if (LOGITS && logits) {
                     float* to = logits + (long long)(t0 + 32 * c) * a.pitch;
+                    if (t0 + kWideTile <= min(n, lim)) {
 #pragma unroll
-                    for (int k = 0; k < 32; ++k)
-                        if (t0 + 32 * c + k < n) to[(long long)k * a.pitch] = 32 * c + k < seen ? __uint_as_float(sc[k]) * f[x] : -CUDART_INF_F;
+                        for (int k = 0; k < 32; ++k, to += a.pitch) *to = __uint_as_float(sc[k]) * f[x];
+                    } else {
+#pragma unroll
+                        for (int k = 0; k < 32; ++k, to += a.pitch)
+                            if (t0 + 32 * c + k < n) *to = 32 * c + k < seen ? __uint_as_float(sc[k]) * f[x] : -CUDART_INF_F;
+                    }
                 }
                 const float d = lv[x] - ref;
                 const uint64_t f2 = pack_f32x2(f[x], f[x]), d2 = pack_f32x2(d, d);
