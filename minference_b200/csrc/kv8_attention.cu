@@ -1086,7 +1086,9 @@ extern "C" int minf_kv8_attention(
         a.qs[i] = q_strides[i];
         a.os[i] = o_strides[i];
         if (o_strides[i] % 4) return fail(MINF_E_ARG, "output strides must be multiples of 4 elements");
+        if (q_strides[i] % 8) return fail(MINF_E_ARG, "query strides must be multiples of 8 elements");
     }
+    if (reinterpret_cast<uintptr_t>(q) & 15) return fail(MINF_E_ARG, "the queries must be 16-byte aligned");
     if (reinterpret_cast<uintptr_t>(o) & 7) return fail(MINF_E_ARG, "the output must be 8-byte aligned");
     a.group = hq / cache->heads;
     a.n_q = n_q;

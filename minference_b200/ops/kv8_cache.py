@@ -163,7 +163,7 @@ def _rows(t: torch.Tensor, what: str, cache: KV8Cache):
         _fail(f"{what} must be bf16 [{cache.batch}, heads, tokens, {HEAD_DIM}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
     s0, s1, s2, s3 = t.stride()
     if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15:
-        t = t.contiguous()
+        t = t.clone(memory_format=torch.contiguous_format)      # (contiguous() leaves a contiguous tensor at an odd address where it is)
     return t
 
 

@@ -109,3 +109,24 @@ def test_decode_layer_refusals(cabi):
     with pytest.raises(cabi.MInferB200Error):
         past.update(two[:1], two[:1], 0)                    # CPU tensors
     assert past.get_seq_length() == 0
+
+
+def test_attention_refuses_misaligned_queries(cabi):
+    lib, d = cabi.lib(), ctypes.byref(_desc(cabi))
+    st, odd = (ctypes.c_int64 * 3)(512, 128, 128), (ctypes.c_int64 * 3)(512, 132, 128)
+    for q, qs, word in [(264, st, b"aligned"), (256, odd, b"strides")]:
+        rc = lib.minf_kv8_attention(d, q, qs, 256, st, 4, 1, None, 100, 128, 1.0, None, None, None, None, None, 256, None)
+        assert rc == -1 and b"quer" in lib.minf_last_error() and word in lib.minf_last_error(), lib.minf_last_error()
+
+
+def test_misaligned_tensors_are_copied(cabi):
+    """A contiguous view at an odd address, and one whose stride along a dimension of size one is odd."""
+    from types import SimpleNamespace
+
+    from minference_b200.ops import kv8_cache
+
+    cache = SimpleNamespace(batch=1, device=torch.device("cpu"))
+    buf = torch.arange(2 * 128 + 8).to(torch.bfloat16)
+    for t in (buf[1:257].view(1, 2, 1, 128), buf[:256].as_strided((1, 2, 1, 128), (129, 128, 3, 1))):
+        r = kv8_cache._rows(t, "query", cache)
+        assert torch.equal(r, t) and r.data_ptr() % 16 == 0 and not any(s % 8 for s in r.stride()[:3])
