@@ -636,3 +636,125 @@ def test_on_another_stream():
             results.append((out, w[..., :1000], w2, kept, *kv8_load(small, n, count=333)))
         stream.synchronize()
     assert all(torch.equal(a, b) for a, b in zip(*results))
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_many_sequences(kind):
+    """More sequences than a warp has lanes, lengths of every sort among them, in the narrow and the wide kernel."""
+    gen = torch.Generator().manual_seed(41)
+    lengths = [(37 * i * i) % 500 for i in range(70)]
+    lengths[3] = lengths[32] = lengths[33] = lengths[69] = 0
+    lengths[31], lengths[64] = 6000, 4999
+    cache, ref = _filled(gen, 70, 1, lengths, kind)
+    _check_attention(cache, ref, lengths, 1, 4, gen, weights=True)
+    _check_attention(cache, ref, lengths, 5, 4, gen)
+    _check_attention(cache, ref, lengths, 33, 1, gen, weights=True)
+    same = [1000] * 40
+    cache, ref = _filled(gen, 40, 2, same, kind)
+    _check_attention(cache, ref, same, 1, 4, gen)
+    _check_attention(cache, ref, same, 1, 4, gen, as_int=True, weights=True)
+
+
+@pytest.mark.parametrize("s, hq", [(1, 4), (5, 8), (40, 2)])
+def test_one_length_for_a_batch(s, hq):
+    gen = torch.Generator().manual_seed(42)
+    cache, ref = _filled(gen, 3, 2, [3011] * 3, torch.float8_e4m3fn)
+    _check_attention(cache, ref, [3011] * 3, s, hq, gen, as_int=True, weights=True)
+    _check_attention(cache, ref, [3011] * 3, s, hq, gen, as_int=True, max_length=3050)
+
+
+def test_only_empty_sequences():
+    from minference_b200 import kv8_attention, kv8_evict
+
+    gen = torch.Generator().manual_seed(43)
+    cache = _poisoned(2, 2, 2048, torch.float8_e4m3fn)
+    n = torch.zeros(2, dtype=torch.int32, device="cuda")
+    for s in (1, 5, 64):
+        _, dq = _rows(gen, 2, 4, s)
+        w = torch.full((2, 2, 2048), -3.0, device="cuda")
+        for lengths in (n, 0):
+            out, lse = kv8_attention(dq, cache, lengths, max_length=2048, weights=w, return_lse=True)
+            assert not out.any() and (lse == -math.inf).all() and (w == -3.0).all()
+    small, m, w2, kept = kv8_evict(cache, n, torch.full((2, 2, 2048), NAN, device="cuda"), 100, recent=10)
+    assert m.tolist() == [0, 0] and not w2.any() and (kept == -1).all()
+    cache.check()
+
+
+def test_misaligned_inputs():
+    from minference_b200 import KV8Cache, kv8_attention, kv8_load, kv8_store
+
+    gen = torch.Generator().manual_seed(44)
+    raw = torch.randn(2 * 300 * 128 + 1, generator=gen).to(torch.bfloat16).cuda()
+    k = raw[1:].view(1, 2, 300, 128)
+    q = raw[1:1 + 8 * 128].view(1, 8, 1, 128)
+    assert k.is_contiguous() and k.data_ptr() % 16 and q.data_ptr() % 16
+    outs = []
+    for kk, qq in ((k, q), (k.clone(), q.clone())):
+        cache = KV8Cache.empty(1, 2, 300)
+        kv8_store(cache, kk, kk, 0)
+        outs.append((*kv8_load(cache, 300), kv8_attention(qq, cache, 300)))
+    assert all(torch.equal(a, b) for a, b in zip(*outs))
+
+
+@pytest.mark.parametrize("s, hq", [(1, 8), (40, 8)])
+def test_attention_and_eviction_in_a_cuda_graph(s, hq):
+    """Captured attention of either kernel with weights, and the eviction behind it, replayed for other lengths."""
+    from minference_b200 import KV8Cache, kv8_attention, kv8_evict, kv8_load
+
+    gen = torch.Generator().manual_seed(45)
+    cache, _ = _filled(gen, 2, 2, [4096, 4096], torch.int8)
+    _, dq = _rows(gen, 2, hq, s)
+    n = torch.tensor([4096, 4096], dtype=torch.int32, device="cuda")
+    out_cache = KV8Cache.empty(2, 2, 700, torch.int8)
+
+    def step():
+        w = torch.zeros(2, 2, 4096, device="cuda")
+        out = kv8_attention(dq, cache, n, max_length=4096, weights=w)
+        small, m, w2, kept = kv8_evict(cache, n, w, 700, recent=64, sink=4, max_length=4096, out=out_cache)
+        return out, w, m, w2, kept, *kv8_load(small, m)
+
+    step()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g, stream=side):
+        got = step()
+    # lengths inside a block read a tail that holds another block's tokens, here NaN: the same numbers all the same
+    for lengths in ([4096, 4096], [2944, 704], [0, 64], [3001, 701], [777, 2222]):
+        n.copy_(torch.tensor(lengths, dtype=torch.int32))
+        want = [t.clone() for t in step()]
+        for t in got[:2]:
+            t.zero_()
+        out_cache.k.view(torch.uint8).zero_(), out_cache.v_tail.zero_()
+        g.replay()
+        torch.cuda.synchronize()
+        for a, b in zip(want, got):
+            torch.testing.assert_close(a, b, rtol=0, atol=0, equal_nan=True)
+    cache.check()
+
+
+@pytest.mark.parametrize("s", [1, 40])
+def test_two_streams_read_one_cache(s):
+    """Calls that overlap in time share no scratch memory."""
+    from minference_b200 import kv8_attention
+
+    gen = torch.Generator().manual_seed(46)
+    cache, _ = _filled(gen, 2, 4, [9000, 7000], torch.float8_e4m3fn)
+    n = torch.tensor([9000, 7000], dtype=torch.int32, device="cuda")
+    qs = [_rows(gen, 2, 8, s)[1] for _ in range(2)]
+    new = lambda: torch.zeros(2, 4, cache.capacity, device="cuda")
+    want = []
+    for q in qs:
+        w = new()
+        want.append((kv8_attention(q, cache, n, weights=w), w))
+    streams = [torch.cuda.Stream() for _ in qs]
+    got = [[], []]
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                w = new()
+                got[i].append((kv8_attention(qs[i], cache, n, weights=w), w))
+    torch.cuda.synchronize()
+    for i in range(2):
+        assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))

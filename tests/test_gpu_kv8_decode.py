@@ -141,7 +141,7 @@ def test_prompt_weights_are_the_estimators_scores():
     p = torch.softmax((q[:, :, -64:].double() @ k.double().repeat_interleave(2, 1).transpose(2, 3) / 128 ** 0.5).masked_fill(
         torch.arange(300)[None, :] > torch.arange(236, 300)[:, None], -math.inf), -1)
     want = p.sum(2).view(1, 2, 2, 300).sum(2)
-    # the estimator rounds its logits to bf16 twice (product and division): 2 * 2^-9 of logits up to their largest magnitude
+    # the estimator rounds its logits to bf16 twice (product and division): 2 * 2^-8 of logits up to their largest magnitude
     top = (q[:, :, -64:].double() @ k.double().repeat_interleave(2, 1).transpose(2, 3) / 128 ** 0.5).abs().max().item()
     rel = 2 * (math.exp(2 * 2.0 ** -8 * top) - 1)
     assert ((w.cpu().double() - want).abs() <= rel * want + 1e-6).all()
@@ -182,3 +182,18 @@ def test_hugging_face_model(tmp_path, monkeypatch):
 
     with pytest.raises(cabi.MInferB200Error):
         past.crop(5)
+
+
+@pytest.mark.parametrize("n", [1, 2, 40, 64, 65, 130])
+def test_short_prompts_with_a_budget(tiny, n):
+    """Prompts shorter than the estimator's 64 queries and around the budget, then decoding past it."""
+    shape, model, ids = tiny
+    kv = model.new_kv(budget=64, recent=16, slack=8, dtype=torch.int8)
+    model.prefill(ids[:n], DENSE, kv=kv)
+    assert all(x.seen == n and x.held == min(n, 64) for x in kv)
+    for x in kv:                # four heads' 64 queries at most, each with probabilities that sum to one (2^-7: should they be bf16)
+        held = x.sums[..., : x.held].sum(-1)
+        assert (held <= 4 * min(n, 64) * (1 + 2.0 ** -7)).all() and (n > 64 or (held >= 4 * n * (1 - 2.0 ** -7)).all())
+    for t in range(80):
+        assert torch.isfinite(model.decode(torch.tensor([t]), kv)).all()
+    assert all(x.seen == n + 80 and x.held < 64 + 8 for x in kv)
