@@ -3,7 +3,7 @@
 // For a row (query head, query token) with logits l_t = sm_scale log2(e) s_K,t (q . c_K,t) over the tokens it sees,
 //   out = sum_t 2^(l_t - lse) s_V,t c_V,t,    lse = log2 sum_t 2^l_t
 // in one pass over the cache.  The running maximum M is that of l_t + log2 s_V,t, so the numerators
-// P_t = 2^(l_t + log2 s_V,t - M) are at most 1 and multiply the codes as they are, whatever the scales; the
+// P_t = 2^(l_t + log2 s_V,t - M) are at most 2^8 (M follows jumps beyond that only) and multiply the codes as they are, whatever the scales; the
 // denominator is the sum over blocks of (sum P_t) / s_V.
 //
 // The products run on the tensor cores with the tokens as rows: S^T = K Q^T and O^T = V^T P^T, m16n8k16 in f16 with
@@ -13,10 +13,15 @@
 // half a step of 2^-11 relative, below the bf16 rounding of the output; sums and outputs are accumulated in fp32.
 // The tail (bf16) takes bf16 products, with P as a sum of two bf16 numbers.
 //
-// The tokens are split over CTAs and, inside one, over warps by units of 32; the parts are joined by their log-sum-exps in a
-// second kernel, launched behind the first one's end.
+// The tokens are split over CTAs and, inside one, over warps by units of 32.  Parts are joined by their log-sum-exps: short
+// sequences' inside a cluster, others' in a second kernel, launched behind the first one's end.
+//
+// Bound: HBM.  Decoding steps of 4 rows per head read 131072 tokens of 8 heads in 45 us (5.9 TB/s; 51 us with the second
+// kernel), 1048576 tokens in 310 us (6.9 TB/s), issue slots 46 % and tensor pipe 18 % busy.  Up to 16 rows take 57 us, up to 24
+// 75 us: there it is the chain of each warp (three warps a scheduler instead of two change nothing).
 #include "kv8_attention.cuh"
 
+#include <cooperative_groups.h>
 #include <math_constants.h>
 
 #include <algorithm>
@@ -31,6 +36,7 @@ constexpr int kRingSlots = 3;
 // Rows per cache head this kernel takes; more go to the wide one.  At 131072 tokens of 8 heads (e4m3, device time): 24 rows 76 us
 // here and 85 us there, 32 rows (a fourth group, since removed) 97 and 90; four sequences of 16384: 32 rows 78 and 57.
 constexpr int kNarrowRows = 24;
+constexpr int kMaxCluster = 8;
 // warps of a CTA: two CTAs fit an SM with 128 registers a thread for one group of rows, twice that for more
 __host__ __device__ constexpr int narrow_warps(int nt) { return nt == 1 ? 8 : 4; }
 
@@ -177,7 +183,7 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
     }
 }
 
-// How the narrow kernel's CTAs share the work: the tokens of all sequences and heads are one row of units, (sequence, head,
+// How the narrow kernel's CTAs share the work of long sequences: the tokens of all sequences and heads are one row of units, (sequence, head,
 // unit) in that order, and CTA i of N takes the units [U i / N, U (i + 1) / N).  Sequences of any lengths keep every CTA
 // equally busy; where a CTA's share crosses into another head or sequence, it works on pieces one after the other.  The
 // tail counts as a unit for each of the W warps.  Every CTA finds its place from the lengths by itself (a warp scans 32
@@ -231,7 +237,6 @@ __device__ __forceinline__ Share share_of(const Kv8AttnArgs& a, bool report) {
         s.units *= a.c.heads;
     }
     s.ctas = a.splits;
-    if (a.single) return s;         // CTA i has head i
     // a whole number of CTAs per head where that leaves few of them idle: then none works on two pieces, which costs it a new
     // start and a second joining
     if (same && pairs <= s.ctas && s.ctas / pairs * pairs * 10 >= s.ctas * 9) s.ctas = s.ctas / pairs * pairs;
@@ -314,26 +319,38 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     extern __shared__ __align__(128) unsigned char ring_all[];
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5, g = lane >> 2, c = lane & 3;
     dependents_launch();
-    const Share share = share_of<kAttnWarps>(a, blockIdx.x == 0);
-    const long long all_units = share.units;
-    const int ctas = share.ctas;
-    if ((int)blockIdx.x >= ctas) return;
-    long long at = a.single ? 0 : mul_div(all_units, blockIdx.x, ctas);
-    const long long stop = a.single ? 1 : mul_div(all_units, blockIdx.x + 1, ctas);
+    Share share{};
+    long long at = 0, stop = 1;                     // a cluster per head: one piece
+    if (!a.cluster) {
+        share = share_of<kAttnWarps>(a, blockIdx.x == 0);
+        if ((int)blockIdx.x >= share.ctas) return;
+        at = mul_div(share.units, blockIdx.x, share.ctas);
+        stop = mul_div(share.units, blockIdx.x + 1, share.ctas);
+    }
 #pragma unroll 1
     while (at < stop) {                             // a piece: units of one sequence and head
-    const Place place = a.single ? Place{(int)blockIdx.x / a.c.heads, (int)blockIdx.x % a.c.heads, 0, clipped_length(a, blockIdx.x / a.c.heads)}
-                                 : locate<kAttnWarps>(a, share, at);
+    Place place;
+    int rank = 0;
+    if (a.cluster) {
+        const int pair = blockIdx.x / a.cluster;
+        rank = blockIdx.x % a.cluster;
+        place.b = pair / a.c.heads;
+        place.h = pair % a.c.heads;
+        place.n = kv8_length(a.lengths, a.length_all, place.b, a.max_length, a.c.status);
+        place.u = units_of<kAttnWarps>(place.n) * rank / a.cluster;
+    } else {
+        place = locate<kAttnWarps>(a, share, at);
+    }
     const int h = place.h, b = place.b, n = place.n;
     const size_t bh = (size_t)b * a.c.heads + h;
     const int full = n / kKv8Block;                 // complete blocks
     const int full_u = full * (kKv8Block / kUnit), units = units_of<kAttnWarps>(n);
-    const int x_lo = place.u, x_hi = a.single ? units : (int)min((long long)units, x_lo + (stop - at));
+    const int x_lo = place.u, x_hi = a.cluster ? units * (rank + 1) / a.cluster : (int)min((long long)units, x_lo + (stop - at));
     const int u_lo = min(full_u, x_lo), u_hi = min(full_u, x_hi);
     const bool takes_tail = x_hi == units;          // the tail's units: its last one's piece takes all of it
-    const bool whole = x_lo == 0 && x_hi == units;  // nothing to join: the output is written here
-    const size_t piece = a.single ? bh : blockIdx.x + bh;       // pieces are numbered so: both grow along the units, one of them at each new piece
-    at = a.single ? stop : at + (x_hi - x_lo);
+    const bool whole = a.cluster == 1 || (!a.cluster && x_lo == 0 && x_hi == units);     // nothing to join: the output is written here
+    const size_t piece = blockIdx.x + bh;           // pieces are numbered so: both grow along the units, one of them at each new piece
+    at = a.cluster ? stop : at + (x_hi - x_lo);
     if (takes_tail && n % kKv8Block) {              // the tail is wanted at the end: on its way to L2 from here
         const char* kt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.k_tail) + bh * kKv8Block * kKv8Dim);
         const char* vt = reinterpret_cast<const char*>(static_cast<const __nv_bfloat16*>(a.c.v_tail) + bh * kKv8Block * kKv8Dim);
@@ -624,6 +641,7 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
     float (*sm_o)[kRows][kKv8Dim] = reinterpret_cast<float (*)[kRows][kKv8Dim]>(ring_all);
     static_assert(kAttnWarps * kRows * kKv8Dim * sizeof(float) <= kRingBytes, "the warps' outputs fit the rings");
     __shared__ float2 sm_ml[kAttnWarps][kRows];     // maximum and denominator; then the warp's weight
+    __shared__ float sm_lse[kRows];                 // of a cluster's part
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
@@ -658,8 +676,10 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
 #pragma unroll
         for (int w = 0; w < kAttnWarps; ++w) sm_ml[w][r].x = lse[w] == 0.f ? 0.f : lse[w] / (sum * l[w]);
         const float all = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+        sm_lse[r] = all;
         if (r < a.rows) {
-            a.part_lse[piece * a.rows + r] = all;
+            if (!a.cluster) a.part_lse[piece * a.rows + r] = all;
+            else if (whole && a.logits) a.part_lse[bh * a.rows + r] = all;
             if (whole && a.lse) {
                 const int hq = h * a.group + r / a.n_q;
                 a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + r % a.n_q] = all;
@@ -695,13 +715,56 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
                     if (!(fabsf(v) < CUDART_INF_F)) acc[k] += v;
                 }
         }
-        if (!whole) {
+        if (a.cluster > 1) {
+            *reinterpret_cast<float4*>(&sm_o[0][r][d]) = make_float4(acc[0], acc[1], acc[2], acc[3]);     // (read by this thread alone)
+        } else if (!whole) {
             *reinterpret_cast<float4*>(a.part_o + (piece * a.rows + r) * kKv8Dim + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
         } else {
             const int hq = h * a.group + (a.n_q == 1 ? r : r / a.n_q), t = a.n_q == 1 ? 0 : r % a.n_q;
             __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
             *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc[0], acc[1]), pack_bf16x2(acc[2], acc[3]));
         }
+    }
+    if (a.cluster > 1) {
+        // the parts of the cluster joined out of its CTAs' shared memories, each CTA some of the rows
+        namespace cg = cooperative_groups;
+        cg::cluster_group cluster = cg::this_cluster();
+        cluster.sync();
+        for (int i = rank * kAttnThreads + threadIdx.x; i < a.rows * 32; i += a.cluster * kAttnThreads) {
+            const int r = i >> 5, d = (i & 31) * 4;
+            float e[kMaxCluster], top = -CUDART_INF_F, sum = 0.f;
+            float4 x[kMaxCluster];
+#pragma unroll
+            for (int k = 0; k < kMaxCluster; ++k) {
+                const int from = min(k, a.cluster - 1);
+                e[k] = *cluster.map_shared_rank(&sm_lse[r], from);
+                x[k] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(&sm_o[0][r][d], from));
+                if (k >= a.cluster) e[k] = -CUDART_INF_F;
+                top = fmaxf(top, e[k]);
+            }
+            float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+            const float ref = top == -CUDART_INF_F ? 0.f : top;
+#pragma unroll
+            for (int k = 0; k < kMaxCluster; ++k) {
+                if (k >= a.cluster) break;
+                const float f = exp2f(e[k] - ref);          // (a part that saw nothing holds zeros; NaN goes through)
+                sum += f;
+                acc.x = fmaf(f, x[k].x, acc.x);
+                acc.y = fmaf(f, x[k].y, acc.y);
+                acc.z = fmaf(f, x[k].z, acc.z);
+                acc.w = fmaf(f, x[k].w, acc.w);
+            }
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            const int hq = h * a.group + (a.n_q == 1 ? r : r / a.n_q), t = a.n_q == 1 ? 0 : r % a.n_q;
+            __nv_bfloat16* o = a.o + b * a.os[0] + hq * a.os[1] + t * a.os[2] + d;
+            *reinterpret_cast<uint2*>(o) = make_uint2(pack_bf16x2(acc.x * inv, acc.y * inv), pack_bf16x2(acc.z * inv, acc.w * inv));
+            if (d == 0) {
+                const float all = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
+                if (a.logits) a.part_lse[bh * a.rows + r] = all;
+                if (a.lse) a.lse[((size_t)b * a.c.heads * a.group + hq) * a.n_q + t] = all;
+            }
+        }
+        cluster.sync();                             // the others read this CTA's part
     }
     __syncthreads();                                // before the next piece's copies
     }
@@ -730,7 +793,7 @@ __device__ __forceinline__ Parts parts_of(const Kv8AttnArgs& a, size_t bh, int r
         return {(bh * a.rows + r) * a.splits, 1, a.splits};
     } else {
         const int b = (int)(bh / a.c.heads), h = (int)(bh % a.c.heads);
-        if (a.single) return {bh * a.rows + r, (size_t)a.rows, 1};     // as numbered there
+        if (a.cluster) return {bh * a.rows + r, (size_t)a.rows, 1};    // (its log-sum-exp, for the weights)
         const Share share = share_of<W>(a, false);
         const long long all = share.units;
         const int ctas = share.ctas;
@@ -972,13 +1035,50 @@ __global__ void __launch_bounds__(kWeightThreads) kv8_weights_kernel(const __gri
 // ---------------------------------------------------------------------------------------------------- host
 struct AttnShape {
     int nt;                         // column groups of the narrow kernel, 0: the wide kernel
-    bool single;                    // narrow kernel: a CTA per head
+    int cluster;                    // narrow kernel: CTAs of a head, 0: all CTAs share all heads evenly
     int tiles, splits, pitch;
     long long tokens;
     size_t part_o, part_lse, row_lse, logits, bytes;
 };
 
-static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights) {
+// Whether the CTAs of the narrow kernel take a head each (or a cluster of 2 to 8 a head, which joins its parts out of its shared
+// memories) or share all heads' units evenly, with a second kernel for the joining.  Costs in units that a warp takes one after
+// the other: 1.35 us at one group of rows, 1.7 at more.  Measured, us, 8 cache heads of 4 query heads, graph / eager:
+//                                evenly        cluster of
+//   1 sequence of    1000    14.4 / 23.6    8:  8.6 / 13.7
+//                    4133    10.5 / 16.0    8: 11.9 / 14.6
+//                    8192    11.7 / 15.7    8: 13.5 / 16.5
+//                   16384    14.4 / 16.8    8: 19.6 / 21.7
+//   16 sequences of  1000    19.7 / 22.6    1: 12.9 / 14.7
+//                    8192    50.3 / 53.4    2: 44.8 / 47.4
+//   1, weights       1000    15.0           8: 11.3
+//                    4133    11.1           8: 14.8
+constexpr double kClusterJoin = 0.5;
+constexpr double kSecondKernel = 3.25, kSecondAnyway = 0.4;     // its start, its launch on the host; with weights it runs all the same
+constexpr double kCrossing = 2.5;                   // CTAs that work on two heads or sequences
+constexpr int kRaggedUnits = 8;                     // where lengths may differ, the longest must not keep a cluster much longer than all the rest
+static int cluster_of(long long pairs, long long units, int warps, bool weights, bool same) {
+    const long long slots = 2 * kSMs, all = pairs * units, ctas = std::min(slots, (all + warps - 1) / warps);
+    const double busy = warps == 8 ? 2.2 : 1.;      // a unit's time where HBM has all warps to serve
+    const double load = busy * (double)all / (double)(slots * warps);
+    const bool crossing = !same || pairs > ctas || ctas / pairs * pairs * 10 < ctas * 9;
+    double best = (weights ? kSecondAnyway : kSecondKernel) + (crossing ? kCrossing : 0.) +
+                  std::max((double)((all + slots * warps - 1) / (slots * warps)), load);
+    int cluster = 0;
+    for (int c = 1; c <= kMaxCluster && (c == 1 || pairs * c <= slots); c *= 2) {
+        const long long turn = (units + c * warps - 1) / (c * warps), waves = (pairs * c + slots - 1) / slots;
+        if (!same && turn > kRaggedUnits) continue;
+        const double cost = std::max((double)(waves * turn), load) + (c > 1 ? kClusterJoin : 0.);
+        if (cost < best) {
+            best = cost;
+            cluster = c;
+        }
+    }
+    return cluster;
+}
+
+// `same`: sequences of one length
+static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_length, bool weights, bool same) {
     AttnShape s{};
     const long long rows = (long long)(hq / heads) * n_q, pairs = (long long)batch * heads;
     s.nt = rows <= kNarrowRows ? (int)((rows + 7) / 8) : 0;
@@ -987,10 +1087,9 @@ static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_
     if (s.nt) {
         const int warps = narrow_warps(s.nt);
         const long long units = (long long)(max_length / kKv8Block) * (kKv8Block / kUnit) + warps;
-        // Short sequences, a unit for every warp and the tail: a CTA per head, and no second kernel unless the weights need one
-        s.single = units <= 2 * warps;
-        s.splits = s.single ? (int)std::min<long long>(pairs, 0x7fffffff) : (int)std::min<long long>(2 * kSMs, (pairs * units + warps - 1) / warps);
-        parts = (s.single ? pairs : s.splits + pairs) * rows;
+        s.cluster = cluster_of(pairs, units, warps, weights, same);
+        s.splits = s.cluster ? (int)(pairs * s.cluster) : (int)std::min<long long>(2 * kSMs, (pairs * units + warps - 1) / warps);
+        parts = s.cluster ? 0 : (s.splits + pairs) * rows;
     } else {
         // one CTA an SM: the number of splits (of two tiles of tokens at least) that wastes least of its last wave; each
         // costs about as much again as two tiles (its start, its end and the joining)
@@ -1012,7 +1111,7 @@ static AttnShape attention_shape(int batch, int hq, int heads, int n_q, int max_
     s.part_o = at;
     at = up(at + (size_t)parts * kKv8Dim * sizeof(float));
     s.part_lse = at;
-    at = up(at + (size_t)parts * sizeof(float));
+    at = up(at + (size_t)(s.cluster && weights ? pairs * rows : parts) * sizeof(float));
     s.row_lse = at;
     if (weights && !s.nt) at = up(at + (size_t)pairs * rows * sizeof(float));
     s.logits = at;
@@ -1031,8 +1130,18 @@ static cudaError_t launch_narrow(const Kv8AttnArgs& a, cudaStream_t stream) {
     static std::atomic<unsigned long long> allowed{0};
     const cudaError_t e = allow_shared(kv8_attention_kernel<FMT, NT, LOGITS>, bytes, allowed);
     if (e != cudaSuccess) return e;
-    kv8_attention_kernel<FMT, NT, LOGITS><<<a.splits, narrow_warps(NT) * 32, bytes, stream>>>(a);
-    return cudaGetLastError();
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeClusterDimension;
+    attr[0].val.clusterDim.x = std::max(1, a.cluster);
+    attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(a.splits);
+    cfg.blockDim = dim3(narrow_warps(NT) * 32);
+    cfg.dynamicSmemBytes = bytes;
+    cfg.stream = stream;
+    cfg.attrs = attr;
+    cfg.numAttrs = a.cluster > 1 ? 1 : 0;
+    return cudaLaunchKernelEx(&cfg, kv8_attention_kernel<FMT, NT, LOGITS>, a);
 }
 
 template <int FMT, bool LOGITS>
@@ -1056,7 +1165,9 @@ using namespace minf;
 
 extern "C" size_t minf_kv8_attention_scratch_bytes(int batch, int hq, int heads, int n_q, int max_length, int with_weights) {
     if (!attention_sizes_ok(batch, hq, heads, n_q, max_length)) return 0;
-    return attention_shape(batch, hq, heads, n_q, max_length, with_weights != 0).bytes;
+    // one sequence has one length; of several the caller may say so or not
+    const size_t bytes = attention_shape(batch, hq, heads, n_q, max_length, with_weights != 0, true).bytes;
+    return batch == 1 ? bytes : std::max(bytes, attention_shape(batch, hq, heads, n_q, max_length, with_weights != 0, false).bytes);
 }
 
 extern "C" int minf_kv8_attention(
@@ -1071,7 +1182,7 @@ extern "C" int minf_kv8_attention(
     if (max_length > cache->capacity) return fail(MINF_E_ARG, "max_length %d is outside the cache of %d tokens", max_length, cache->capacity);
     if (!lengths && (length_all < 0 || length_all > max_length)) return fail(MINF_E_ARG, "length %d is outside [0, max_length %d]", length_all, max_length);
     if (add_to && !weights) return fail(MINF_E_ARG, "add_to without weights");
-    const AttnShape s = attention_shape(cache->batch, hq, cache->heads, n_q, max_length, weights != nullptr);
+    const AttnShape s = attention_shape(cache->batch, hq, cache->heads, n_q, max_length, weights != nullptr, !lengths || cache->batch == 1);
     const long long a_rows = (long long)(hq / cache->heads) * n_q;
     if (s.bytes && !scratch) return fail(MINF_E_ARG, "scratch is needed (%zu bytes)", s.bytes);
     if (reinterpret_cast<uintptr_t>(scratch) & 15) return fail(MINF_E_ARG, "scratch must be 16-byte aligned");
@@ -1098,7 +1209,7 @@ extern "C" int minf_kv8_attention(
     a.max_length = max_length;
     a.scale_log2 = sm_scale * 1.4426950408889634f;
     a.splits = s.splits;
-    a.single = s.single;
+    a.cluster = s.cluster;
     char* base = static_cast<char*>(scratch);
     a.part_o = reinterpret_cast<float*>(base + s.part_o);
     a.part_lse = reinterpret_cast<float*>(base + s.part_lse);
@@ -1123,7 +1234,7 @@ extern "C" int minf_kv8_attention(
     const long long pairs = (long long)cache->batch * cache->heads, rows = pairs * a.rows;
     a.chunk = kFinishTokens * (int)std::max(1ll, std::min(16ll, pairs * (max_length / kFinishTokens) / kFinishCtas));
     const long long chunks = weights ? ((long long)max_length + a.chunk - 1) / a.chunk : 0;
-    if (s.nt && s.single && !chunks) return MINF_OK;
+    if (s.cluster && !chunks) return MINF_OK;
     if (s.nt) {
         const dim3 grid((unsigned)(rows + pairs * chunks));
         e = narrow_warps(s.nt) == 8 ? launch_behind(kv8_finish_kernel<8>, grid, kFinishThreads, 0, st, a)

@@ -17,7 +17,7 @@ struct Kv8AttnArgs {
     int length_all, max_length;
     float scale_log2;
     int splits;                     // wide kernel: parts of a head's tokens; narrow kernel: CTAs in all
-    bool single;                    // narrow kernel: CTA i has all of head i
+    int cluster;                    // narrow kernel: CTAs of a head, which join their parts themselves; 0: all CTAs share all heads
     float* part_o;                  // results of parts, normalised, fp32 [..][128]: wide [batch*heads*rows][splits], narrow [piece][rows]
     float* part_lse;                // their log-sum-exps
     float* lse;                     // caller's, [batch, hq, n_q], or NULL
