@@ -75,21 +75,35 @@ __device__ __forceinline__ uint2 values_to_codes(const float (&x)[8], float scal
             c[i] = (uint32_t)lo | ((uint32_t)hi << 16);
         }
     } else {
-        // x / scale rounded to an integer: by the reciprocal, which is right unless the quotient lies next to a half (its
-        // error is below 127 * 2^-22), and there by the division the definition has
+        // x / scale rounded to an integer: by the reciprocal, which is right unless the quotient lies next to a half (both
+        // quotients' errors together are below 127 * 2^-23), and there by the division the definition has.  Adding 1.5 * 2^23
+        // rounds to the nearest integer and leaves it in the low bits.
+        constexpr float kRound = 12582912.f;
         const float inv = __fdiv_rn(1.f, scale);
+        bool sure = true;                                   // (false for what is not finite too)
 #pragma unroll
         for (int i = 0; i < 2; ++i) {
-            uint32_t w = 0;
+            uint32_t q[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) {
-                const float y = x[4 * i + j] * inv;
-                float q = rintf(y);
-                if (fabsf(fabsf(y - q) - 0.5f) < 1e-4f) q = rintf(__fdiv_rn(x[4 * i + j], scale));
-                const int r = q != q ? 0 : (int)fminf(fmaxf(q, -127.f), 127.f);
-                w |= (uint32_t)(r & 0xff) << (8 * j);
+                const float t = __fmaf_rn(x[4 * i + j], inv, kRound);
+                sure = sure && fabsf(__fmaf_rn(x[4 * i + j], inv, -(t - kRound))) < 0.49998f;
+                q[j] = __float_as_uint(t);
             }
-            c[i] = w;
+            c[i] = __byte_perm(__byte_perm(q[0], q[1], 0x0040), __byte_perm(q[2], q[3], 0x0040), 0x5410);
+        }
+        if (!sure) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) {
+                uint32_t w = 0;
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float q = rintf(__fdiv_rn(x[4 * i + j], scale));
+                    const int r = q != q ? 0 : (int)fminf(fmaxf(q, -127.f), 127.f);
+                    w |= (uint32_t)(r & 0xff) << (8 * j);
+                }
+                c[i] = w;
+            }
         }
     }
     return make_uint2(c[0], c[1]);
@@ -552,10 +566,24 @@ __global__ void __launch_bounds__(kStoreThreads, 6) kv8_gather_kernel(const __gr
         float top = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            float x[8];
-            values(i, x);
+            float big = INFINITY;
+            if (coded >> i & 1u) {                          // the largest code (NaN is passed over) times its scale
+                uint32_t h[4];
+                codes_to_half<FMT>(raw[i].x, h[0], h[1]);
+                codes_to_half<FMT>(raw[i].y, h[2], h[3]);
+                __half2 m = __float2half2_rn(0.f);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) top = fmaxf(top, finite_magnitude(x[j]));
+                for (int j = 0; j < 4; ++j) m = __hmax2(m, __habs2(*reinterpret_cast<const __half2*>(&h[j])));
+                big = fmaxf(__low2float(m), __high2float(m)) * scale_in[i];
+            }
+            if (!(big < INFINITY)) {                        // the tail's values, and codes next to fp32's largest
+                float x[8];
+                values(i, x);
+                big = 0.f;
+#pragma unroll
+                for (int j = 0; j < 8; ++j) big = fmaxf(big, finite_magnitude(x[j]));
+            }
+            top = fmaxf(top, big);
         }
         top = block_max<kStoreThreads>(top, red);
         const float scale = scale_of<FMT>(top);

@@ -515,6 +515,28 @@ def test_evict_ties_and_odd_weights(case):
         _check_evict(cache, R_copy(ref), weights, [n], budget, 100, 3)
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_evict_values_at_their_edges(kind):
+    """Requantising blocks that mix zeros, the tiniest and the largest values (e4m3's largest code overflows fp32 there), halves
+    between two codes, infinities and NaN."""
+    from minference_b200 import kv8_store
+
+    gen = torch.Generator().manual_seed(22)
+    parts = [torch.full((64, 128), f) for f in (0.0, 448.0, 2.0 ** -133, 3e38, 3.3895e38, -127.0)]
+    halves = (torch.arange(64 * 128).reshape(64, 128) % 253 - 126) / 2.0
+    bad = torch.randn(64, 128, generator=gen)
+    bad[3, 5], bad[7, 9], bad[60, 127] = NAN, math.inf, -math.inf
+    x = torch.stack(parts + [halves, bad, torch.full((64, 128), NAN), torch.randn(64, 128, generator=gen)]).reshape(1, 1, -1, 128).to(torch.bfloat16)
+    x = torch.cat((x, x[:, :, 300:333]), 2)
+    n = x.shape[2]
+    cache, ref = _poisoned(1, 1, n, kind), R.RefCache(1, 1, kind)
+    kv8_store(cache, x.cuda(), x.flip(2).cuda(), 0)
+    ref.append(x, x.flip(2))
+    for budget in (n, 513, 200):
+        weights = torch.rand(1, 1, cache.capacity, generator=gen)
+        _check_evict(cache, R_copy(ref), weights, [n], budget, 20, 3)
+
+
 def R_copy(ref):
     new = R.RefCache(ref.batch, ref.heads, ref.kind)
     new.raw = {n: [list(x) for x in t] for n, t in ref.raw.items()}
