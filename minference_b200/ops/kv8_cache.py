@@ -149,7 +149,7 @@ class KV8Cache:
 def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
     """(device pointer or None, host value, tensor to keep alive) of an int or an int32 tensor ``[B]``."""
     if isinstance(x, torch.Tensor):
-        if x.dtype != torch.int32 or x.dim() != 1 or x.numel() != cache.batch or x.device != cache.device or not x.is_contiguous():
+        if x.dtype != torch.int32 or x.shape != (cache.batch,) or x.device != cache.device or not x.is_contiguous():
             _fail(f"{what} must be an int or a contiguous int32 tensor [{cache.batch}] on {cache.device} (got {x.dtype} {tuple(x.shape)} on {x.device})")
         return x.data_ptr(), 0
     x = int(x)
@@ -159,7 +159,8 @@ def _per_sequence(cache: KV8Cache, x, what: str, low: int, high: int):
 
 
 def _rows(t: torch.Tensor, what: str, cache: KV8Cache):
-    if t.dim() != 4 or t.shape[0] != cache.batch or t.shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or t.device != cache.device:
+    shape = t.shape
+    if len(shape) != 4 or shape[0] != cache.batch or shape[3] != HEAD_DIM or t.dtype != torch.bfloat16 or t.device != cache.device:
         _fail(f"{what} must be bf16 [{cache.batch}, heads, tokens, {HEAD_DIM}] on {cache.device} (got {t.dtype} {tuple(t.shape)} on {t.device})")
     s0, s1, s2, s3 = t.stride()
     if s3 != 1 or (s0 | s1 | s2) & 7 or t.data_ptr() & 15:
@@ -167,8 +168,14 @@ def _rows(t: torch.Tensor, what: str, cache: KV8Cache):
     return t
 
 
+@functools.lru_cache(maxsize=4096)
+def _c_strides(*strides):
+    return _I64x3(*strides[:3])
+
+
 def _strides(t: torch.Tensor):
-    return _I64x3(*t.stride()[:3])
+    """The first three strides for a C entry point (the array of equal ones is made once: it is only read)."""
+    return _c_strides(*t.stride())
 
 
 def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
@@ -176,9 +183,9 @@ def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, co
     int32 tensor ``[B]``); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
     same call.  A block that fills is quantised from its 64 tokens' bf16 values.  Only the touched blocks are written."""
     key, value = _rows(key, "key", cache), _rows(value, "value", cache)
-    if key.shape[1] != cache.kv_heads or key.shape != value.shape:
-        _fail(f"key and value must be [{cache.batch}, {cache.kv_heads}, n, {HEAD_DIM}] both (got {tuple(key.shape)}, {tuple(value.shape)})")
-    n = key.shape[2]
+    _, h, n, _ = shape = key.shape
+    if h != cache.kv_heads or shape != value.shape:
+        _fail(f"key and value must be [{cache.batch}, {cache.kv_heads}, n, {HEAD_DIM}] both (got {tuple(shape)}, {tuple(value.shape)})")
     dev_counts = None
     if counts is not None:
         if not isinstance(counts, torch.Tensor):
@@ -238,7 +245,7 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
                   weights: torch.Tensor | None = None, add_to: torch.Tensor | None = None, return_lse: bool = False):
     """Attention of the last S tokens of every sequence, ``query [B, H, S, 128]`` (bf16, H a multiple of the cache's
     heads), over the cache that already holds them: query i of a sequence of n tokens sees its first ``n - S + 1 + i``.
-    Returns ``[B, H, S, 128]`` bf16 and, with ``return_lse``, the base-2 log-sum-exp of the scaled logits, fp32
+    Returns ``[B, H, S, 128]`` bf16 (in memory in the query's order of dimensions) and, with ``return_lse``, the base-2 log-sum-exp of the scaled logits, fp32
     ``[B, H, S]``.  A row that sees nothing gives zeros and -inf.
 
     ``lengths``: int or int32 tensor ``[B]``, the new tokens included; ``max_length``: an upper bound of them known on the
@@ -263,12 +270,12 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
         _weights_arg(add_to, "add_to", cache, longest)
     if weights is not None:
         _check_written(weights, add_to)
-    out = query.new_empty((b, hq, s, d))
+    out = torch.empty_like(query)           # in the query's order of dimensions: what a projection behind it wants
     lse = _like(cache.device, torch.float32).new_empty((b, hq, s)) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)
     scratch = cache.status.new_empty(nbytes // 4) if nbytes else None       # (in words of four bytes)
     _launch("minf_kv8_attention", cache,
-            cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _I64x3(hq * s * d, s * d, d), hq, s, dev_n, n, longest,
+            cache._ref, query.data_ptr(), _strides(query), out.data_ptr(), _strides(out), hq, s, dev_n, n, longest,
             d ** -0.5 if sm_scale is None else float(sm_scale), lse.data_ptr() if return_lse else None,
             weights.data_ptr() if weights is not None else None, _strides(weights) if weights is not None else None,
             add_to.data_ptr() if add_to is not None else None, _strides(add_to) if add_to is not None else None,

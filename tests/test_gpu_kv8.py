@@ -780,3 +780,23 @@ def test_two_streams_read_one_cache(s):
     torch.cuda.synchronize()
     for i in range(2):
         assert all(torch.equal(a, b) for pair in got[i] for a, b in zip(pair, want[i]))
+
+
+@pytest.mark.parametrize("s, hq, hkv, n", [(1, 4, 2, 700), (3, 4, 2, 9000), (40, 4, 2, 300)])
+def test_query_and_output_layouts(s, hq, hkv, n):
+    """Queries sliced out of a joint projection, head-major, with gaps, and expanded over the batch give the same numbers."""
+    from minference_b200 import kv8_attention
+
+    gen = torch.Generator().manual_seed(47)
+    cache, _ = _filled(gen, 2, hkv, [n, n], torch.float8_e4m3fn)
+    joint = torch.randn(2, s, hq + 2 * hkv, 128, generator=gen).to(torch.bfloat16).cuda()
+    q = joint[:, :, :hq].transpose(1, 2)
+    plain = q.contiguous()
+    want = kv8_attention(plain, cache, n)
+    assert want.is_contiguous() and want.shape == (2, hq, s, 128)
+    gaps = torch.zeros(2, hq, 2 * s, 136, dtype=torch.bfloat16, device="cuda")[:, :, ::2, :128]
+    gaps.copy_(plain)
+    for x in (q, gaps, plain.transpose(2, 3).contiguous().transpose(2, 3)):
+        assert torch.equal(kv8_attention(x, cache, n), want)
+    one = plain[:1].expand(2, hq, s, 128)
+    assert torch.equal(kv8_attention(one, cache, n), kv8_attention(one.contiguous(), cache, n))
