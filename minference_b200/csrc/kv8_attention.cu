@@ -924,7 +924,9 @@ __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, 
 }
 
 // The first CTAs join the parts of a row each (narrow kernel: up to a few dozen parts, eight warps) or of eight rows (wide
-// kernel).  The others (narrow kernel) sum the weights, for which they join the log-sum-exps of their head's rows themselves: no second wait.
+// kernel).  The others (narrow kernel) sum the weights, for which they join the log-sum-exps of their head's rows themselves: no
+// second wait.  Behind the attention of 131072 tokens it takes 4-5 us; with the weights of 262144 tokens and 28 query heads,
+// whose 34 MB of logits come out of L2, 13 us.
 template <int W>
 __global__ void __launch_bounds__(kFinishThreads) kv8_finish_kernel(const __grid_constant__ Kv8AttnArgs a) {
     __shared__ float4 sm[8][32];

@@ -18,8 +18,11 @@
 // In tiles that some row does not see to its end, values that are infinite or NaN are left out of the product (zero
 // times them would reach rows that do not see them) and added to the rows that do at the end.
 //
-// Bound: with 128 live rows the tensor pipe, 16 products of 64 cycles a tile; with few rows the 32 KB a tile takes from
-// HBM (about 1400 cycles of an SM's share), under which 1024 cycles of padded products hide.
+// Bound: the chain of a softmax warp.  A tile takes 2400 cycles (131072 tokens of 8 heads: 128 rows 96 us, 256 rows 162 us;
+// 256 new tokens of 32 heads over 16384: 101 us), of which the products need 1024, the exponentials 1024, shared memory 1792
+// and HBM's share 1400; ALU 58 % busy, issue slots 55 %, exponentials 43 %, tensor pipe 41 %.  Two ways round a part of it were
+// 2-4 % slower: S in two halves, the next one asked for as soon as P of the half before is used up; codes straight from HBM
+// into registers instead of through the raw tiles.
 #include "kv8_attention.cuh"
 
 #include <math_constants.h>
