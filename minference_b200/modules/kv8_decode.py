@@ -32,7 +32,8 @@ class KV8Layer:
     ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``.  ``budget``: tokens kept per head when the cache is cut down
     (None: never); ``sink`` first and ``recent`` last tokens are always kept (``recent=None``: a quarter of the budget).
     The cache is cut down after the prompt, and again whenever ``slack`` more tokens than the budget have come in.
-    ``seen`` counts all tokens (the next one's position), ``held`` those in the cache."""
+    ``seen`` counts all tokens (the next one's position), ``held`` those in the cache.  ``taken`` is False between the
+    ``update`` of a ``KV8HFCache`` and the attention function that takes its tokens."""
 
     def __init__(self, dtype=torch.float8_e4m3fn, budget: int | None = None, recent: int | None = None, sink: int = 4, slack: int = 256,
                  capacity: int = 0):
@@ -47,6 +48,7 @@ class KV8Layer:
         self.cache: KV8Cache | None = None
         self.sums: torch.Tensor | None = None
         self.held = self.seen = 0
+        self.taken = True
 
     def _room(self, key: torch.Tensor) -> None:
         b, h, n, _ = key.shape
@@ -108,12 +110,14 @@ def _hf_base():
 
     class Layer(CacheLayerMixin):
         """A layer of ``KV8HFCache``.  ``update`` returns the new tokens only, marked with the layer that holds the others:
-        the patched attention function attends over the 8-bit cache."""
+        the patched attention function attends over the 8-bit cache.  A function that does not know the mark would attend
+        over the new tokens alone, so the next ``update`` of any layer (``last``, shared by the cache's layers, is the one before
+        it) looks whether they were taken: in the same pass of the model if it has two layers or more."""
         is_sliding = False
 
-        def __init__(self, make):
+        def __init__(self, make, last):
             super().__init__()
-            self.kv = make()
+            self.kv, self.last = make(), last
             self.is_initialized = True
 
         def lazy_initialization(self, key_states, value_states):
@@ -122,7 +126,11 @@ def _hf_base():
         def update(self, key_states, value_states, *args, **kwargs):
             if key_states.shape[0] != 1:
                 raise _cabi.MInferB200Error("the 8-bit cache of a Hugging Face model takes one sequence, like the sparse prefill")
+            if self.last and not self.last[0].taken:
+                raise _cabi.MInferB200Error("no attention function took the tokens that were last put into the 8-bit cache: the model is not "
+                                            "patched with MInference, or makes other tensors of the keys before its attention")
             self.kv.append(key_states, value_states)
+            self.kv.taken, self.last[:] = False, [self.kv]
             key_states = key_states.view(key_states.shape)      # a tensor object of its own to carry the mark
             key_states.minf_kv8 = self.kv
             return key_states, value_states
@@ -146,13 +154,15 @@ def _hf_base():
 
     class KV8HFCache(Cache):
         def __init__(self, **options):
-            super().__init__(layer_class_to_replicate=lambda: Layer(lambda: KV8Layer(**options)))
+            last = []
+            super().__init__(layer_class_to_replicate=lambda: Layer(lambda: KV8Layer(**options), last))
 
     return KV8HFCache
 
 
 def KV8HFCache(dtype=torch.float8_e4m3fn, budget: int | None = None, recent: int | None = None, sink: int = 4, slack: int = 256, capacity: int = 0):
     """``past_key_values`` for a model patched with ``MInference(...)(model)``: keys and values in 8 bits, options as in
-    ``KV8Layer``.  One sequence; ``model(ids, past_key_values=KV8HFCache(...))`` or ``model.generate(...)``."""
+    ``KV8Layer``.  One sequence; ``model(ids, past_key_values=KV8HFCache(...))`` or ``model.generate(...)``.  A model that is not
+    patched is refused."""
     KV8Layer(dtype, budget, recent, sink, slack, capacity)       # the options' own checks, now rather than at the first token
     return _hf_base()(dtype=dtype, budget=budget, recent=recent, sink=sink, slack=slack, capacity=capacity)

@@ -67,6 +67,7 @@ def _make_attention_function(config):
     def minference_attention(module, query, key, value, attention_mask=None, dropout=0.0, scaling=None, **kwargs):
         kv8 = getattr(key, "minf_kv8", None)         # the 8-bit cache that holds this layer's tokens, these included
         if kv8 is not None:
+            kv8.taken = True
             if kv8.seen > query.shape[2]:
                 if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None:
                     raise MInferB200Error("sliding-window or soft-capped layers cannot attend over an 8-bit cache")

@@ -1,0 +1,86 @@
+"""Host paths around the 8-bit cache that must not go wrong without a word (no GPU needed: the storage is stubbed)."""
+from types import SimpleNamespace
+
+import pytest
+import torch
+
+
+@pytest.fixture()
+def cabi(built_lib):
+    from minference_b200 import _cabi
+
+    return _cabi
+
+
+@pytest.fixture()
+def counted(monkeypatch):
+    """KV8Layer that only counts its tokens and answers with zeros."""
+    from minference_b200 import KV8Layer
+
+    def append(self, key, value):
+        self.held += key.shape[2]
+        self.seen += key.shape[2]
+
+    monkeypatch.setattr(KV8Layer, "append", append)
+    monkeypatch.setattr(KV8Layer, "attend", lambda self, query, sm_scale=None: torch.zeros_like(query))
+
+
+def _model(layers, implementation="sdpa"):
+    from transformers import LlamaConfig, LlamaForCausalLM
+
+    torch.manual_seed(0)
+    cfg = LlamaConfig(vocab_size=50, hidden_size=256, intermediate_size=64, num_hidden_layers=layers, num_attention_heads=2,
+                      num_key_value_heads=1, head_dim=128, max_position_embeddings=256, attn_implementation=implementation)
+    return LlamaForCausalLM(cfg).eval()
+
+
+IDS = torch.arange(6)[None]
+
+
+@torch.no_grad()
+def _steps(model, past, steps=3):
+    model(IDS, past_key_values=past, use_cache=True)
+    for _ in range(steps):
+        model(IDS[:, :1], past_key_values=past, use_cache=True)
+
+
+@pytest.mark.parametrize("layers", [1, 2])
+def test_a_model_that_is_not_patched_is_refused(cabi, counted, layers):
+    """Its attention would see the new tokens alone.  Two layers show it in the first call, one layer in the second."""
+    from minference_b200 import KV8HFCache
+
+    past = KV8HFCache()
+    with pytest.raises(cabi.MInferB200Error, match="patched"):
+        _steps(_model(layers), past, 1)
+    past.reset()
+    assert past.get_seq_length() == 0
+
+
+def test_a_copy_of_the_keys_is_refused(cabi, counted):
+    """A step between the cache and the attention function that makes another tensor of the keys loses their mark."""
+    from transformers.modeling_utils import ALL_ATTENTION_FUNCTIONS
+
+    from minference_b200 import KV8HFCache, MInference
+
+    model = MInference("dense")(_model(2))
+    name = model.config._attn_implementation
+    real = ALL_ATTENTION_FUNCTIONS[name]
+    ALL_ATTENTION_FUNCTIONS[name] = lambda module, q, k, v, mask, **kw: real(module, q, k.clone(), v, mask, **kw)
+    try:
+        with pytest.raises(cabi.MInferB200Error, match="patched"):
+            _steps(model, KV8HFCache())
+    finally:
+        ALL_ATTENTION_FUNCTIONS[name] = real
+
+
+@pytest.mark.parametrize("layers", [1, 2])
+@pytest.mark.filterwarnings("ignore:minference_b200. this prefill")
+def test_a_patched_model_is_taken(cabi, counted, layers):
+    from minference_b200 import KV8HFCache, MInference
+
+    model, past = MInference("dense")(_model(layers)), KV8HFCache()
+    _steps(model, past)
+    assert past.get_seq_length() == 9
+    past.reset()
+    _steps(model, past)
+    assert past.get_seq_length() == 9
