@@ -18,6 +18,7 @@ from dataclasses import dataclass
 
 import torch
 
+from ._cabi import MInferB200Error
 from .modules.minference_forward import minference_prefill_forward
 from .synthetic import apply_rope, rope_cos_sin
 
@@ -75,8 +76,11 @@ class LlamaPrefill:
         ``attention(q, k, v, layer_idx)`` replaces the single-GPU operator (the ring passes one).
         ``timing``: a dict that receives CUDA-event pairs, ``"gemm"`` around every projection / MLP product and
         ``"attention"`` around every layer's attention (see ``split_times``).
-        ``kv``: one ``KV8Layer`` per layer (``new_kv``), which keep the prompt's keys and values for ``decode``.
+        ``kv``: one ``KV8Layer`` per layer (``new_kv``), which keep the prompt's keys and values for ``decode``: the whole
+        prompt's, so it goes with neither ``positions`` nor ``attention`` (a rank of the ring has its own chunks only).
         """
+        if kv is not None and (positions is not None or attention is not None):
+            raise MInferB200Error("kv keeps the whole prompt: it cannot be given together with positions or attention")
         s = self.shape
         n = ids.numel()
         dev, dt = self.device, self.dtype

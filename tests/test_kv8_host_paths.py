@@ -84,3 +84,20 @@ def test_a_patched_model_is_taken(cabi, counted, layers):
     past.reset()
     _steps(model, past)
     assert past.get_seq_length() == 9
+
+
+@pytest.fixture(scope="module")
+def runner():
+    from minference_b200.prefill_runner import LlamaPrefill, LlamaShape
+
+    return LlamaPrefill(LlamaShape(layers=2, hidden=64, q_heads=2, kv_heads=1, head_dim=128, ffn=64, vocab=50), "cpu")
+
+
+@pytest.mark.parametrize("option", [{"positions": torch.arange(6)}, {"attention": lambda q, k, v, layer: q},
+                                    {"positions": torch.arange(6), "attention": lambda q, k, v, layer: q}])
+def test_a_sharded_prompt_is_not_kept(cabi, counted, runner, option):
+    """Under the ring a rank has a part of the prompt: it must not become the cache that decoding goes on from."""
+    kv = runner.new_kv()
+    with pytest.raises(cabi.MInferB200Error, match="whole prompt"):
+        runner.prefill(IDS[0], {}, kv=kv, **option)
+    assert all(x.seen == 0 for x in kv)
