@@ -3,14 +3,16 @@
 // For a row (query head, query token) with logits l_t = sm_scale log2(e) s_K,t (q . c_K,t) over the tokens it sees,
 //   out = sum_t 2^(l_t - lse) s_V,t c_V,t,    lse = log2 sum_t 2^l_t
 // in one pass over the cache.  The running maximum M is that of l_t + log2 s_V,t, so the numerators
-// P_t = 2^(l_t + log2 s_V,t - M) are at most 2^8 (M follows jumps beyond that only) and multiply the codes as they are, whatever the scales; the
-// denominator is the sum over blocks of (sum P_t) / s_V.
+// P_t = 2^(l_t + log2 s_V,t - M) are at most 2^8 (M follows jumps beyond that only) and multiply the codes as they are; the
+// denominator is the sum over blocks of (sum P_t) / s_V.  (All of it holds while the scales of the values of one head stay within
+// 2^100 of each other: below that a block's numerators leave fp32.)
 //
 // The products run on the tensor cores with the tokens as rows: S^T = K Q^T and O^T = V^T P^T, m16n8k16 in f16 with
 // fp32 accumulation.  Eight query rows (a group of query heads that share a cache head, times the new tokens) fill the
 // narrow side without padding to sixteen, and a code becomes an f16 value exactly.  Q is scaled by a power of two per
-// row so that its bf16 values are f16 values (what is lost lies 2^-24 below the row's largest).  P is rounded to f16:
-// half a step of 2^-11 relative, below the bf16 rounding of the output; sums and outputs are accumulated in fp32.
+// row so that its bf16 values are f16 values (what is lost lies 2^-24 below the row's largest).  P is rounded to f16 with the
+// headroom of kv8_attention.cuh: half a step of 2^-11 relative, below the bf16 rounding of the output, or 2^-32 of the largest;
+// sums and outputs are accumulated in fp32.
 // The tail (bf16) takes bf16 products, with P as a sum of two bf16 numbers.
 //
 // The tokens are split over CTAs and, inside one, over warps by units of 32.  Parts are joined by their log-sum-exps: short
@@ -96,7 +98,7 @@ struct Rows {
 template <int NT, int SUB, bool LOGITS>
 __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, float (&s)[SUB][NT][4], float k_scale, float v_scale,
                                              int t0, bool masked, int all_see, int end, size_t bh, int tg, int c) {
-    const float lv = __log2f(v_scale), inv_v = __fdividef(1.f, v_scale);
+    const float lv = __log2f(v_scale), inv_v = __fdividef(kHeadroomOut, v_scale);
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const float f0 = R.mul[nt][0] * k_scale, f1 = R.mul[nt][1] * k_scale;
@@ -141,8 +143,8 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             mx0 = fmaxf(mx0, fmaxf(x[0], x[2]));
             mx1 = fmaxf(mx1, fmaxf(x[1], x[3]));
         }
-        // the reference is raised on a jump of more than 2^8: P stays far below f16's largest, outputs are rarely rescaled,
-        // and the lanes compare their maxima only then
+        // the reference is raised on a jump of more than 2^8: P stays below f16's largest, outputs are rarely rescaled, and the
+        // lanes compare their maxima only then
         mx0 += lv;
         mx1 += lv;
         if (__any_sync(0xffffffffu, mx0 > R.m[nt][0] + 8.f || mx1 > R.m[nt][1] + 8.f)) {
@@ -166,7 +168,7 @@ __device__ __forceinline__ void softmax_step(const Kv8AttnArgs& a, Rows<NT>& R, 
             }
         }
         // nothing seen yet: -inf - 0
-        const float d0 = lv - (R.m[nt][0] == -CUDART_INF_F ? 0.f : R.m[nt][0]), d1 = lv - (R.m[nt][1] == -CUDART_INF_F ? 0.f : R.m[nt][1]);
+        const float d0 = lv + kHeadroom - (R.m[nt][0] == -CUDART_INF_F ? 0.f : R.m[nt][0]), d1 = lv + kHeadroom - (R.m[nt][1] == -CUDART_INF_F ? 0.f : R.m[nt][1]);
         float sum0 = 0.f, sum1 = 0.f;
 #pragma unroll
         for (int j = 0; j < SUB; ++j) {
@@ -674,7 +676,7 @@ __global__ void __launch_bounds__(narrow_warps(NT) * 32, 2) kv8_attention_kernel
             sum += lse[w];
         }
 #pragma unroll
-        for (int w = 0; w < kAttnWarps; ++w) sm_ml[w][r].x = lse[w] == 0.f ? 0.f : lse[w] / (sum * l[w]);
+        for (int w = 0; w < kAttnWarps; ++w) sm_ml[w][r].x = lse[w] == 0.f ? 0.f : lse[w] * kHeadroomOut / (sum * l[w]);
         const float all = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
         sm_lse[r] = all;
         if (r < a.rows) {

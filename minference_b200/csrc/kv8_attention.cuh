@@ -6,6 +6,13 @@ namespace minf {
 
 constexpr int kSMs = 148;
 
+// Numerators are kept as f16 kHeadroom powers of two above their value.  The reference they are relative to follows jumps of
+// more than 2^8 only, so they reach 2^15 (f16 ends at 65504); a token is rounded to 2^-11 of its numerator down to 2^-21 of the
+// largest, and to 2^-32 of the largest below that.  (Without the headroom those were 2^-14 and 2^-25: behind a strong token of no
+// value, weak ones 24 bits below it came out wrong by a percent, ones of 26 bits by half.)  Denominators take it out again term
+// by term, outputs at the end.
+constexpr float kHeadroom = 7.f, kHeadroomOut = 0.0078125f;
+
 struct Kv8AttnArgs {
     minf_kv8_cache c;
     const __nv_bfloat16* q;

@@ -385,7 +385,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             for (int x = 0; x < 2; ++x) {
                 f[x] *= mul;
                 lv[x] = __log2f(inv_v[x]);
-                inv_v[x] = __fdividef(1.f, inv_v[x]);
+                inv_v[x] = __fdividef(kHeadroomOut, inv_v[x]);
             }
             ok = __all_sync(0xffffffffu, mbar_wait(bar(&ctl->s_full[grp]), (i >> 1) & 1, abort_flag));
             if (!ok) break;
@@ -437,12 +437,12 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             const float ma = fmaxf(largest(s0), largest(s1));
             const float mx = fmaxf(ma == -CUDART_INF_F ? ma : fmaf(ma, f[0], lv[0]), mb == -CUDART_INF_F ? mb : fmaf(mb, f[1], lv[1]));   // (-inf times zero)
             float alpha = 1.f;
-            if (mx > m_ref + 8.f) {                 // the reference is raised on a jump of more than 2^8: P stays far below f16's largest
+            if (mx > m_ref + 8.f) {                 // the reference is raised on a jump of more than 2^8: P stays below f16's largest
                 alpha = fast_exp2(m_ref - mx);
                 l_sum *= alpha;
                 m_ref = mx;
             }
-            const float ref = m_ref == -CUDART_INF_F ? 0.f : m_ref;
+            const float ref = m_ref == -CUDART_INF_F ? 0.f : m_ref - kHeadroom;
             if (i > 1 && __any_sync(0xffffffffu, alpha != 1.f)) {       // (O is at rest: this tile's S came behind its last product)
 #pragma unroll 1
                 for (int c = 0; c < 16; ++c) {
@@ -530,7 +530,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
         const float mine = l_sum == 0.f ? -CUDART_INF_F : (m_ref == -CUDART_INF_F ? l_sum : m_ref + log2f(l_sum));
         if (grp == 1) {
             ctl->lse[r] = mine;
-            const float inv = l_sum == 0.f ? 0.f : 1.f / l_sum;
+            const float inv = l_sum == 0.f ? 0.f : kHeadroomOut / l_sum;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
                 uint32_t o[16];
@@ -548,7 +548,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             const float theirs = ctl->lse[r], top = fmaxf(mine, theirs);
             const float e0 = mine == -CUDART_INF_F ? 0.f : exp2f(mine - top), e1 = theirs == -CUDART_INF_F ? 0.f : exp2f(theirs - top);
             const float sum = e0 + e1;
-            const float w0 = e0 == 0.f ? 0.f : e0 / (sum * l_sum), w1 = e1 == 0.f ? 0.f : e1 / sum;
+            const float w0 = e0 == 0.f ? 0.f : e0 * kHeadroomOut / (sum * l_sum), w1 = e1 == 0.f ? 0.f : e1 / sum;
             const float lse = sum == 0.f ? -CUDART_INF_F : top + log2f(sum);
             const size_t row = bh * a.rows + gr;
             const int hq = h * a.group + gr / a.n_q, t = gr % a.n_q;
