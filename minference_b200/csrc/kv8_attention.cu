@@ -900,15 +900,16 @@ __device__ __forceinline__ void sum_weights(const Kv8AttnArgs& a, int b, int h, 
 #pragma unroll
         for (int k = 0; k < kEach; ++k)
             l[k] = load_now4(x + row[k] * a.pitch + r);
-        // rows behind the last: +inf, so that whatever their columns hold counts nothing
-        const float e0 = row_lse[r], e1 = r + 1 < a.rows ? row_lse[r + 1] : CUDART_INF_F, e2 = r + 2 < a.rows ? row_lse[r + 2] : CUDART_INF_F,
-                    e3 = r + 3 < a.rows ? row_lse[r + 3] : CUDART_INF_F;
+        // columns behind the last row hold anything, NaN too: their finished terms are dropped
+        const bool r1 = r + 1 < a.rows, r2 = r + 2 < a.rows, r3 = r + 3 < a.rows;
+        const float e0 = row_lse[r], e1 = r1 ? row_lse[r + 1] : 0.f, e2 = r2 ? row_lse[r + 2] : 0.f, e3 = r3 ? row_lse[r + 3] : 0.f;
 #pragma unroll
         for (int k = 0; k < kEach; ++k) {
+            const float w1 = weight_of(l[k].y, e1), w2 = weight_of(l[k].z, e2), w3 = weight_of(l[k].w, e3);
             sum[k] += weight_of(l[k].x, e0);
-            sum[k] += weight_of(l[k].y, e1);
-            sum[k] += weight_of(l[k].z, e2);
-            sum[k] += weight_of(l[k].w, e3);
+            sum[k] += r1 ? w1 : 0.f;
+            sum[k] += r2 ? w2 : 0.f;
+            sum[k] += r3 ? w3 : 0.f;
         }
     }
     if (a.pitch == 2) {

@@ -42,3 +42,27 @@ def test_many_weak_tokens_behind_a_strong_one_of_no_value(kind, gap, s, hq):
         assert (half_steps <= 2.0 ** (gap - 30) * want).all()
         off = (out[0, h] - want).abs()
         assert (off <= tol).all(), (h, (off / want).max().item(), (tol / want).max().item())
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [100, 1000, 20001])
+@pytest.mark.parametrize("hq", [1, 2, 3, 5, 6, 7, 11, 23, 25, 30])
+def test_weights_next_to_an_infinite_key(kind, n, hq):
+    """A key of -inf that every head's logit goes to -inf with: its weight is zero, whatever the padding columns of the heads
+    (zero times that key) hold."""
+    from minference_b200 import kv8_attention, kv8_store
+
+    gen = torch.Generator().manual_seed(n + hq)
+    k, _ = _rows(gen, 1, 1, n)
+    v, dv = _rows(gen, 1, 1, n)
+    q, _ = _rows(gen, 1, hq, 1)
+    k[:, :, -2], q[..., 0] = 0, 1
+    k[:, :, -2, 0] = -math.inf                   # in the tail: those blocks keep infinities
+    cache = _poisoned(1, 1, n, kind)
+    kv8_store(cache, k.cuda(), dv, 0)
+    w = torch.zeros(1, 1, cache.capacity, device="cuda")
+    out, lse = kv8_attention(q.cuda(), cache, n, weights=w, return_lse=True)
+    assert torch.isfinite(out).all() and torch.isfinite(lse).all()
+    w = w[0, 0].cpu().double()
+    assert torch.isfinite(w).all() and w[n - 2] == 0 and not w[n:].any()
+    assert abs(w.sum().item() - hq) <= 1e-5 * hq
