@@ -2,7 +2,8 @@
 
 ``KV8Layer`` holds them in an 8-bit cache (``ops/kv8_cache.py``), attends over it for new tokens and, where a budget is
 set, sums the attention weights and cuts the cache down by them; the prompt's weights are the estimator's column sums (the
-softmax of its last 64 queries), the same numbers the vertical lines are selected by.  ``KV8HFCache`` is the same as a
+softmax of its last 64 queries), the same numbers the vertical lines are selected by; a model with another logit scale than
+1/sqrt(128) takes its own last queries' weights over the cache instead.  ``KV8HFCache`` is the same as a
 ``past_key_values`` object for a Hugging Face model patched with ``MInference``.  The role of the reference's kv_type
 caches (minference/modules/kvcompression.py's SnapKV and its decoding forward); the methods are this repository's own.
 """
@@ -14,7 +15,7 @@ import torch
 
 from .. import _cabi
 from ..ops.kv8_cache import BLOCK, KV8Cache, kv8_attention, kv8_evict, kv8_store
-from .minference_forward import vertical_slash_estimate
+from .minference_forward import last_q, vertical_slash_estimate
 
 
 def prompt_weights(query: torch.Tensor, key: torch.Tensor) -> torch.Tensor:
@@ -90,11 +91,15 @@ class KV8Layer:
             self.evict()
         return out
 
-    def after_prompt(self, query: torch.Tensor, key: torch.Tensor) -> None:
+    def after_prompt(self, query: torch.Tensor, key: torch.Tensor, sm_scale: float | None = None) -> None:
         """Cut the prompt down to the budget by its own weights (``query`` and ``key`` as its attention saw them)."""
         if self.budget is None:
             return
-        self.sums[..., : self.held] = prompt_weights(query, key)
+        plain = query.shape[-1] ** -0.5
+        if sm_scale is None or abs(float(sm_scale) - plain) <= 1e-6 * plain:
+            self.sums[..., : self.held] = prompt_weights(query, key)
+        else:                                   # the estimator knows no other scale: the same queries' weights over the cache
+            kv8_attention(query[:, :, -last_q:], self.cache, self.held, sm_scale=sm_scale, weights=self.sums)
         if self.held > self.budget:
             self.evict()
 

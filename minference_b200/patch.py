@@ -73,7 +73,7 @@ def _make_attention_function(config):
                     raise MInferB200Error("sliding-window or soft-capped layers cannot attend over an 8-bit cache")
                 return kv8.attend(query, scaling).transpose(1, 2), None
             out = prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs)
-            kv8.after_prompt(query, key)
+            kv8.after_prompt(query, key, scaling)
             return out
         return prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs)
 

@@ -66,3 +66,61 @@ def test_weights_next_to_an_infinite_key(kind, n, hq):
     w = w[0, 0].cpu().double()
     assert torch.isfinite(w).all() and w[n - 2] == 0 and not w[n:].any()
     assert abs(w.sum().item() - hq) <= 1e-5 * hq
+
+
+def _layer_with(gen, n, hq, hkv, kind, **options):
+    """(KV8Layer holding n tokens, queries, keys on the GPU; queries on the CPU, its definition)."""
+    from minference_b200 import KV8Layer
+
+    kv, ref = KV8Layer(kind, **options), R.RefCache(1, hkv, kind)
+    k, dk = _rows(gen, 1, hkv, n)
+    v, dv = _rows(gen, 1, hkv, n)
+    q, dq = _rows(gen, 1, hq, n)
+    kv.append(dk, dv)
+    ref.append(k, v)
+    return kv, dq, dk, dv, q, ref
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("n", [1, 50, 64, 300])
+@pytest.mark.parametrize("scaling", [1 / 128, 0.25, None])
+def test_a_prompts_weights_are_those_of_the_models_scaling(kind, n, scaling):
+    """The patched attention function hands a prompt's weights on with the scale the model uses: the probabilities of its last
+    64 queries."""
+    from types import SimpleNamespace
+
+    from minference_b200 import MInferenceConfig
+    from minference_b200.patch import _make_attention_function
+
+    gen = torch.Generator().manual_seed(n)
+    hq, hkv = 4, 2
+    kv, dq, dk, dv, q, ref = _layer_with(gen, n, hq, hkv, kind, budget=400, slack=50)
+    key = dk.view(dk.shape)
+    key.minf_kv8 = kv
+    module = SimpleNamespace(layer_idx=0, config=SimpleNamespace(num_hidden_layers=1), num_key_value_groups=hq // hkv, is_causal=True, training=False)
+    _make_attention_function(MInferenceConfig(attn_type="dense"))(module, dq, key, dv, scaling=scaling)
+    assert kv.held == n
+    for h in range(hkv):
+        want, tol = torch.zeros(n, dtype=torch.float64), torch.zeros(n, dtype=torch.float64)
+        for g in range(hq // hkv):
+            _, _, _, _, p, rel = R.attend(ref, q[0, h * (hq // hkv) + g, -64:], 0, h, scaling)
+            want += p.sum(0)
+            tol += (p * rel[:, None]).sum(0)
+        got = kv.sums[0, h, :n].cpu().double()
+        if scaling is None:
+            # the estimator's scores, of keys in bf16 and logits rounded to bf16 twice, stay as they were: no more than their sum here
+            assert abs(got.sum() - want.sum()) <= 2.0 ** -7 * want.sum()
+        else:
+            assert ((got - want).abs() <= tol + (hq // hkv * 64 + 1) * 2.0 ** -24 * want).all(), (got - want).abs().max()
+    assert not kv.sums[..., n:].any()
+
+
+def test_eviction_of_a_prompt_goes_by_the_models_scaling():
+    """A scale of zero makes all tokens a query sees alike: the earliest are kept, whatever the keys are."""
+    gen = torch.Generator().manual_seed(8)
+    kv, dq, dk, _, _, _ = _layer_with(gen, 500, 4, 2, torch.int8, budget=128, recent=16, sink=4)
+    kv.after_prompt(dq, dk, 0.0)
+    assert kv.held == 128
+    w = kv.sums[0, :, :112]                      # the sink and the earliest: each of 2 x 64 queries sees them among 437 to 500 tokens
+    want = 2 * (1 / torch.arange(437.0, 501.0).double()).sum().item()
+    assert ((w.double() - want).abs() <= 2.0 ** -15 * want).all()
