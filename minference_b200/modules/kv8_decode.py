@@ -84,9 +84,14 @@ class KV8Layer:
 
     def attend(self, query: torch.Tensor, sm_scale: float | None = None) -> torch.Tensor:
         """Attention of the last tokens appended, ``query [B, H, S, 128]``; their weights are added up where a budget is
-        set, and the cache cut down once it is ``slack`` tokens over it."""
+        set, and the cache cut down once it is ``slack`` tokens over it.  Of more than 64 new tokens the last 64 count, as of a
+        prompt: a long follow-up does not outweigh all that came before, nor need 4 bytes for each of its rows and tokens held."""
         weights = {} if self.budget is None else {"weights": self.sums, "add_to": self.sums}
-        out = kv8_attention(query, self.cache, self.held, sm_scale=sm_scale, **weights)
+        if not weights or query.shape[2] <= last_q:
+            out = kv8_attention(query, self.cache, self.held, sm_scale=sm_scale, **weights)
+        else:
+            out = kv8_attention(query, self.cache, self.held, sm_scale=sm_scale)
+            kv8_attention(query[:, :, -last_q:], self.cache, self.held, sm_scale=sm_scale, **weights)
         if self.budget is not None and self.held >= self.budget + self.slack:
             self.evict()
         return out

@@ -124,3 +124,43 @@ def test_eviction_of_a_prompt_goes_by_the_models_scaling():
     w = kv.sums[0, :, :112]                      # the sink and the earliest: each of 2 x 64 queries sees them among 437 to 500 tokens
     want = 2 * (1 / torch.arange(437.0, 501.0).double()).sum().item()
     assert ((w.double() - want).abs() <= 2.0 ** -15 * want).all()
+
+
+@pytest.mark.parametrize("new", [64, 65, 700])
+def test_a_long_follow_up_adds_the_weights_of_its_last_queries(new):
+    """As a prompt does, and in memory that does not grow with the new tokens times those held."""
+    from minference_b200 import KV8Layer, kv8_attention
+
+    gen = torch.Generator().manual_seed(new)
+    kv = KV8Layer(torch.int8, budget=256, slack=4096)
+    kv.append(_rows(gen, 1, 2, 300)[1], _rows(gen, 1, 2, 300)[1])
+    kv.sums[..., :300] = torch.rand(1, 2, 300, generator=gen).cuda()
+    before = kv.sums.clone()
+    kv.append(_rows(gen, 1, 2, new)[1], _rows(gen, 1, 2, new)[1])
+    _, dq = _rows(gen, 1, 8, new)
+    out = kv.attend(dq)
+    n = 300 + new
+    assert kv.held == n and torch.equal(out, kv8_attention(dq, kv.cache, n))
+    want = torch.zeros_like(kv.sums)
+    want[..., :300] = before[..., :300]
+    kv8_attention(dq[:, :, -64:], kv.cache, n, weights=want, add_to=want)
+    assert torch.equal(kv.sums[..., :n], want[..., :n]) and not kv.sums[..., n:].any()
+
+
+def test_a_long_follow_up_under_a_budget_needs_little_memory():
+    from minference_b200 import KV8Layer
+
+    kv = KV8Layer(budget=512, slack=64)
+    rows = lambda h, n: torch.randn(1, h, n, 128, dtype=torch.bfloat16, device="cuda")
+    kv.append(rows(8, 500), rows(8, 500))
+    k, v, q = rows(8, 4096), rows(8, 4096), rows(32, 4096)
+    kv.append(k, v)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    out = kv.attend(q)
+    torch.cuda.synchronize()
+    # 33.5 MB of output; logits of 64 queries of 32 heads over 4596 tokens, 38 MB; parts of 64 x 32 rows and of all rows where
+    # they are split (of 148 CTAs with 128 rows of 512 bytes at most): 10 MB each.  All rows' logits would be 2.4 GB
+    assert torch.cuda.max_memory_allocated() - base <= 128 << 20
+    assert kv.held == 512 and torch.isfinite(out).all()
