@@ -33,8 +33,9 @@ class KV8Layer:
     ``dtype``: ``torch.float8_e4m3fn`` or ``torch.int8``.  ``budget``: tokens kept per head when the cache is cut down
     (None: never); ``sink`` first and ``recent`` last tokens are always kept (``recent=None``: a quarter of the budget).
     The cache is cut down after the prompt, and again whenever ``slack`` more tokens than the budget have come in.
-    ``seen`` counts all tokens (the next one's position), ``held`` those in the cache.  ``taken`` is False between the
-    ``update`` of a ``KV8HFCache`` and the attention function that takes its tokens."""
+    ``seen`` counts all tokens (the next one's position), ``held`` those in the cache; ``cache.check()`` raises for what the
+    device reported since the layer was last reset.  ``taken`` is False between the ``update`` of a ``KV8HFCache`` and the
+    attention function that takes its tokens."""
 
     def __init__(self, dtype=torch.float8_e4m3fn, budget: int | None = None, recent: int | None = None, sink: int = 4, slack: int = 256,
                  capacity: int = 0):
@@ -58,7 +59,7 @@ class KV8Layer:
             return
         # the prompt and what decoding adds to it; doubled when that runs out
         cap = max(self.capacity, need + 512 if self.cache is None else 2 * need)
-        new = KV8Cache.empty(b, h, cap, self.dtype, key.device)
+        new = KV8Cache.empty(b, h, cap, self.dtype, key.device) if self.cache is None else self.cache._sibling(cap)
         sums = torch.zeros((b, h, new.capacity), dtype=torch.float32, device=key.device) if self.budget is not None else None
         if self.cache is not None and self.held:
             self._copy(new)
@@ -109,7 +110,7 @@ class KV8Layer:
             self.evict()
 
     def evict(self) -> None:
-        out = KV8Cache.empty(self.cache.batch, self.cache.kv_heads, self.budget + self.slack + 1, self.dtype, self.cache.device)
+        out = self.cache._sibling(self.budget + self.slack + 1)
         self.cache, _, self.sums, _ = kv8_evict(self.cache, self.held, self.sums, self.budget, recent=self.recent, sink=self.sink, out=out)
         self.held = min(self.held, self.budget)
 

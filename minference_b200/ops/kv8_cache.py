@@ -93,7 +93,7 @@ class KV8Cache:
         self._desc = _cabi.Kv8Desc(*[t.data_ptr() for t in self._tensors], status.data_ptr(), self.batch, self.kv_heads, self.capacity, _FORMATS[k.dtype])
         self._ref = ctypes.byref(self._desc)
 
-    def _smaller(self, capacity: int):
+    def _sibling(self, capacity: int):
         """An empty cache like this one; it reports into this one's status.  Its tensors are views of one allocation, made when
         somebody asks for them."""
         b, h, cap = self.batch, self.kv_heads, (capacity + BLOCK - 1) // BLOCK * BLOCK
@@ -300,7 +300,7 @@ def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, rece
     dev_n, n = _per_sequence(cache, lengths, "lengths", 0, longest)
     _weights_arg(weights, "weights", cache, longest)
     if out is None:
-        out = cache._smaller(budget)
+        out = cache._sibling(budget)
     elif out is cache or (out.batch, out.kv_heads, out.dtype, out.device) != (cache.batch, cache.kv_heads, cache.dtype, cache.device) or out.capacity < budget:
         _fail("out must be another cache of the same batch, heads, type and device with room for the budget")
     kept = cache.status.new_empty((cache.batch, cache.kv_heads, budget))

@@ -164,3 +164,24 @@ def test_a_long_follow_up_under_a_budget_needs_little_memory():
     # they are split (of 148 CTAs with 128 rows of 512 bytes at most): 10 MB each.  All rows' logits would be 2.4 GB
     assert torch.cuda.max_memory_allocated() - base <= 128 << 20
     assert kv.held == 512 and torch.isfinite(out).all()
+
+
+@pytest.mark.parametrize("how", ["evict", "grow"])
+def test_what_the_device_reported_outlives_the_layers_cache(how):
+    """A layer that cuts its cache down, or moves to a larger one, goes on reporting what happened before."""
+    from minference_b200 import KV8Layer, _cabi
+    from minference_b200._cabi import MInferB200Error
+
+    gen = torch.Generator().manual_seed(10)
+    kv = KV8Layer(budget=100, slack=10)
+    kv.append(_rows(gen, 1, 2, 105)[1], _rows(gen, 1, 2, 105)[1])
+    kv.cache.status[_cabi.ST_ERROR] = 1          # as an abandoned wait leaves it
+    old = kv.cache
+    if how == "evict":
+        kv.evict()
+    else:
+        kv.append(_rows(gen, 1, 2, 5000)[1], _rows(gen, 1, 2, 5000)[1])
+    assert kv.cache is not old
+    with pytest.raises(MInferB200Error, match="0x1 "):
+        kv.cache.check()
+    kv.cache.check()
