@@ -56,7 +56,7 @@ __device__ __forceinline__ float scale_of(float top) {
     if constexpr (FMT == MINF_KV8_E4M3) {
         int e;
         const float m = frexpf(top, &e);    // top = m * 2^e, 0.5 <= m < 1;  448 = 0.875 * 2^9
-        return exp2f((float)max(m <= 0.875f ? e - 9 : e - 8, -100));
+        return __uint_as_float((uint32_t)(max(m <= 0.875f ? e - 9 : e - 8, -100) + 127) << 23);     // (p is 120 at most)
     } else {
         return fmaxf(__fdiv_rn(top, 127.f), kKv8MinScale);
     }

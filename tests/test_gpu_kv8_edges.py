@@ -185,3 +185,18 @@ def test_what_the_device_reported_outlives_the_layers_cache(how):
     with pytest.raises(MInferB200Error, match="0x1 "):
         kv.cache.check()
     kv.cache.check()
+
+
+def test_every_exponent_of_an_e4m3_scale():
+    """Blocks whose largest value is 448 * 2^p or next to it, for every p that a scale may take: scales are 2^p to the bit."""
+    from minference_b200 import kv8_store
+
+    cache = _poisoned(1, 1, 64 * 440, torch.float8_e4m3fn)
+    p = torch.arange(-100, 120, dtype=torch.float64)
+    tops = torch.stack((448 * torch.exp2(p), 450 * torch.exp2(p - 1)), 1).flatten()      # (450 = 448 + one bf16 step)
+    x = torch.zeros(1, 1, 440, 64, 128)
+    x[0, 0, :, 5, 7] = -tops.float()
+    x = x.view(1, 1, -1, 128).to(torch.bfloat16).cuda()
+    kv8_store(cache, x, x, 0)
+    want = torch.exp2(p).repeat_interleave(2).float().clone()
+    assert torch.equal(cache.k_scale.cpu().flatten(), want) and torch.equal(cache.v_scale.cpu().flatten(), want)
