@@ -241,6 +241,18 @@ def _max_length(cache: KV8Cache, lengths, max_length):
     return int(max_length)
 
 
+class _ForwardOnly(torch.autograd.Function):
+    """The attention of queries that require a gradient: there is no backward pass, so one that would need it is an error."""
+
+    @staticmethod
+    def forward(ctx, *args):
+        return kv8_attention(*args)
+
+    @staticmethod
+    def backward(ctx, *grads):
+        _fail("kv8_attention is forward only: no gradient can pass through it")
+
+
 def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int | None = None, sm_scale: float | None = None,
                   weights: torch.Tensor | None = None, add_to: torch.Tensor | None = None, return_lse: bool = False):
     """Attention of the last S tokens of every sequence, ``query [B, H, S, 128]`` (bf16, H a multiple of the cache's
@@ -253,9 +265,11 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
     ``weights [B, Hkv, >= max_length]`` fp32 receives the attention weight of each token -- the probabilities summed over
     the head's queries -- plus ``add_to`` (``add_to=weights`` sums up in place); entries behind a sequence's length are
     left as they were.  It takes scratch memory of 4 bytes for every query row and token.
-    Forward only.  One to 24 rows per cache head (H / Hkv * S) and more take different kernels; both are within the
+    Forward only: a backward pass through it raises.  One to 24 rows per cache head (H / Hkv * S) and more take different kernels; both are within the
     roundings of P to 16 bits of the exact result.
     """
+    if query.requires_grad and torch.is_grad_enabled():
+        return _ForwardOnly.apply(query, cache, lengths, max_length, sm_scale, weights, add_to, return_lse)
     query = _rows(query, "query", cache)
     b, hq, s, d = query.shape
     if s < 1 or hq % cache.kv_heads:

@@ -200,3 +200,27 @@ def test_every_exponent_of_an_e4m3_scale():
     kv8_store(cache, x, x, 0)
     want = torch.exp2(p).repeat_interleave(2).float().clone()
     assert torch.equal(cache.k_scale.cpu().flatten(), want) and torch.equal(cache.v_scale.cpu().flatten(), want)
+
+
+@pytest.mark.parametrize("s, hq", [(1, 4), (40, 2)])
+def test_a_backward_pass_is_refused(s, hq):
+    """The operator is forward only: a gradient that would have to pass through it is an error, not a zero."""
+    from minference_b200 import kv8_attention
+    from minference_b200._cabi import MInferB200Error
+
+    gen = torch.Generator().manual_seed(5)
+    cache, _ = _filled(gen, 1, 1, [100], torch.int8)
+    _, q = _rows(gen, 1, hq, s)
+    want, want_lse = kv8_attention(q, cache, 100, return_lse=True)
+    leaf = q.detach().clone().requires_grad_()
+    out, lse = kv8_attention(leaf, cache, 100, return_lse=True)
+    assert torch.equal(out, want) and torch.equal(lse, want_lse) and out.requires_grad and out.stride() == torch.empty_like(leaf).stride()
+    with pytest.raises(MInferB200Error, match="forward only"):
+        (out.float() * 2).sum().backward()
+    with pytest.raises(MInferB200Error, match="forward only"):
+        kv8_attention(leaf, cache, 100, return_lse=True)[1].sum().backward()
+    out, _ = kv8_attention(leaf, cache, 100, return_lse=True)
+    assert torch.equal(out.mul_(2), want * 2)    # an output of its own, not a view
+    with torch.no_grad():
+        assert not kv8_attention(leaf, cache, 100).requires_grad
+    assert not kv8_attention(q, cache, 100).requires_grad and leaf.grad is None
