@@ -71,6 +71,8 @@ def _make_attention_function(config):
             if kv8.seen > query.shape[2]:
                 if kwargs.get("sliding_window") is not None or kwargs.get("softcap") is not None:
                     raise MInferB200Error("sliding-window or soft-capped layers cannot attend over an 8-bit cache")
+                if attention_mask is not None:
+                    raise MInferB200Error("the attention over an 8-bit cache takes no attention mask")
                 return kv8.attend(query, scaling).transpose(1, 2), None
             out = prompt_attention(module, query, key, value, attention_mask, dropout, scaling, kwargs)
             kv8.after_prompt(query, key, scaling)

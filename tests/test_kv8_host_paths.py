@@ -101,3 +101,17 @@ def test_a_sharded_prompt_is_not_kept(cabi, counted, runner, option):
     with pytest.raises(cabi.MInferB200Error, match="whole prompt"):
         runner.prefill(IDS[0], {}, kv=kv, **option)
     assert all(x.seen == 0 for x in kv)
+
+
+def test_a_decoding_step_with_a_mask_is_refused(cabi, counted):
+    """The attention over the cache takes no mask: one that the model hands on must not be left out without a word."""
+    from minference_b200 import KV8Layer, MInferenceConfig
+    from minference_b200.patch import _make_attention_function
+
+    attention = _make_attention_function(MInferenceConfig(attn_type="dense"))
+    kv, q, key = KV8Layer(), torch.zeros(1, 2, 1, 128), torch.zeros(1, 1, 1, 128)
+    kv.append(torch.zeros(1, 1, 9, 128), None)
+    key.minf_kv8 = kv
+    assert attention(None, q, key, key, None)[0].shape == (1, 1, 2, 128)
+    with pytest.raises(cabi.MInferB200Error, match="mask"):
+        attention(None, q, key, key, torch.zeros(1, 1, 1, 9))
