@@ -81,6 +81,8 @@ class LlamaPrefill:
         """
         if kv is not None and (positions is not None or attention is not None):
             raise MInferB200Error("kv keeps the whole prompt: it cannot be given together with positions or attention")
+        if kv is not None:
+            self._check_kv(kv)
         s = self.shape
         n = ids.numel()
         dev, dt = self.device, self.dtype
@@ -142,10 +144,15 @@ class LlamaPrefill:
 
         return [KV8Layer(**options) for _ in self.layers]
 
+    def _check_kv(self, kv: list) -> None:
+        if len(kv) != len(self.layers):
+            raise MInferB200Error(f"a cache for each of the {len(self.layers)} layers is wanted (got {len(kv)})")
+
     @torch.no_grad()
     def decode(self, ids: torch.Tensor, kv: list) -> torch.Tensor:
         """Logits (fp32 ``[S, vocab]``) behind each of the new tokens ``ids [S]``, which follow the tokens ``kv`` has seen and
         are added to it: a decoding step (S = 1), proposed tokens to check, or a follow-up prompt."""
+        self._check_kv(kv)
         s = self.shape
         n, nq, nk = ids.numel(), s.q_heads * s.head_dim, s.kv_heads * s.head_dim
         cos, sin = rope_cos_sin(n, s.head_dim, s.rope_theta, self.device, start=kv[0].seen)

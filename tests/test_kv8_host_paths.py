@@ -115,3 +115,13 @@ def test_a_decoding_step_with_a_mask_is_refused(cabi, counted):
     assert attention(None, q, key, key, None)[0].shape == (1, 1, 2, 128)
     with pytest.raises(cabi.MInferB200Error, match="mask"):
         attention(None, q, key, key, torch.zeros(1, 1, 1, 9))
+
+
+def test_the_runner_wants_a_cache_for_every_layer(cabi, counted, runner):
+    """Fewer would leave layers out of a decoding step without a word."""
+    for kv in (runner.new_kv()[:1], runner.new_kv() + runner.new_kv(), []):
+        with pytest.raises(cabi.MInferB200Error, match="2 layers"):
+            runner.decode(IDS[0, :1], kv)
+        with pytest.raises(cabi.MInferB200Error, match="2 layers"):
+            runner.prefill(IDS[0], {}, kv=kv)
+    assert runner.decode(IDS[0, :1], runner.new_kv()).shape == (1, 50)
