@@ -170,7 +170,12 @@ class LlamaPrefill:
         return (self._rms(x, self.final_norm) @ self.lm_head).float()
 
     def generate(self, ids: torch.Tensor, new_tokens: int, attn_forward_config: dict, kv: list | None = None, **options) -> torch.Tensor:
-        """``new_tokens`` greedy tokens behind the prompt ``ids [N]``: sparse prefill, then decoding over 8-bit caches."""
+        """``new_tokens`` greedy tokens behind the prompt ``ids [N]``: sparse prefill, then decoding over 8-bit caches (``kv``, or
+        new ones with ``options``)."""
+        if new_tokens < 1:
+            raise MInferB200Error(f"new_tokens must be positive (got {new_tokens})")
+        if kv is not None and options:
+            raise MInferB200Error(f"kv has options of its own (got {sorted(options)} too)")
         kv = self.new_kv(**options) if kv is None else kv
         nxt = self.prefill(ids, attn_forward_config, kv=kv).argmax()[None]
         out = [nxt]

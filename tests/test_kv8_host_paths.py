@@ -125,3 +125,13 @@ def test_the_runner_wants_a_cache_for_every_layer(cabi, counted, runner):
         with pytest.raises(cabi.MInferB200Error, match="2 layers"):
             runner.prefill(IDS[0], {}, kv=kv)
     assert runner.decode(IDS[0, :1], runner.new_kv()).shape == (1, 50)
+
+
+def test_generate_refuses_what_it_would_leave_out(cabi, counted, runner, monkeypatch):
+    monkeypatch.setattr(type(runner), "prefill", lambda self, ids, cfg, kv=None: torch.arange(50.0))
+    assert runner.generate(IDS[0], 1, {}).tolist() == [49]
+    for n in (0, -1):
+        with pytest.raises(cabi.MInferB200Error, match="new_tokens"):
+            runner.generate(IDS[0], n, {})
+    with pytest.raises(cabi.MInferB200Error, match="options"):
+        runner.generate(IDS[0], 1, {}, kv=runner.new_kv(), budget=100)
