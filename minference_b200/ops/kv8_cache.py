@@ -196,12 +196,14 @@ def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, co
 
 
 def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
-    """Values of tokens ``first .. first + count`` (``count=None``: to the end of the capacity) as ``(k, v)``, bf16
+    """Values of tokens ``first .. first + count`` (``count=None``, for an int ``first``: to the end of the capacity) as ``(k, v)``, bf16
     ``[B, Hkv, count, 128]``; zeros outside ``[0, length)``.  ``lengths`` and ``first``: int or int32 tensor ``[B]``."""
     dev_n, n = _per_sequence(cache, lengths, "lengths", 0, cache.capacity)
-    dev_first, first = _per_sequence(cache, first, "first", -(1 << 30), 1 << 30)
     if count is None:
-        count = cache.capacity - first
+        if isinstance(first, torch.Tensor):
+            _fail("count must be given where first is a tensor")
+        count = cache.capacity - int(first)
+    dev_first, first = _per_sequence(cache, first, "first", -(1 << 30), 1 << 30)
     if count < 0:
         _fail(f"count {count} must not be negative")
     shape = (cache.batch, cache.kv_heads, count, HEAD_DIM)

@@ -130,3 +130,21 @@ def test_misaligned_tensors_are_copied(cabi):
     for t in (buf[1:257].view(1, 2, 1, 128), buf[:256].as_strided((1, 2, 1, 128), (129, 128, 3, 1))):
         r = kv8_cache._rows(t, "query", cache)
         assert torch.equal(r, t) and r.data_ptr() % 16 == 0 and not any(s % 8 for s in r.stride()[:3])
+
+
+def test_load_to_the_end_wants_one_first_token(cabi, monkeypatch):
+    """With a first token for each sequence there is no one number of tokens up to the capacity."""
+    from types import SimpleNamespace
+
+    from minference_b200.ops import kv8_cache
+
+    calls = []
+    monkeypatch.setattr(kv8_cache, "_launch", lambda entry, cache, *args: calls.append(args))
+    cache = SimpleNamespace(batch=1, kv_heads=2, capacity=128, device=torch.device("cpu"), _ref=None)
+    for batch in (1, 2):
+        cache.batch = batch
+        first = torch.zeros(batch, dtype=torch.int32)
+        with pytest.raises(cabi.MInferB200Error, match="count"):
+            kv8_cache.kv8_load(cache, 100, first=first)
+        assert kv8_cache.kv8_load(cache, 100, first=first, count=5)[0].shape == (batch, 2, 5, 128)
+    assert kv8_cache.kv8_load(cache, 100, first=28)[0].shape == (2, 2, 100, 128) and len(calls) == 3
