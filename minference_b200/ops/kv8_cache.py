@@ -225,10 +225,14 @@ def _extent(t: torch.Tensor):
     return t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride())))
 
 
-def _check_written(weights: torch.Tensor, add_to: torch.Tensor | None) -> None:
-    """No element of ``weights`` may be written twice, or be read as ``add_to`` of another token."""
-    if (weights.shape[0] > 1 and weights.stride(0) == 0) or (weights.shape[1] > 1 and weights.stride(1) == 0):
-        _fail("weights must not be an expanded view: its elements are written")
+def _check_written(weights: torch.Tensor, add_to: torch.Tensor | None, tokens: int) -> None:
+    """No element of ``weights`` may be written twice (the first ``tokens`` of every head are), or be read as ``add_to`` of
+    another token."""
+    (b, h, _), (sb, sh, _) = weights.shape, weights.stride()
+    if not ((h == 1 or sh >= tokens) and (b == 1 or sb >= (h - 1) * sh + tokens)):      # (as a contiguous tensor has them)
+        starts = sorted(i * sb + j * sh for i in range(b) for j in range(h))
+        if any(y - x < tokens for x, y in zip(starts, starts[1:])):
+            _fail("weights must not be an expanded or overlapping view: its elements are written")
     if add_to is not None and add_to is not weights:
         a, b = _extent(weights), _extent(add_to)
         if a[0] < b[1] and b[0] < a[1] and (a[0] != b[0] or weights.stride() != add_to.stride()):
@@ -285,7 +289,7 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
             _fail("add_to without weights")
         _weights_arg(add_to, "add_to", cache, longest)
     if weights is not None:
-        _check_written(weights, add_to)
+        _check_written(weights, add_to, longest)
     out = torch.empty_like(query)           # in the query's order of dimensions: what a projection behind it wants
     lse = _like(cache.device, torch.float32).new_empty((b, hq, s)) if return_lse else None
     nbytes = _scratch_bytes(b, hq, cache.kv_heads, s, longest, weights is not None)

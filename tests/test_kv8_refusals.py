@@ -148,3 +148,31 @@ def test_load_to_the_end_wants_one_first_token(cabi, monkeypatch):
             kv8_cache.kv8_load(cache, 100, first=first)
         assert kv8_cache.kv8_load(cache, 100, first=first, count=5)[0].shape == (batch, 2, 5, 128)
     assert kv8_cache.kv8_load(cache, 100, first=28)[0].shape == (2, 2, 100, 128) and len(calls) == 3
+
+
+@pytest.mark.parametrize("strides, taken", [
+    ((200, 100, 1), True), ((100, 200, 1), True), ((1 << 20, 1 << 10, 1), True), ((150, 100, 1), False), ((150, 300, 1), True),
+    ((100, 100, 1), False), ((100, 50, 1), False), ((99, 300, 1), False), ((100, 0, 1), False), ((0, 100, 1), False)])
+def test_weights_of_two_heads_must_not_overlap(cabi, strides, taken):
+    """Each element is written by one head of one sequence: [2, 2, >= 100] with 100 tokens of them written."""
+    from minference_b200.ops import kv8_cache
+
+    w = torch.zeros(1 << 21).as_strided((2, 2, 120), strides)
+    if taken:
+        kv8_cache._check_written(w, None, 100)
+        kv8_cache._check_written(w, w, 100)
+    else:
+        with pytest.raises(cabi.MInferB200Error, match="written"):
+            kv8_cache._check_written(w, None, 100)
+
+
+def test_weights_that_interleave_without_overlapping_are_taken(cabi):
+    """Three heads 100 elements apart and two sequences 150 apart: 50 tokens each, no two at the same place."""
+    from minference_b200.ops import kv8_cache
+
+    w = torch.zeros(1000).as_strided((2, 3, 50), (150, 100, 1))
+    kv8_cache._check_written(w, None, 50)
+    with pytest.raises(cabi.MInferB200Error):
+        kv8_cache._check_written(w, None, 51)
+    kv8_cache._check_written(torch.zeros(3, 1, 50).expand(3, 4, 50)[:, :1], None, 50)
+    kv8_cache._check_written(torch.zeros(1, 1, 50).expand(4, 4, 50), None, 0)       # nothing is written
