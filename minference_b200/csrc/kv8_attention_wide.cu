@@ -559,6 +559,7 @@ __global__ void __launch_bounds__(kWideThreads, 1) kv8_attention_wide_kernel(con
             const __nv_bfloat16* vt = static_cast<const __nv_bfloat16*>(a.c.v_tail) + bh * kKv8Block * kKv8Dim;
 #pragma unroll 1
             for (int c = 0; c < 8; ++c) {
+                __syncwarp();                       // (a warp's rows part below; its loads from TMEM are of all lanes together)
                 uint32_t o[16];
                 if (any) {
                     tmem_ld16(t_o + 16 * c, o);
