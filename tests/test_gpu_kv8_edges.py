@@ -224,3 +224,13 @@ def test_a_backward_pass_is_refused(s, hq):
     with torch.no_grad():
         assert not kv8_attention(leaf, cache, 100).requires_grad
     assert not kv8_attention(q, cache, 100).requires_grad and leaf.grad is None
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("s, hq", [(1, 24), (1, 25), (6, 4), (5, 5), (24, 1), (25, 1), (3, 8), (8, 3), (1, 8), (1, 9), (1, 16), (1, 17)])
+def test_rows_around_the_kernels_borders(kind, s, hq):
+    """24 rows are the narrow kernel's last, 25 the wide one's first; 8 and 16 fill groups of columns."""
+    gen = torch.Generator().manual_seed(100 * s + hq)
+    lengths = [700, 65, max(s - 1, 0)]
+    cache, ref = _filled(gen, 3, 1, lengths, kind)
+    _check_attention(cache, ref, lengths, s, hq, gen, weights=True)
