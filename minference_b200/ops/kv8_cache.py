@@ -65,7 +65,11 @@ class KV8Cache:
     """Tensors of one layer's cache: ``k, v [B, Hkv, capacity, 128]`` codes (``torch.float8_e4m3fn`` or ``torch.int8``),
     ``k_scale, v_scale [B, Hkv, capacity / 64]`` fp32, ``k_tail, v_tail [B, Hkv, 64, 128]`` bf16 (token t of the last,
     incomplete block in row ``t % 64``), all contiguous on one CUDA device.  The number of tokens held is the caller's
-    (it is an argument of every call), so one cache serves captured graphs whose lengths change between replays."""
+    (it is an argument of every call), so one cache serves captured graphs whose lengths change between replays.
+
+    Tokens are dropped from the end by going on with a smaller number, as long as it ends in the same block: the tail is that
+    of the last block stored.  To go back from n to m tokens in an earlier block, put that block's values into the tail first:
+    ``cache.k_tail[:], cache.v_tail[:] = kv8_load(cache, n, first=m // 64 * 64, count=64)`` (rounded by their 8 bits then)."""
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
         _cabi.require_cuda(k, v, k_scale, v_scale, k_tail, v_tail)
@@ -180,7 +184,7 @@ def _strides(t: torch.Tensor):
 
 def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
     """Append tokens ``key, value [B, Hkv, n, 128]`` (bf16) behind the ``start`` tokens each sequence holds (an int or an
-    int32 tensor ``[B]``); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
+    int32 tensor ``[B]``; ``KV8Cache`` says how to drop tokens before); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
     same call.  A block that fills is quantised from its 64 tokens' bf16 values.  Only the touched blocks are written."""
     key, value = _rows(key, "key", cache), _rows(value, "value", cache)
     _, h, n, _ = shape = key.shape

@@ -151,7 +151,7 @@ class LlamaPrefill:
     @torch.no_grad()
     def decode(self, ids: torch.Tensor, kv: list) -> torch.Tensor:
         """Logits (fp32 ``[S, vocab]``) behind each of the new tokens ``ids [S]``, which follow the tokens ``kv`` has seen and
-        are added to it: a decoding step (S = 1), proposed tokens to check, or a follow-up prompt."""
+        are added to it and stay: a decoding step (S = 1), several tokens at once, or a follow-up prompt."""
         self._check_kv(kv)
         s = self.shape
         n, nq, nk = ids.numel(), s.q_heads * s.head_dim, s.kv_heads * s.head_dim

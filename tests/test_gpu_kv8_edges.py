@@ -234,3 +234,31 @@ def test_rows_around_the_kernels_borders(kind, s, hq):
     lengths = [700, 65, max(s - 1, 0)]
     cache, ref = _filled(gen, 3, 1, lengths, kind)
     _check_attention(cache, ref, lengths, s, hq, gen, weights=True)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_going_back_into_a_complete_block(kind):
+    """Proposed tokens fill a block and are then dropped: its tokens go back into the tail by the documented lines."""
+    from minference_b200 import kv8_load, kv8_store
+
+    gen = torch.Generator().manual_seed(12)
+    cache, ref = _filled(gen, 1, 2, [190], kind, capacity=320)
+    k, dk = _rows(gen, 1, 2, 5)
+    v, dv = _rows(gen, 1, 2, 5)
+    kv8_store(cache, dk, dv, 190)                # 195 tokens: block 2 is complete, the tail holds 192 to 194
+    ref.append(k, v)
+    kept = 191
+    block = kept // 64 * 64
+    cache.k_tail[:], cache.v_tail[:] = kv8_load(cache, 195, first=block, count=64)
+    back = R.RefCache(1, 2, kind)
+    for name in ("k", "v"):
+        for h in range(2):
+            x = ref.values(name, 0, h)[0]        # of the block that was complete: values of codes, rounded to bf16
+            x[block:] = x[block:].to(torch.bfloat16).double()
+            back.raw[name][0][h] = torch.cat((ref.raw[name][0][h][:block], x[block:kept]))
+    _check_attention(cache, back, [kept], 1, 8, gen, weights=True)
+    k, dk = _rows(gen, 1, 2, 70)
+    v, dv = _rows(gen, 1, 2, 70)
+    kv8_store(cache, dk, dv, kept)
+    back.append(k, v)
+    _check_attention(cache, back, [kept + 70], 3, 8, gen)
