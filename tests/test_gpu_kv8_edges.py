@@ -262,3 +262,33 @@ def test_going_back_into_a_complete_block(kind):
     kv8_store(cache, dk, dv, kept)
     back.append(k, v)
     _check_attention(cache, back, [kept + 70], 3, 8, gen)
+
+
+@pytest.mark.parametrize("s", [1, 40])
+def test_the_first_call_of_a_process_may_be_captured(s):
+    import subprocess
+    import sys
+
+    from tests.conftest import ROOT
+
+    code = f"""
+import torch
+from minference_b200 import KV8Cache, kv8_attention, kv8_evict, kv8_store
+gen = torch.Generator("cuda").manual_seed(1)
+rows = lambda h, n: torch.randn(1, h, n, 128, generator=gen, device="cuda").to(torch.bfloat16)
+cache, out = KV8Cache.empty(1, 2, 512), KV8Cache.empty(1, 2, 64)
+k, v, q = rows(2, 300), rows(2, 300), rows(8, {s})
+def step():
+    kv8_store(cache, k, v, 0)
+    w = torch.zeros(1, 2, 512, device="cuda")
+    return kv8_attention(q, cache, 300, weights=w), w, kv8_evict(cache, 300, w, 64, recent=8, out=out)[3]
+g = torch.cuda.CUDAGraph()
+with torch.cuda.graph(g):
+    got = step()
+g.replay()
+torch.cuda.synchronize()
+assert all(torch.equal(a, b) for a, b in zip(got, step()))
+print("captured")
+"""
+    r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
