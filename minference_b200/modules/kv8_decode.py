@@ -39,6 +39,8 @@ class KV8Layer:
 
     def __init__(self, dtype=torch.float8_e4m3fn, budget: int | None = None, recent: int | None = None, sink: int = 4, slack: int = 256,
                  capacity: int = 0):
+        if dtype not in (torch.float8_e4m3fn, torch.int8):
+            raise _cabi.MInferB200Error(f"cache codes must be float8_e4m3fn or int8 (got {dtype})")
         if budget is not None:
             recent = budget // 4 if recent is None else recent
             if budget < 1 or recent < 0 or sink < 0 or recent + sink > budget or slack < 1:
@@ -87,6 +89,8 @@ class KV8Layer:
         """Attention of the last tokens appended, ``query [B, H, S, 128]``; their weights are added up where a budget is
         set, and the cache cut down once it is ``slack`` tokens over it.  Of more than 64 new tokens the last 64 count, as of a
         prompt: a long follow-up does not outweigh all that came before, nor need 4 bytes for each of its rows and tokens held."""
+        if self.cache is None:
+            raise _cabi.MInferB200Error("the layer holds no tokens")
         weights = {} if self.budget is None else {"weights": self.sums, "add_to": self.sums}
         if not weights or query.shape[2] <= last_q:
             out = kv8_attention(query, self.cache, self.held, sm_scale=sm_scale, **weights)
@@ -110,6 +114,9 @@ class KV8Layer:
             self.evict()
 
     def evict(self) -> None:
+        """Cut the cache down to the budget."""
+        if self.budget is None or self.cache is None:
+            raise _cabi.MInferB200Error("the layer has no budget" if self.budget is None else "the layer holds no tokens")
         out = self.cache._sibling(self.budget + self.slack + 1)
         self.cache, _, self.sums, _ = kv8_evict(self.cache, self.held, self.sums, self.budget, recent=self.recent, sink=self.sink, out=out)
         self.held = min(self.held, self.budget)

@@ -135,3 +135,19 @@ def test_generate_refuses_what_it_would_leave_out(cabi, counted, runner, monkeyp
             runner.generate(IDS[0], n, {})
     with pytest.raises(cabi.MInferB200Error, match="options"):
         runner.generate(IDS[0], 1, {}, kv=runner.new_kv(), budget=100)
+
+
+def test_a_layer_that_holds_nothing_is_refused(cabi):
+    from minference_b200 import KV8Layer
+
+    for kv in (KV8Layer(), KV8Layer(budget=100)):
+        with pytest.raises(cabi.MInferB200Error, match="no tokens"):
+            kv.attend(torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16))
+        with pytest.raises(cabi.MInferB200Error, match="no tokens|no budget"):
+            kv.evict()
+    kv = KV8Layer()
+    kv.cache = "something"
+    with pytest.raises(cabi.MInferB200Error, match="no budget"):
+        kv.evict()
+    with pytest.raises(cabi.MInferB200Error, match="float8_e4m3fn or int8"):
+        KV8Layer(torch.float16)
