@@ -108,8 +108,13 @@ class KV8Layer:
         plain = query.shape[-1] ** -0.5
         if sm_scale is None or abs(float(sm_scale) - plain) <= 1e-6 * plain:
             self.sums[..., : self.held] = prompt_weights(query, key)
-        else:                                   # the estimator knows no other scale: the same queries' weights over the cache
-            kv8_attention(query[:, :, -last_q:], self.cache, self.held, sm_scale=sm_scale, weights=self.sums)
+        else:
+            # the estimator knows no other scale: the same queries' weights over the cache, one query head of each cache head
+            # at a time, because a call needs 4 bytes for every row and token
+            last, hkv = query[:, :, -last_q:], self.cache.kv_heads
+            for g in range(query.shape[1] // hkv):
+                kv8_attention(last.unflatten(1, (hkv, -1))[:, :, g], self.cache, self.held, sm_scale=sm_scale, weights=self.sums,
+                              add_to=self.sums if g else None)
         if self.held > self.budget:
             self.evict()
 

@@ -292,3 +292,21 @@ print("captured")
 """
     r = subprocess.run([sys.executable, "-c", code], cwd=ROOT, capture_output=True, text=True, timeout=300)
     assert r.returncode == 0 and "captured" in r.stdout, r.stderr[-2000:]
+
+
+def test_a_long_prompt_of_another_scaling_needs_little_memory():
+    from minference_b200 import KV8Layer
+
+    n = 65536
+    rows = lambda h: torch.randn(1, h, n, 128, dtype=torch.bfloat16, device="cuda")
+    kv, k, q = KV8Layer(budget=4096), rows(8), rows(32)
+    kv.append(k, k)
+    torch.cuda.synchronize()
+    torch.cuda.reset_peak_memory_stats()
+    base = torch.cuda.memory_allocated()
+    kv.after_prompt(q, k, 0.05)
+    torch.cuda.synchronize()
+    # logits of 64 queries of a query head for each of 8 heads, 134 MB; their parts, at most 148 CTAs' 128 rows of 512 bytes;
+    # the smaller cache, 11 MB.  All query heads' logits would be 537 MB
+    assert torch.cuda.max_memory_allocated() - base <= 192 << 20
+    assert kv.held == 4096 and abs(kv.sums.sum().item() / 2048) <= 1 + 1e-5
