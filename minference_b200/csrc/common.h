@@ -35,7 +35,8 @@ inline int fail(int code, const char* fmt, ...) {
 
 // Range-checked debug build (-DMINF_BOUNDS, `python -m minference_b200.build --bounds`): every store of the index
 // kernels and every plan-derived coordinate of the attention kernel is checked against the capacity of its
-// destination; a violation sets bit 3 of status[MINF_ST_ERROR] and the access is skipped.  Nothing traps.
+// destination; a violation sets bit 3 of status[MINF_ST_ERROR] and the access is skipped.  Nothing traps.  (The 8-bit cache's
+// kernels have no such checks: their places come from lengths that are clipped to the cache in every build.)
 #ifdef MINF_BOUNDS
 #define MINF_IN_BOUNDS(status, cond) ((cond) ? true : (atomicOr((status) + MINF_ST_ERROR, 8), false))
 #else

@@ -5,7 +5,7 @@
 // in one pass over the cache.  The running maximum M is that of l_t + log2 s_V,t, so the numerators
 // P_t = 2^(l_t + log2 s_V,t - M) are at most 2^8 (M follows jumps beyond that only) and multiply the codes as they are; the
 // denominator is the sum over blocks of (sum P_t) / s_V.  (All of it holds while the scales of the values of one head stay within
-// 2^100 of each other: below that a block's numerators leave fp32.)
+// 2^100 of each other, below which a block's numerators leave fp32, and the tail's values, which have no scale, below 2^104.)
 //
 // The products run on the tensor cores with the tokens as rows: S^T = K Q^T and O^T = V^T P^T, m16n8k16 in f16 with
 // fp32 accumulation.  Eight query rows (a group of query heads that share a cache head, times the new tokens) fill the
@@ -19,8 +19,8 @@
 // sequences' inside a cluster, others' in a second kernel, launched behind the first one's end.
 //
 // Bound: HBM.  Decoding steps of 4 rows per head read 131072 tokens of 8 heads in 45 us (5.9 TB/s; 51 us with the second
-// kernel), 1048576 tokens in 310 us (6.9 TB/s), issue slots 46 % and tensor pipe 18 % busy.  Up to 16 rows take 57 us, up to 24
-// 75 us: there it is the chain of each warp (three warps a scheduler instead of two change nothing).
+// kernel), 1048576 tokens in 310 us (6.9 TB/s), issue slots 43 % (int8: 53 %) and tensor pipe 18 % busy.  Up to 16 rows take
+// 57 us, up to 24 75 us: there it is the chain of each warp (three warps a scheduler instead of two change nothing).
 #include "kv8_attention.cuh"
 
 #include <cooperative_groups.h>
@@ -1058,6 +1058,9 @@ struct AttnShape {
 //                    8192    50.3 / 53.4    2: 44.8 / 47.4
 //   1, weights       1000    15.0           8: 11.3
 //                    4133    11.1           8: 14.8
+// The rule goes by eager calls: at 4133 tokens it takes the cluster, which is the slower in a captured graph.  Lengths on the
+// device may differ, so kRaggedUnits shuts out clusters whose warps would take more than eight units, even where the lengths
+// turn out equal: 16 sequences of 8192 tokens take 50 us then instead of 45.
 constexpr double kClusterJoin = 0.5;
 constexpr double kSecondKernel = 3.25, kSecondAnyway = 0.4;     // its start, its launch on the host; with weights it runs all the same
 constexpr double kCrossing = 2.5;                   // CTAs that work on two heads or sequences

@@ -9,7 +9,8 @@
 //                        the next one in flight while one is converted into the team's two 128-byte-swizzled stages.  A
 //                        thread converts what it copied itself, so the copies need no barrier
 //   warp 14              issues the MMAs
-// (Four warps share a scheduler at most, so a thread may hold 128 registers: half a row of S.)  Built and measured as well:
+// (Four warps share a scheduler at most, so of the launch's registers a thread has 128: half a row of S, and 88 bytes of spills,
+// 96 with logits.  Moving registers to the softmax warps, as the prefill kernel of this library does, was not tried.)  Built and measured as well:
 // two threads a row and one group (3070 cycles a tile, all of it one chain), conversion by one team of four warps (its
 // 2200 cycles a tile bound the rest).
 // TMEM: O and S of the two groups, 4 x 128 columns.

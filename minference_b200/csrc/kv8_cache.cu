@@ -112,8 +112,9 @@ __device__ __forceinline__ uint2 values_to_codes(const float (&x)[8], float scal
 // ------------------------------------------------------------------------------------------------- store
 // One CTA per (block of 64 tokens that gets new ones, head, keys or values).  256 threads hold the block in
 // registers, sixteen values of two rows each: one read of the new tokens, one write of the codes.
-// Bound by HBM: 4 B read and 2 B written per (key, value) pair of elements; 131072 tokens of 8 heads (537 MB read, 268 MB
-// written) take 126 us, 6.4 TB/s.
+// Bound by HBM for e4m3: 4 B read and 2 B written per (key, value) pair of elements; 131072 tokens of 8 heads (537 MB read,
+// 268 MB written) take 123 us, 6.5 TB/s.  int8 takes 187 us, 4.3 TB/s: its rounding and its search for quotients next to a half
+// keep the issue slots 75 % busy.
 struct StoreArgs {
     minf_kv8_cache c;
     const __nv_bfloat16* src[2];
@@ -217,7 +218,7 @@ __global__ void __launch_bounds__(kStoreThreads) kv8_store_kernel(const __grid_c
 
 // -------------------------------------------------------------------------------------------------- load
 // One CTA per (64 tokens, head, keys or values), sixteen values of two rows a thread.  Bound by HBM, one byte read for two
-// written: 131072 tokens of 8 heads take 126 us, 6.4 TB/s.
+// written: 131072 tokens of 8 heads take 126-128 us of either type, 6.4 TB/s.
 struct LoadArgs {
     minf_kv8_cache c;
     const int32_t* lengths;
@@ -305,8 +306,8 @@ constexpr int kSelectWords = 2 * kSelectBins + 3 * kSelectBins + kSelectList;
 // 4800 cycles instead of 1300 and a barrier.)  Then the warps, each with a contiguous stretch, count what they keep and
 // write it at the offset of everything before them: ascending order without a sort, equal keys by position.
 // What bounds it at 131072 tokens: the first pass (4 B a token read, atomics on a few dozen hot bins) and seven barriers
-// across the cluster of 1500 cycles each: 28 us alone for 8 heads, 17 us for 64 heads of 9000 tokens.  Four histograms a CTA
-// instead of two gain 1 us there and lose 1 us here.
+// across the cluster of 1500 cycles each: 24 us for 8 heads (30 with cold caches), 16 us (19) for 32 heads of 9000 tokens.  Four
+// histograms a CTA instead of two gain 1 us there and lose 1 us here.  ptxas gives it 32 registers and 20 bytes of spills.
 __global__ void __launch_bounds__(kSelectThreads) kv8_select_kernel(const __grid_constant__ SelectArgsKv8 a) {
     extern __shared__ uint32_t dyn[];
     uint32_t* hist = dyn;
@@ -514,7 +515,8 @@ struct GatherArgs {
 };
 
 // One CTA per (block of the new cache, head, keys or values): the kept tokens' values, quantised again as a block.  Bound by
-// two reads one after the other (which token, then its codes): 10 us for 8 heads of 4096 tokens, 11 MB.
+// two reads one after the other (which token, then its codes): 8-9 us for 8 heads of 4096 tokens, 11 MB (12 with cold caches).
+// The six CTAs an SM leave 40 registers a thread, of which int8 spills 8 bytes.
 template <int FMT>
 __global__ void __launch_bounds__(kStoreThreads, 6) kv8_gather_kernel(const __grid_constant__ GatherArgs a) {
     __shared__ float red[kStoreThreads / 32];
