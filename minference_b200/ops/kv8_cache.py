@@ -67,9 +67,10 @@ class KV8Cache:
     incomplete block in row ``t % 64``), all contiguous on one CUDA device.  The number of tokens held is the caller's
     (it is an argument of every call), so one cache serves captured graphs whose lengths change between replays.
 
-    Tokens are dropped from the end by going on with a smaller number, as long as it ends in the same block: the tail is that
-    of the last block stored.  To go back from n to m tokens in an earlier block, put that block's values into the tail first:
-    ``cache.k_tail[:], cache.v_tail[:] = kv8_load(cache, n, first=m // 64 * 64, count=64)`` (rounded by their 8 bits then)."""
+    Tokens are dropped from the end by going on with a smaller number of them: a multiple of 64, or one that ends in the block
+    that was incomplete, whose tokens the tail holds.  To go back from n to m tokens inside a complete block, put its values into
+    the tail first: ``cache.k_tail[:], cache.v_tail[:] = kv8_load(cache, n, first=m // 64 * 64, count=64)`` (rounded by their 8
+    bits then)."""
 
     def __init__(self, k, v, k_scale, v_scale, k_tail, v_tail):
         _cabi.require_cuda(k, v, k_scale, v_scale, k_tail, v_tail)
@@ -184,8 +185,9 @@ def _strides(t: torch.Tensor):
 
 def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, counts=None) -> None:
     """Append tokens ``key, value [B, Hkv, n, 128]`` (bf16) behind the ``start`` tokens each sequence holds (an int or an
-    int32 tensor ``[B]``; ``KV8Cache`` says how to drop tokens before); of a padded batch only the first ``counts[b]`` of the n.  One token and whole prompts take the
-    same call.  A block that fills is quantised from its 64 tokens' bf16 values.  Only the touched blocks are written."""
+    int32 tensor ``[B]``; ``KV8Cache`` says how to drop tokens before); of a padded batch only the first ``counts[b]`` of the
+    n.  One token and whole prompts take the same call.  A block that fills is quantised from its 64 tokens' bf16 values.  Only
+    the touched blocks are written."""
     key, value = _rows(key, "key", cache), _rows(value, "value", cache)
     _, h, n, _ = shape = key.shape
     if h != cache.kv_heads or shape != value.shape:
@@ -200,8 +202,8 @@ def kv8_store(cache: KV8Cache, key: torch.Tensor, value: torch.Tensor, start, co
 
 
 def kv8_load(cache: KV8Cache, lengths, first=0, count: int | None = None):
-    """Values of tokens ``first .. first + count`` (``count=None``, for an int ``first``: to the end of the capacity) as ``(k, v)``, bf16
-    ``[B, Hkv, count, 128]``; zeros outside ``[0, length)``.  ``lengths`` and ``first``: int or int32 tensor ``[B]``."""
+    """Values of tokens ``first .. first + count`` (``count=None``, for an int ``first``: to the end of the capacity) as
+    ``(k, v)``, bf16 ``[B, Hkv, count, 128]``; zeros outside ``[0, length)``.  ``lengths`` and ``first``: int or int32 tensor ``[B]``."""
     dev_n, n = _per_sequence(cache, lengths, "lengths", 0, cache.capacity)
     if count is None:
         if isinstance(first, torch.Tensor):
@@ -275,8 +277,8 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
     ``weights [B, Hkv, >= max_length]`` fp32 receives the attention weight of each token -- the probabilities summed over
     the head's queries -- plus ``add_to`` (``add_to=weights`` sums up in place); entries behind a sequence's length are
     left as they were.  It takes scratch memory of 4 bytes for every query row and token.
-    Forward only: a backward pass through it raises.  One to 24 rows per cache head (H / Hkv * S) and more take different kernels; both are within the
-    roundings of P to 16 bits of the exact result.
+    Forward only: a backward pass through it raises.  One to 24 rows per cache head (H / Hkv * S) and more take different
+    kernels; both are within the roundings of P to 16 bits of the exact result.
     """
     if query.requires_grad and torch.is_grad_enabled():
         return _ForwardOnly.apply(query, cache, lengths, max_length, sm_scale, weights, add_to, return_lse)
@@ -310,7 +312,8 @@ def kv8_attention(query: torch.Tensor, cache: KV8Cache, lengths, max_length: int
 def kv8_evict(cache: KV8Cache, lengths, weights: torch.Tensor, budget: int, recent: int, sink: int = 0,
               max_length: int | None = None, out: KV8Cache | None = None):
     """Keep ``budget`` tokens of every head: the first ``sink``, the last ``recent`` and those with the largest ``weights
-    [B, Hkv, >= max_length]`` (fp32, as ``kv8_attention`` sums them up) of the others; equal weights: the earlier token.
+    [B, Hkv, >= max_length]`` (fp32, as ``kv8_attention`` sums them up) of the others; equal weights: the earlier token, NaN
+    is the largest.
     Sequences of ``budget`` tokens or fewer are copied.
 
     Writes into ``out`` (another cache of the same type, batch and heads; a new one with room for ``budget`` tokens, which

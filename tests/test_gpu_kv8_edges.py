@@ -310,3 +310,22 @@ def test_a_long_prompt_of_another_scaling_needs_little_memory():
     # the smaller cache, 11 MB.  All query heads' logits would be 537 MB
     assert torch.cuda.max_memory_allocated() - base <= 192 << 20
     assert kv.held == 4096 and abs(kv.sums.sum().item() / 2048) <= 1 + 1e-5
+
+
+def test_going_back_by_a_smaller_length():
+    """To a multiple of 64, and inside the block that was incomplete, a smaller length is all it takes."""
+    from minference_b200 import kv8_store
+
+    gen = torch.Generator().manual_seed(13)
+    cache, ref = _filled(gen, 1, 2, [170], torch.float8_e4m3fn, capacity=320)
+    for kept in (169, 129, 128, 64):
+        cut = R.RefCache(1, 2, torch.float8_e4m3fn)
+        for name in ("k", "v"):
+            for h in range(2):
+                cut.raw[name][0][h] = ref.raw[name][0][h][:kept]
+        _check_attention(cache, cut, [kept], 1, 8, gen)
+    k, dk = _rows(gen, 1, 2, 80)
+    v, dv = _rows(gen, 1, 2, 80)
+    kv8_store(cache, dk, dv, 64)
+    cut.append(k, v)
+    _check_attention(cache, cut, [144], 1, 8, gen)
